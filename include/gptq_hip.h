@@ -315,6 +315,52 @@ int gptq_hip_qmatmul_grouped(void *stream, const void *x, int x_dtype, int64_t M
                              int64_t R, int64_t C, const void *zero, const void *scale, int zs_dtype,
                              int64_t group_size, int bits, int transpose_b, void *out, void *ws, size_t ws_bytes);
 
+/* ---- mixture of experts on packed weights -----------------------------------------------------
+ * No counterpart in the reference, whose packed product takes one matrix (op.py:19-69).
+ * A router gives each of `tokens` tokens top_k expert numbers; pair i = token * top_k + choice.  An id outside
+ * 0 .. n_experts - 1 marks a pair that goes nowhere.  Limits: 1 <= n_experts <= 1024, tokens < 2^24, at most 2^30
+ * pairs, rows of at most 2^25 elements.
+ *
+ * expert_sort: ids [pairs] of id_bytes bytes (4 or 8, signed) -> order [pairs], the pairs by expert, ties in order of
+ * the pair, those of nowhere last; position [pairs], its inverse; offsets [n_experts + 1], where each expert's rows
+ * begin and, last, where the rows of nowhere begin.  ws: gptq_hip_expert_sort_workspace_bytes (its contents need no
+ * preparation; calls that overlap in time need one each).
+ * expert_gather: out [tokens * top_k, K], row p = x[order[p] / top_k], zero for rows of nowhere.
+ * expert_combine: out[t] = sum_j weights[t, j] * y[position[t, j]], fp32 in order of j, rounded once; weights null:
+ * ones; pairs of nowhere are left out and their rows of y not read.  It is also the gradient of expert_gather.
+ * out_dtype: y_dtype, or any type where y is fp32.
+ * expert_combine_grad: dy [tokens * top_k, N] = weights * g, zero for rows of nowhere, and dw [tokens, top_k] =
+ * <g, y>, zero for pairs of nowhere, in w_dtype; either may be null; weights null: ones.
+ * The sums run in a fixed order: equal calls give equal bits. */
+size_t gptq_hip_expert_sort_workspace_bytes(int64_t pairs, int n_experts);
+int gptq_hip_expert_sort(void *stream, const void *ids, int id_bytes, int64_t pairs, int n_experts, int32_t *order,
+                         int32_t *position, int32_t *offsets, void *ws, size_t ws_bytes);
+int gptq_hip_expert_gather(void *stream, const void *x, int dtype, int64_t tokens, int top_k, int64_t K,
+                           const int32_t *position, const int32_t *offsets, int n_experts, void *out);
+int gptq_hip_expert_combine(void *stream, const void *y, int y_dtype, int64_t tokens, int top_k, int64_t N,
+                            const int32_t *position, const int32_t *offsets, int n_experts, const void *weights,
+                            int w_dtype, void *out, int out_dtype);
+int gptq_hip_expert_combine_grad(void *stream, const void *y, const void *g, int dtype, int64_t tokens, int top_k,
+                                 int64_t N, const int32_t *position, const int32_t *offsets, int n_experts,
+                                 const void *weights, int w_dtype, void *dy, void *dw);
+
+/* expert_qmatmul: every expert's rows times its packed matrix.  packed [n_experts, R, C] (bits 4: two rows of W a
+ * byte, bits 8: one), zero / scale [n_experts, C], or [n_experts, K / group_size, C] with group_size > 0 that divides
+ * K (and is even for 4 bits).  offsets: as expert_sort writes them.
+ *   transpose_b = 0: out [rows, C] = x @ W[e];  transpose_b = 1: out [rows, K] = x @ W[e]^T.
+ * order null: x holds the rows in sorted order (x_rows == rows); else row p is x[order[p] / top_k] and
+ * rows == x_rows * top_k.  Rows of nowhere give zeros and are not read.  Codes enter the products exactly, sums and
+ * scales are fp32, the result is rounded once to out_dtype (x_dtype or F32).  A row with an infinity or a NaN may be
+ * NaN throughout; other rows are untouched by it.  rows < 2^24, K <= 262140, C <= 2^20.
+ * ws: gptq_hip_expert_qmatmul_workspace_bytes (contents need no preparation; calls that overlap in time need one
+ * each). */
+size_t gptq_hip_expert_qmatmul_workspace_bytes(int64_t x_rows, int64_t rows, int64_t R, int64_t C, int bits,
+                                               int64_t group_size, int n_experts, int x_dtype, int transpose_b);
+int gptq_hip_expert_qmatmul(void *stream, const void *x, int x_dtype, int64_t x_rows, const int32_t *order, int top_k,
+                            int64_t rows, const int32_t *offsets, int n_experts, const uint8_t *packed, int64_t R,
+                            int64_t C, const void *zero, const void *scale, int zs_dtype, int64_t group_size, int bits,
+                            int transpose_b, void *out, int out_dtype, void *ws, size_t ws_bytes);
+
 /* ---- packed-int4 matmul that allocates nothing and takes no workspace ----------------------
  * No counterpart in the reference.  For callers that cannot allocate device memory: code under
  * HIP graph capture, tight serving loops, harnesses that forbid hipMalloc.  Same operation,

@@ -1,0 +1,16 @@
+// Arguments of the experts' product, shared by its kernels.
+#pragma once
+#include "common.h"
+
+struct ExpertArgs {
+  const void *x;
+  const uint8_t *packed;          // [E, R, C]
+  const void *zero, *scale;       // [E, C] or [E, K / group, C]
+  void *out;                      // [P, C], transposed [P, K]
+  const int *order;               // [P] pairs by expert, or null: the rows of x are in that order
+  const int *offsets;             // [E + 1]
+  int64_t T;                      // rows of x
+  int64_t P;                      // rows of the result
+  int64_t R, C, group;
+  int top_k, E, bits, x_dtype, zs_dtype, out_dtype, transpose;
+};

@@ -1,0 +1,157 @@
+// Rows of every expert times its packed matrix.
+//
+// E matrices W[e] [K, N], packed along K as for the single matrix (4 bits: byte [j, n] holds rows 2 j and 2 j + 1; 8
+// bits: one row a byte), with zero / scale [E, N] or, for groups of g input features, [E, K / g, N]:
+//   y[p, n]  = sum_k x[p, k] (c[k, n] - z[G(k), n]) s[G(k), n]      (transposed: x[p, n] summed over n)
+// Row p belongs to the expert e with offsets[e] <= p < offsets[e + 1]; rows from offsets[E] on are zero.  The row of x
+// is p itself or, with `order`, the token order[p] / top_k.
+#include "expert_qmm.h"
+
+namespace {
+
+// the expert of row p (E: none), by bisection
+__device__ __forceinline__ int expert_of(const int *__restrict__ offsets, int E, int64_t p) {
+  int lo = 0, hi = E;                       // offsets[lo] <= p is kept
+  if (p >= offsets[E]) return E;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (offsets[mid] <= p) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ int64_t x_row(const int *__restrict__ order, int top_k, int64_t T, int64_t p) {
+  if (!order) return p;
+  const int64_t t = order[p] / top_k;
+  return t < 0 ? 0 : (t < T ? t : T - 1);
+}
+
+template <int BITS>
+__device__ __forceinline__ float code_at(const uint8_t *__restrict__ w, int64_t C, int64_t k, int64_t n) {
+  if (BITS == 8) return (float)w[k * C + n];
+  const uint8_t b = w[(k >> 1) * C + n];
+  return (float)((k & 1) ? b >> 4 : b & 15);
+}
+
+// One thread per output.  The shapes that no tiled kernel takes: groups that are no multiple of 32 features.
+template <typename TX, typename TO, typename TZ, int BITS>
+__global__ __launch_bounds__(256) void simple_fwd_kernel(ExpertArgs a) {
+  const int64_t p = blockIdx.x;
+  const int64_t n = (int64_t)blockIdx.y * 256 + threadIdx.x;
+  if (n >= a.C) return;
+  const int e = expert_of(a.offsets, a.E, p);
+  TO *out = (TO *)a.out + p * a.C + n;
+  if (e == a.E) {
+    *out = from_f32<TO>(0.f);
+    return;
+  }
+  const int64_t K = BITS == 4 ? 2 * a.R : a.R, g = a.group ? a.group : K, tables = a.group ? K / a.group : 1;
+  const TX *x = (const TX *)a.x + x_row(a.order, a.top_k, a.T, p) * K;
+  const uint8_t *w = a.packed + (int64_t)e * a.R * a.C;
+  const TZ *zero = (const TZ *)a.zero + (int64_t)e * tables * a.C + n;
+  const TZ *scale = (const TZ *)a.scale + (int64_t)e * tables * a.C + n;
+  float total = 0.f;
+  const int64_t run = a.group ? a.group : 128;       // a long sum is made of short ones
+  for (int64_t k0 = 0; k0 < K; k0 += run) {
+    const float z = to_f32(zero[k0 / g * a.C]);
+    const int64_t k1 = k0 + run < K ? k0 + run : K;
+    float sum = 0.f;
+    for (int64_t k = k0; k < k1; ++k) sum = fmaf(to_f32(x[k]), code_at<BITS>(w, a.C, k, n) - z, sum);
+    total = fmaf(sum, to_f32(scale[k0 / g * a.C]), total);
+  }
+  *out = from_f32<TO>(total);
+}
+
+// One wavefront per output column of the transposed product (a row of W).
+template <typename TX, typename TO, typename TZ, int BITS>
+__global__ __launch_bounds__(256) void simple_bwd_kernel(ExpertArgs a) {
+  const int64_t p = blockIdx.x;
+  const int lane = threadIdx.x & 63;
+  const int64_t K = BITS == 4 ? 2 * a.R : a.R, k = (int64_t)blockIdx.y * 4 + (threadIdx.x >> 6);
+  if (k >= K) return;
+  const int e = expert_of(a.offsets, a.E, p);
+  TO *out = (TO *)a.out + p * K + k;
+  if (e == a.E) {
+    if (lane == 0) *out = from_f32<TO>(0.f);
+    return;
+  }
+  const int64_t g = a.group ? a.group : K, tables = a.group ? K / a.group : 1;
+  const TX *x = (const TX *)a.x + x_row(a.order, a.top_k, a.T, p) * a.C;
+  const uint8_t *w = a.packed + (int64_t)e * a.R * a.C;
+  const TZ *zero = (const TZ *)a.zero + ((int64_t)e * tables + k / g) * a.C;
+  const TZ *scale = (const TZ *)a.scale + ((int64_t)e * tables + k / g) * a.C;
+  float sum = 0.f;
+  for (int64_t n = lane; n < a.C; n += 64)
+    sum = fmaf(to_f32(x[n]) * to_f32(scale[n]), code_at<BITS>(w, a.C, k, n) - to_f32(zero[n]), sum);
+  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+  if (lane == 0) *out = from_f32<TO>(sum);
+}
+
+template <typename TX, typename TO, typename TZ, int BITS>
+static int simple_launch(hipStream_t s, const ExpertArgs &a) {
+  const int64_t K = BITS == 4 ? 2 * a.R : a.R;
+  if (a.transpose)
+    simple_bwd_kernel<TX, TO, TZ, BITS><<<dim3((unsigned)a.P, (unsigned)ceil_div64(K, 4)), 256, 0, s>>>(a);
+  else
+    simple_fwd_kernel<TX, TO, TZ, BITS><<<dim3((unsigned)a.P, (unsigned)ceil_div64(a.C, 256)), 256, 0, s>>>(a);
+  GPTQ_CHECK_LAUNCH();
+  return GPTQ_HIP_OK;
+}
+template <typename TX, typename TO>
+static int simple_tables(hipStream_t s, const ExpertArgs &a) {
+  if (a.zs_dtype == GPTQ_HIP_F32)
+    return a.bits == 4 ? simple_launch<TX, TO, float, 4>(s, a) : simple_launch<TX, TO, float, 8>(s, a);
+  if (a.zs_dtype == GPTQ_HIP_F16)
+    return a.bits == 4 ? simple_launch<TX, TO, __half, 4>(s, a) : simple_launch<TX, TO, __half, 8>(s, a);
+  return a.bits == 4 ? simple_launch<TX, TO, __hip_bfloat16, 4>(s, a)
+                     : simple_launch<TX, TO, __hip_bfloat16, 8>(s, a);
+}
+static int simple_run(hipStream_t s, const ExpertArgs &a) {
+  if (a.x_dtype == GPTQ_HIP_F32) return simple_tables<float, float>(s, a);
+  if (a.x_dtype == GPTQ_HIP_F16)
+    return a.out_dtype == GPTQ_HIP_F32 ? simple_tables<__half, float>(s, a) : simple_tables<__half, __half>(s, a);
+  return a.out_dtype == GPTQ_HIP_F32 ? simple_tables<__hip_bfloat16, float>(s, a)
+                                     : simple_tables<__hip_bfloat16, __hip_bfloat16>(s, a);
+}
+
+static bool float_type(int dt) { return dt == GPTQ_HIP_F32 || dt == GPTQ_HIP_F16 || dt == GPTQ_HIP_BF16; }
+
+// GPTQ_HIP_OK, or why the product is refused
+static int check_args(const ExpertArgs &a) {
+  if (a.bits != 4 && a.bits != 8) return GPTQ_HIP_EINVAL;
+  if (!float_type(a.x_dtype) || !float_type(a.out_dtype) || !float_type(a.zs_dtype)) return GPTQ_HIP_EDTYPE;
+  if (a.out_dtype != a.x_dtype && a.out_dtype != GPTQ_HIP_F32) return GPTQ_HIP_EDTYPE;
+  const int64_t lim = (int64_t)1 << 30;
+  if (a.E < 1 || a.E > 1024 || a.top_k < 1 || a.T < 0 || a.P < 0 || a.R < 1 || a.C < 1) return GPTQ_HIP_EINVAL;
+  // (the plain kernels have one workgroup of 256 threads per row and four output columns in a grid dimension)
+  if (a.P >= (int64_t)1 << 24 || a.R > lim || a.C > (int64_t)1 << 20 || a.T > lim) return GPTQ_HIP_EINVAL;
+  const int64_t K = a.bits == 4 ? 2 * a.R : a.R;
+  if (K > 262140) return GPTQ_HIP_EINVAL;
+  if (a.group < 0 || (a.group && (K % a.group || (a.bits == 4 && a.group % 2)))) return GPTQ_HIP_EINVAL;
+  if (a.order ? a.P != a.T * a.top_k : a.P != a.T) return GPTQ_HIP_EINVAL;
+  if (a.P == 0) return GPTQ_HIP_OK;
+  if (!a.x || !a.offsets || !a.packed || !a.zero || !a.scale || !a.out) return GPTQ_HIP_EINVAL;
+  return GPTQ_HIP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t gptq_hip_expert_qmatmul_workspace_bytes(int64_t x_rows, int64_t rows, int64_t R, int64_t C, int bits,
+                                               int64_t group_size, int n_experts, int x_dtype, int transpose_b) {
+  return 0;
+}
+
+int gptq_hip_expert_qmatmul(void *stream, const void *x, int x_dtype, int64_t x_rows, const int32_t *order, int top_k,
+                            int64_t rows, const int32_t *offsets, int n_experts, const uint8_t *packed, int64_t R,
+                            int64_t C, const void *zero, const void *scale, int zs_dtype, int64_t group_size, int bits,
+                            int transpose_b, void *out, int out_dtype, void *ws, size_t ws_bytes) {
+  const ExpertArgs a = {x, packed, zero, scale, out, order, offsets, x_rows, rows, R, C, group_size, top_k, n_experts,
+                        bits, x_dtype, zs_dtype, out_dtype, transpose_b ? 1 : 0};
+  if (int rc = check_args(a)) return rc;
+  if (a.P == 0) return GPTQ_HIP_OK;
+  return simple_run(as_stream(stream), a);
+}
+
+}  // extern "C"

@@ -7,9 +7,10 @@ and the operator in ``op`` (``from jax_gptq_amd.op import quantized_matmul``); `
 ``use_quantized`` are the callers of that path: the sequential calibration driver and the
 inference-time dispatch.
 """
-from . import gptq, op, utils  # noqa: F401  (submodules, as in the reference's layout)
+from . import experts, gptq, op, utils  # noqa: F401  (submodules, as in the reference's layout)
+from .experts import QuantizedExperts
 from .gptq import QuantizedMatrix
 from .quantize_interpreter import quantize
 from .transform import use_quantized
 
-__all__ = ["QuantizedMatrix", "gptq", "op", "utils", "quantize", "use_quantized"]
+__all__ = ["QuantizedExperts", "QuantizedMatrix", "experts", "gptq", "op", "utils", "quantize", "use_quantized"]

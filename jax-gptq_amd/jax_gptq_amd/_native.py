@@ -60,6 +60,15 @@ SIGNATURES = {
     "gptq_hip_dequant_grouped": (_i32, [_vp, _vp, _i64, _i64, _vp, _vp, _i32, _i64, _i32, _vp]),
     "gptq_hip_qmatmul_grouped": (_i32, [_vp, _vp, _i32, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _i64, _i32, _i32, _vp,
                                         _vp, _sz]),
+    "gptq_hip_expert_sort_workspace_bytes": (_sz, [_i64, _i32]),
+    "gptq_hip_expert_sort": (_i32, [_vp, _vp, _i32, _i64, _i32, _vp, _vp, _vp, _vp, _sz]),
+    "gptq_hip_expert_gather": (_i32, [_vp, _vp, _i32, _i64, _i32, _i64, _vp, _vp, _i32, _vp]),
+    "gptq_hip_expert_combine": (_i32, [_vp, _vp, _i32, _i64, _i32, _i64, _vp, _vp, _i32, _vp, _i32, _vp, _i32]),
+    "gptq_hip_expert_combine_grad": (_i32, [_vp, _vp, _vp, _i32, _i64, _i32, _i64, _vp, _vp, _i32, _vp, _i32, _vp,
+                                            _vp]),
+    "gptq_hip_expert_qmatmul_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i32, _i64, _i32, _i32, _i32]),
+    "gptq_hip_expert_qmatmul": (_i32, [_vp, _vp, _i32, _i64, _vp, _i32, _i64, _vp, _i32, _vp, _i64, _i64, _vp, _vp,
+                                       _i32, _i64, _i32, _i32, _vp, _i32, _vp, _sz]),
     "gptq_hip_qmatmul_static": (_i32, [_vp, _vp, _i32, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _i32, _vp]),
     "gptq_hip_qmatmul_plan_query": (_i32, [_i64, _i64, _i64, _i32, _i32, _i32, _i32, _i64, _i32, _vp]),
     "gptq_hip_qmatmul_kernel_name": (ctypes.c_char_p, [_i32]),
