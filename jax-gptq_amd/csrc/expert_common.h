@@ -1,0 +1,179 @@
+// Device parts the experts' product kernels share: operand types, codes as matrix-core operands, the tile of a workgroup.
+#pragma once
+#include "expert_qmm.h"
+
+namespace xqmm {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bfloat8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// loads of 4, 8, 16 bytes at any address that fits the element type
+struct __attribute__((packed, aligned(1))) U32u { uint32_t v; };
+struct __attribute__((packed, aligned(1))) U64u { uint32_t v[2]; };
+struct __attribute__((packed, aligned(2))) U128u { uint32_t v[4]; };
+__device__ __forceinline__ u32x4 load16(const void *p) {
+  const U128u r = *reinterpret_cast<const U128u *>(p);
+  return u32x4{r.v[0], r.v[1], r.v[2], r.v[3]};
+}
+
+// Operand types of the matrix cores for activations of type XT: fp16 as they are, bf16 as they are, fp32 as three
+// bf16 parts (truncated: 3 x 8 bits are all 24, so the parts add up to the value exactly).
+// Codes are exact in either: a 4-bit code sits in the mantissa under the exponent of 64 (fp16: 64 + c) or 128 (bf16:
+// 128 + c), and the offset leaves with the zero point; 8-bit codes, and codes against fp32 parts, where the offset
+// would cost bits of the sum, become c itself.  (The bits of a code are also the subnormal fp16 c 2^-24, one
+// instruction less; but sums of products with subnormals came out with errors of 1e-4 of their size, two thousand
+// times those of the same sums with 64 + c.)
+template <int XT> struct Op;
+template <> struct Op<GPTQ_HIP_F16> {
+  static constexpr int PARTS = 1;
+  static constexpr uint32_t ONE = 0x3C003C00u;
+  static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+  }
+};
+template <> struct Op<GPTQ_HIP_BF16> {
+  static constexpr int PARTS = 1;
+  static constexpr uint32_t ONE = 0x3F803F80u;
+  static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bfloat8, a), __builtin_bit_cast(bfloat8, b), c, 0, 0, 0);
+  }
+};
+template <> struct Op<GPTQ_HIP_F32> : Op<GPTQ_HIP_BF16> {
+  static constexpr int PARTS = 3;
+};
+
+// Packed rows of one k-step (32 input features) that a lane holds, and how their bytes become B operands.  Lane
+// (l16, g) owns features 8 g .. 8 g + 7 of the step: 4 packed rows of 4-bit codes, 8 of 8-bit codes.
+template <int XT, int BITS> struct Codes {
+  static constexpr int ROWS = BITS == 4 ? 4 : 8;
+  static constexpr bool CONVERT = XT == GPTQ_HIP_F32 || (XT == GPTQ_HIP_BF16 && BITS == 8);
+  static constexpr float OFFSET = (CONVERT || BITS == 8) ? 0.f : (XT == GPTQ_HIP_BF16 ? 128.f : 64.f);
+  // features in the order 0 2 1 3 4 6 5 7 (4-bit codes taken pairwise from two rows): the activations are dealt alike
+  static constexpr bool DEALT = BITS == 4 && !CONVERT;
+
+  static __device__ __forceinline__ uint32_t pair_f32(float a, float b) {      // {bf16(a), bf16(b)}, exact here
+    return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x07060302u);
+  }
+  static __device__ __forceinline__ float byte_f32(uint32_t w, int q) { return (float)((w >> (8 * q)) & 255u); }
+
+  // B operand of byte q (0 .. 3) of the dwords r[0 .. ROWS - 1]
+  static __device__ __forceinline__ u32x4 operand(const uint32_t *r, int q) {
+    u32x4 b;
+    if (CONVERT && BITS == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        b[i] = pair_f32(byte_f32(r[i] & 0x0F0F0F0Fu, q), byte_f32((r[i] >> 4) & 0x0F0F0F0Fu, q));
+    } else if (CONVERT) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) b[i] = pair_f32(byte_f32(r[2 * i], q), byte_f32(r[2 * i + 1], q));
+    } else if (BITS == 8) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t p = __builtin_amdgcn_perm(r[2 * i + 1], r[2 * i], 0x0C040C00u + 0x00010001u * q);
+        const half2 v = __builtin_bit_cast(half2, p | 0x64006400u) - half2{(_Float16)1024.f, (_Float16)1024.f};
+        b[i] = __builtin_bit_cast(uint32_t, v);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t p = __builtin_amdgcn_perm(r[2 * i + 1], r[2 * i], 0x0C040C00u + 0x00010001u * q);
+        if (XT == GPTQ_HIP_BF16) {
+          b[2 * i] = (p & 0x000F000Fu) | 0x43004300u;
+          b[2 * i + 1] = ((p >> 4) & 0x000F000Fu) | 0x43004300u;
+        } else {
+          b[2 * i] = ((p << 4) & 0x00F000F0u) | 0x54005400u;
+          b[2 * i + 1] = (p & 0x00F000F0u) | 0x54005400u;
+        }
+      }
+    }
+    return b;
+  }
+};
+
+// 8 activations in natural order -> the order of Codes::DEALT
+__device__ __forceinline__ u32x4 deal(u32x4 a) {
+  return u32x4{__builtin_amdgcn_perm(a[1], a[0], 0x05040100u), __builtin_amdgcn_perm(a[1], a[0], 0x07060302u),
+               __builtin_amdgcn_perm(a[3], a[2], 0x05040100u), __builtin_amdgcn_perm(a[3], a[2], 0x07060302u)};
+}
+
+// 8 fp32 values -> three operands of bf16 parts
+__device__ __forceinline__ void parts3(const u32x4 &lo4, const u32x4 &hi4, u32x4 *out) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t w[2] = {i < 2 ? lo4[2 * i] : hi4[2 * i - 4], i < 2 ? lo4[2 * i + 1] : hi4[2 * i - 3]};
+    uint32_t part[3][2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float v = __builtin_bit_cast(float, w[j]);
+      part[0][j] = w[j];
+      const float r1 = v - __builtin_bit_cast(float, w[j] & 0xFFFF0000u);
+      part[1][j] = __builtin_bit_cast(uint32_t, r1);
+      const float r2 = r1 - __builtin_bit_cast(float, part[1][j] & 0xFFFF0000u);
+      part[2][j] = __builtin_bit_cast(uint32_t, r2);
+    }
+#pragma unroll
+    for (int p = 0; p < 3; ++p) out[p][i] = __builtin_amdgcn_perm(part[p][1], part[p][0], 0x07060302u);
+  }
+}
+
+// Which rows a workgroup owns: tiles of H rows are counted expert by expert (the rows of nowhere as one more), and
+// tile number `tile` is found by a scan over the experts, 64 at a time.  Every wavefront does it for itself.
+struct Tile {
+  int expert, row0, rows;        // rows == 0: there is no such tile
+};
+__device__ __forceinline__ Tile find_tile(const int *__restrict__ offsets, int E, int P, int H, int tile) {
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int e0 = 0; e0 <= E; e0 += 64) {
+    const int e = e0 + lane;
+    int lo = 0, hi = 0;
+    if (e <= E) {
+      lo = offsets[e];
+      hi = e < E ? offsets[e + 1] : P;
+    }
+    const int n = (hi - lo + H - 1) / H;
+    int scan = n;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int up = __shfl_up(scan, d);
+      if (lane >= d) scan += up;
+    }
+    const uint64_t past = __ballot(before + scan > tile);
+    if (past) {
+      const int who = __ffsll((unsigned long long)past) - 1;
+      const int first = before + __shfl(scan - n, who);
+      const int l = __shfl(lo, who), h = __shfl(hi, who);
+      const int row0 = l + (tile - first) * H;
+      int rows = h - row0;
+      rows = rows < H ? rows : H;
+      return {__builtin_amdgcn_readfirstlane(e0 + who), __builtin_amdgcn_readfirstlane(row0),
+              __builtin_amdgcn_readfirstlane(rows)};
+    }
+    before += __shfl(scan, 63);
+  }
+  return {0, 0, 0};
+}
+// tiles there can be
+static inline int64_t tile_bound(int64_t P, int E, int H) { return P / H + (P < E + 1 ? P : E + 1); }
+
+// the row of x that row p reads
+__device__ __forceinline__ int64_t x_row_of(const int *__restrict__ order, int top_k, int64_t T, int64_t p) {
+  if (!order) return p;
+  const uint32_t t = (uint32_t)order[p] / (uint32_t)top_k;
+  return (int64_t)t < T ? t : T - 1;
+}
+
+template <int XT> struct Elem { typedef __half type; };
+template <> struct Elem<GPTQ_HIP_BF16> { typedef __hip_bfloat16 type; };
+template <> struct Elem<GPTQ_HIP_F32> { typedef float type; };
+
+template <int XT>
+__device__ __forceinline__ void store_out(void *out, bool f32, int64_t i, float v) {
+  if (f32) ((float *)out)[i] = v;
+  else ((typename Elem<XT>::type *)out)[i] = from_f32<typename Elem<XT>::type>(v);
+}
+
+}  // namespace xqmm

@@ -14,3 +14,8 @@ struct ExpertArgs {
   int64_t R, C, group;
   int top_k, E, bits, x_dtype, zs_dtype, out_dtype, transpose;
 };
+
+// rows of one expert by strips of channels (expert_strip.h), 16 * row_blocks rows at a time
+int expert_strip_f16(hipStream_t s, const ExpertArgs &a, int row_blocks);
+int expert_strip_bf16(hipStream_t s, const ExpertArgs &a, int row_blocks);
+int expert_strip_f32(hipStream_t s, const ExpertArgs &a, int row_blocks);

@@ -116,6 +116,11 @@ static int simple_run(hipStream_t s, const ExpertArgs &a) {
 
 static bool float_type(int dt) { return dt == GPTQ_HIP_F32 || dt == GPTQ_HIP_F16 || dt == GPTQ_HIP_BF16; }
 
+static int strip_run(hipStream_t s, const ExpertArgs &a, int row_blocks) {
+  if (a.x_dtype == GPTQ_HIP_F32) return expert_strip_f32(s, a, row_blocks);
+  return a.x_dtype == GPTQ_HIP_F16 ? expert_strip_f16(s, a, row_blocks) : expert_strip_bf16(s, a, row_blocks);
+}
+
 // GPTQ_HIP_OK, or why the product is refused
 static int check_args(const ExpertArgs &a) {
   if (a.bits != 4 && a.bits != 8) return GPTQ_HIP_EINVAL;
@@ -151,7 +156,10 @@ int gptq_hip_expert_qmatmul(void *stream, const void *x, int x_dtype, int64_t x_
                         bits, x_dtype, zs_dtype, out_dtype, transpose_b ? 1 : 0};
   if (int rc = check_args(a)) return rc;
   if (a.P == 0) return GPTQ_HIP_OK;
-  return simple_run(as_stream(stream), a);
+  hipStream_t s = as_stream(stream);
+  const bool matrix = (a.group == 0 || a.group % 32 == 0) && a.C >= 8;
+  if (matrix && !a.transpose && a.P <= 512 * a.E) return strip_run(s, a, a.P <= 12 * a.E ? 1 : 2);
+  return simple_run(s, a);
 }
 
 }  // extern "C"

@@ -346,11 +346,22 @@ def test_transposed_product_of_tokens(X, T, k, E, K, N, bits, group, dt):
     check_product(y, x[torch.tensor(order) // k], layer, offsets, transpose=True)
     g = torch.randn(T * k, K).to(TYPES[dt])
     (dx,) = torch.autograd.grad(y, xg, g.cuda())
-    dr = X.quantized_expert_matmul(g.cuda().float(), layer.stack, plan, sorted_rows=True)
-    want = X.combine_tokens(dr, plan).double().cpu()
-    size = X.combine_tokens(dr.abs(), plan).double().cpu()
-    # both sides carry the products' own error; what is compared is the sum over the copies and its one rounding
-    within(dx, want, half_step(want, x.dtype) + 2.0 ** -14 * size + 1e-6)
+    # the gradient is the untransposed product summed over a token's copies: every copy brings K 2^-24 of the norm of
+    # its terms (an error relative to the terms, not to their sum: a sum near zero keeps it) and 2^-23 of itself for
+    # its fp32 value and the addition
+    token = torch.tensor(order) // k
+    ref, tol = torch.zeros(T, N, dtype=torch.float64), torch.zeros(T, N, dtype=torch.float64)
+    for e in range(E):
+        a, b = offsets[e], offsets[e + 1]
+        if a == b:
+            continue
+        c, z, s = layer.parts(e)
+        gd = g[a:b].double()
+        one = gd @ ((c - z) * s)
+        ref.index_add_(0, token[a:b], one)
+        tol.index_add_(0, token[a:b], K * 2.0 ** -24 * (gd.square() @ ((c + 128 + z.abs()) * s).square()).sqrt()
+                       + 2.0 ** -23 * one.abs())
+    within(dx, ref, tol + half_step(ref, x.dtype))
 
 
 @pytest.mark.parametrize("T", [1, 9, 60, 200])
