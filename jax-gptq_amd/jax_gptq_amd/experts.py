@@ -19,12 +19,10 @@ that no eager graph still refers to.
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _native as N
-from .gptq import _DT, QuantizedMatrix, _dev, _float_dev, _ptr, gptq, pack_matrix
+from .gptq import _DT, QuantizedMatrix, _dev, _float_dev, gptq, pack_matrix
 
 __all__ = ["QuantizedExperts", "TokenPlan", "stack_experts", "gptq_experts", "sort_tokens", "gather_tokens",
            "combine_tokens", "quantized_expert_matmul"]
@@ -32,8 +30,19 @@ __all__ = ["QuantizedExperts", "TokenPlan", "stack_experts", "gptq_experts", "so
 MAX_EXPERTS = 1024
 
 
-def _stream_of(t):
-    return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+_raw_stream = torch._C._cuda_getCurrentRawStream       # (torch.cuda.current_stream builds an object: 2 us a call)
+
+
+def _launch(entry, device, what, *args):
+    """Calls a C entry point on ``device``'s current stream; pointers are passed as integers."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        code = entry(_raw_stream(index), *args)
+    else:
+        with torch.cuda.device(index):
+            code = entry(_raw_stream(index), *args)
+    if code:
+        N.check(code, what)
 
 
 def _on_device(t, like, what):
@@ -167,15 +176,14 @@ def sort_tokens(expert_ids, n_experts):
     if top_k == 0:
         raise ValueError("at least one choice per token")
     ids = ids.contiguous()
-    P = ids.numel()
+    P, device = ids.numel(), ids.device
     lib = N.load()
-    with torch.cuda.device(ids.device):
-        store = torch.empty(2 * P + n_experts + 1, dtype=torch.int32, device=ids.device)
-        order, position, offsets = store[:P], store[P:2 * P], store[2 * P:]
-        nbytes = lib.gptq_hip_expert_sort_workspace_bytes(P, n_experts)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=ids.device) if nbytes else None
-        N.check(lib.gptq_hip_expert_sort(_stream_of(ids), _ptr(ids), ids.element_size(), P, n_experts, _ptr(order),
-                                         _ptr(position), _ptr(offsets), _ptr(ws), nbytes), "expert_sort")
+    order, position, offsets = torch.empty(2 * P + n_experts + 1, dtype=torch.int32, device=device).split(
+        (P, P, n_experts + 1))
+    nbytes = lib.gptq_hip_expert_sort_workspace_bytes(P, n_experts)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    _launch(lib.gptq_hip_expert_sort, device, "expert_sort", ids.data_ptr(), ids.element_size(), P, n_experts,
+            order.data_ptr(), position.data_ptr(), offsets.data_ptr(), ws.data_ptr() if nbytes else None, nbytes)
     return TokenPlan(order, position, offsets, ids.shape[:-1], top_k, n_experts)
 
 
@@ -184,33 +192,33 @@ def _rows_of(x, rows, plan, what):
     if x.dim() < 2:
         raise ValueError(f"{what} must have at least 2 dimensions")
     x = _on_device(x, plan.order, what)
-    width = x.shape[-1]
+    shape = x.shape
+    width = shape[-1]
     if width == 0 or x.numel() != rows * width:
         raise ValueError(f"{what} has {x.numel() // max(width, 1)} rows of {width}, expected {rows}")
-    return x.reshape(rows, width)
+    return x if len(shape) == 2 else x.reshape(rows, width)
 
 
 def _combine_raw(y, plan, weights, out_dtype):
-    lib = N.load()
-    out = torch.empty((plan.n_tokens, y.shape[1]), dtype=out_dtype, device=y.device)
-    with torch.cuda.device(y.device):
-        N.check(lib.gptq_hip_expert_combine(_stream_of(y), _ptr(y), _DT[y.dtype], plan.n_tokens, plan.top_k,
-                                            y.shape[1], _ptr(plan.position), _ptr(plan.offsets), plan.n_experts,
-                                            _ptr(weights), _DT[weights.dtype] if weights is not None else N.F32,
-                                            _ptr(out), _DT[out_dtype]), "expert_combine")
+    width, device = y.shape[1], y.device
+    out = torch.empty((plan.n_tokens, width), dtype=out_dtype, device=device)
+    _launch(N.load().gptq_hip_expert_combine, device, "expert_combine", y.data_ptr(), _DT[y.dtype], plan.n_tokens,
+            plan.top_k, width, plan.position.data_ptr(), plan.offsets.data_ptr(), plan.n_experts,
+            None if weights is None else weights.data_ptr(), N.F32 if weights is None else _DT[weights.dtype],
+            out.data_ptr(), _DT[out_dtype])
     return out
 
 
 def _gather_raw(x, plan):
-    lib = N.load()
-    out = torch.empty((plan.n_rows, x.shape[1]), dtype=x.dtype, device=x.device)
-    with torch.cuda.device(x.device):
-        N.check(lib.gptq_hip_expert_gather(_stream_of(x), _ptr(x), _DT[x.dtype], plan.n_tokens, plan.top_k,
-                                           x.shape[1], _ptr(plan.position), _ptr(plan.offsets), plan.n_experts,
-                                           _ptr(out)), "expert_gather")
+    width, device = x.shape[1], x.device
+    out = torch.empty((plan.n_rows, width), dtype=x.dtype, device=device)
+    _launch(N.load().gptq_hip_expert_gather, device, "expert_gather", x.data_ptr(), _DT[x.dtype], plan.n_tokens,
+            plan.top_k, width, plan.position.data_ptr(), plan.offsets.data_ptr(), plan.n_experts, out.data_ptr())
     return out
 
 
+# The backward passes are launches that record nothing, so where a graph of the gradient itself is asked for (grad mode
+# is on in a backward pass then) they go through the differentiable operators instead.
 class _GatherFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, plan):
@@ -218,8 +226,9 @@ class _GatherFn(torch.autograd.Function):
         return _gather_raw(x, plan)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
+        if torch.is_grad_enabled():
+            return combine_tokens(g, ctx.plan).reshape(ctx.plan.n_tokens, -1), None
         return _combine_raw(g.contiguous(), ctx.plan, None, g.dtype), None
 
 
@@ -238,20 +247,32 @@ class _CombineFn(torch.autograd.Function):
         return _combine_raw(y, plan, weights, y.dtype)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         y, weights = ctx.saved_tensors
         plan = ctx.plan
+        if torch.is_grad_enabled():
+            return _combine_grad_graph(y, weights, g, plan) + (None,)
         g = g.contiguous()
         dy = torch.empty_like(y) if ctx.needs_input_grad[0] else None
-        dw = torch.empty_like(weights) if weights is not None and ctx.needs_input_grad[1] else None
-        lib = N.load()
-        with torch.cuda.device(y.device):
-            N.check(lib.gptq_hip_expert_combine_grad(
-                _stream_of(y), _ptr(y), _ptr(g), _DT[y.dtype], plan.n_tokens, plan.top_k, y.shape[1],
-                _ptr(plan.position), _ptr(plan.offsets), plan.n_experts, _ptr(weights),
-                _DT[weights.dtype] if weights is not None else N.F32, _ptr(dy), _ptr(dw)), "expert_combine_grad")
+        dw = torch.empty_like(weights) if ctx.needs_input_grad[1] else None
+        _launch(N.load().gptq_hip_expert_combine_grad, y.device, "expert_combine_grad", y.data_ptr(), g.data_ptr(),
+                _DT[y.dtype], plan.n_tokens, plan.top_k, y.shape[1], plan.position.data_ptr(),
+                plan.offsets.data_ptr(), plan.n_experts, None if weights is None else weights.data_ptr(),
+                N.F32 if weights is None else _DT[weights.dtype], None if dy is None else dy.data_ptr(),
+                None if dw is None else dw.data_ptr())
         return dy, dw, None
+
+
+def _combine_grad_graph(y, weights, g, plan):
+    """The gradients of ``combine_tokens`` as differentiable operations."""
+    rows = gather_tokens(g, plan)
+    if weights is None:
+        return rows, None
+    live = (torch.arange(plan.n_rows, device=y.device) < plan.offsets[-1])[:, None]
+    sorted_weights = weights.reshape(-1)[plan.order.long()][:, None].float()
+    dy = torch.where(live, rows.float() * sorted_weights, 0.0).to(y.dtype)
+    dots = torch.where(live, rows.float() * y.float(), 0.0).sum(dim=1)
+    return dy, dots[plan.position.long()].reshape(weights.shape).to(weights.dtype)
 
 
 def combine_tokens(y, plan, weights=None):
@@ -267,46 +288,42 @@ def combine_tokens(y, plan, weights=None):
         out = _CombineFn.apply(y, weights, plan)
     else:
         out = _combine_raw(y, plan, weights, y.dtype)
-    return out.reshape(plan.token_shape + (y.shape[1],))
+    return out if len(plan.token_shape) == 1 else out.reshape(plan.token_shape + (y.shape[1],))
 
 
-def _expert_matmul_raw(x, experts, plan, sorted_rows, transpose_b, out_dtype):
-    lib = N.load()
-    iw, zero, scale = experts
-    packed, bits, group = iw
+def _expert_matmul_raw(x, packed, zero, scale, bits, group, plan, sorted_rows, transpose_b, out_dtype):
+    lib, device = N.load(), x.device
     E, R, C = packed.shape
-    K = R * (8 // bits)
-    out = torch.empty((plan.n_rows, K if transpose_b else C), dtype=out_dtype, device=x.device)
-    with torch.cuda.device(x.device):
-        nbytes = lib.gptq_hip_expert_qmatmul_workspace_bytes(x.shape[0], plan.n_rows, R, C, bits, group, E,
-                                                             _DT[x.dtype], int(transpose_b))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-        N.check(lib.gptq_hip_expert_qmatmul(
-            _stream_of(x), _ptr(x), _DT[x.dtype], x.shape[0], _ptr(None if sorted_rows else plan.order), plan.top_k,
-            plan.n_rows, _ptr(plan.offsets), E, _ptr(packed), R, C, _ptr(zero), _ptr(scale), _DT[zero.dtype], group,
-            bits, int(transpose_b), _ptr(out), _DT[out_dtype], _ptr(ws), nbytes), "expert_qmatmul")
+    x_rows, x_dtype, n_rows = x.shape[0], _DT[x.dtype], plan.n_rows
+    out = torch.empty((n_rows, R * (8 // bits) if transpose_b else C), dtype=out_dtype, device=device)
+    nbytes = lib.gptq_hip_expert_qmatmul_workspace_bytes(x_rows, n_rows, R, C, bits, group, E, x_dtype, transpose_b)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    _launch(lib.gptq_hip_expert_qmatmul, device, "expert_qmatmul", x.data_ptr(), x_dtype, x_rows,
+            None if sorted_rows else plan.order.data_ptr(), plan.top_k, n_rows, plan.offsets.data_ptr(), E,
+            packed.data_ptr(), R, C, zero.data_ptr(), scale.data_ptr(), _DT[zero.dtype], group, bits, transpose_b,
+            out.data_ptr(), _DT[out_dtype], ws.data_ptr() if nbytes else None, nbytes)
     return out
 
 
 class _ExpertMatmulFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, packed, zero, scale, bits, group, plan, sorted_rows, transpose_b):
-        ctx.save_for_backward(packed, zero, scale)
-        ctx.rest = (bits, group, plan, sorted_rows, transpose_b)
-        return _expert_matmul_raw(x, ((packed, bits, group), zero, scale), plan, sorted_rows, transpose_b, x.dtype)
+    def forward(ctx, x, experts, packed, zero, scale, plan, sorted_rows, transpose_b):
+        ctx.rest = (experts, packed, zero, scale, plan, sorted_rows, transpose_b)
+        return _expert_matmul_raw(x, packed, zero, scale, experts.bits, experts.group_size, plan, sorted_rows,
+                                  transpose_b, x.dtype)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        packed, zero, scale = ctx.saved_tensors
-        bits, group, plan, sorted_rows, transpose_b = ctx.rest
-        experts = ((packed, bits, group), zero, scale)
+        experts, packed, zero, scale, plan, sorted_rows, transpose_b = ctx.rest
+        if torch.is_grad_enabled():
+            dx = quantized_expert_matmul(g, experts, plan, sorted_rows=True, transpose_b=not transpose_b)
+            return (dx if sorted_rows else combine_tokens(dx, plan).reshape(plan.n_tokens, -1),) + (None,) * 7
         # a token's copies are added up before the one rounding: their gradients travel in fp32
-        dx = _expert_matmul_raw(g.contiguous(), experts, plan, True, not transpose_b,
-                                g.dtype if sorted_rows else torch.float32)
+        dx = _expert_matmul_raw(g.contiguous(), packed, zero, scale, experts.bits, experts.group_size, plan, True,
+                                not transpose_b, g.dtype if sorted_rows else torch.float32)
         if not sorted_rows:
             dx = _combine_raw(dx, plan, None, g.dtype)
-        return (dx,) + (None,) * 8
+        return (dx,) + (None,) * 7
 
 
 def quantized_expert_matmul(x, experts, plan, sorted_rows=False, transpose_b=False):
@@ -323,17 +340,16 @@ def quantized_expert_matmul(x, experts, plan, sorted_rows=False, transpose_b=Fal
     if len(experts) != plan.n_experts:
         raise ValueError(f"{len(experts)} matrices for a plan of {plan.n_experts} experts")
     x = _rows_of(_float_tensor(x), plan.n_rows if sorted_rows else plan.n_tokens, plan, "x")
-    _, K, C = experts.shape
-    assert x.shape[1] == (C if transpose_b else K), f"Inner dim mismatch: {x.shape[1]} != {C if transpose_b else K}"
+    inner = experts.shape[2 if transpose_b else 1]
+    assert x.shape[1] == inner, f"Inner dim mismatch: {x.shape[1]} != {inner}"
     packed = _on_device(experts.int_weight, x, "int_weight")
     zero = _float_tensor(_on_device(experts.zero, x, "zero"))
     scale = _on_device(experts.scale, x, "scale")
     if scale.dtype != zero.dtype:
         scale = scale.to(zero.dtype)
     if x.requires_grad:
-        return _ExpertMatmulFn.apply(x, packed, zero, scale, experts.bits, experts.group_size, plan,
-                                     bool(sorted_rows), bool(transpose_b))
-    return _expert_matmul_raw(x, ((packed, experts.bits, experts.group_size), zero, scale), plan, bool(sorted_rows),
+        return _ExpertMatmulFn.apply(x, experts, packed, zero, scale, plan, bool(sorted_rows), bool(transpose_b))
+    return _expert_matmul_raw(x, packed, zero, scale, experts.bits, experts.group_size, plan, bool(sorted_rows),
                               bool(transpose_b), x.dtype)
 
 

@@ -587,6 +587,33 @@ def test_gradient_in_a_graph(X):
             assert torch.equal(a, b)
 
 
+def test_gradient_of_the_gradient(X):
+    """A graph of the gradient (create_graph) goes through the operators again; fp32 against the 64-bit block."""
+    E, k, K, H, T = 3, 2, 64, 96, 9
+    up, gate, down = Layer(X, 1, E, K, H, 4, 32), Layer(X, 2, E, K, H, 4, 32), Layer(X, 3, E, H, K, 4, 32)
+    ids = ids_of(4, T, k, E, 0.2)
+    x, w, g = torch.randn(T, K), torch.rand(T, k), torch.randn(T, K)
+
+    def second(block, x, w, g, ids):
+        out = block(x, ids, w)
+        dx, dw = torch.autograd.grad(out, (x, w), g, create_graph=True)
+        return torch.autograd.grad(dx.square().sum() + dw.square().sum(), (x, w))
+    got = second(lambda a, i, b: _block(X, a, up, gate, down, i, b), x.cuda().requires_grad_(),
+                 w.cuda().requires_grad_(), g.cuda(), ids.cuda())
+    ref = second(lambda a, i, b: _block_ref(a, up, gate, down, i, b), x.double().requires_grad_(),
+                 w.double().requires_grad_(), g.double(), ids)
+    for a, b in zip(got, ref):
+        assert (a.cpu().double() - b).abs().max() <= 2.0 ** -12 * b.abs().max()
+    # and the rows' own operators
+    plan = X.sort_tokens(ids.cuda(), E)
+    r = torch.randn(T, K).cuda().requires_grad_()
+    rows = X.gather_tokens(r, plan)
+    (d,) = torch.autograd.grad(rows.square().sum(), r, create_graph=True)
+    (dd,) = torch.autograd.grad(d.sum(), r)
+    live = torch.tensor([[float(0 <= int(i) < E) for i in row] for row in ids]).sum(1).cuda()
+    assert torch.allclose(dd, 2 * live[:, None].expand_as(dd))
+
+
 # ------------------------------------------------------------------------------------ the solve for a layer of experts
 @pytest.mark.parametrize("group", [None, 128])
 def test_gptq_experts(X, group):
