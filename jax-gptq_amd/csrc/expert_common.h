@@ -19,6 +19,18 @@ __device__ __forceinline__ u32x4 load16(const void *p) {
   return u32x4{r.v[0], r.v[1], r.v[2], r.v[3]};
 }
 
+__device__ __forceinline__ u32x4 load16u(const uint8_t *p) {
+  struct __attribute__((packed, aligned(1))) U128b { uint32_t v[4]; };
+  const U128b r = *reinterpret_cast<const U128b *>(p);
+  return u32x4{r.v[0], r.v[1], r.v[2], r.v[3]};
+}
+// one value of a scale or zero table
+__device__ __forceinline__ float table_value(const char *p, int dtype, int64_t i) {
+  if (dtype == GPTQ_HIP_F32) return ((const float *)p)[i];
+  if (dtype == GPTQ_HIP_F16) return __half2float(((const __half *)p)[i]);
+  return __bfloat162float(((const __hip_bfloat16 *)p)[i]);
+}
+
 // Operand types of the matrix cores for activations of type XT: fp16 as they are, bf16 as they are, fp32 as three
 // bf16 parts (truncated: 3 x 8 bits are all 24, so the parts add up to the value exactly).
 // Codes are exact in either: a 4-bit code sits in the mantissa under the exponent of 64 (fp16: 64 + c) or 128 (bf16:
@@ -156,6 +168,15 @@ __device__ __forceinline__ Tile find_tile(const int *__restrict__ offsets, int E
   }
   return {0, 0, 0};
 }
+// how many tiles there are
+__device__ __forceinline__ int count_tiles(const int *__restrict__ offsets, int E, int P, int H) {
+  const int lane = threadIdx.x & 63;
+  int n = 0;
+  for (int e = lane; e <= E; e += 64) n += ((e < E ? offsets[e + 1] : P) - offsets[e] + H - 1) / H;
+#pragma unroll
+  for (int d = 32; d; d >>= 1) n += __shfl_xor(n, d);
+  return __builtin_amdgcn_readfirstlane(n);
+}
 // tiles there can be
 static inline int64_t tile_bound(int64_t P, int E, int H) { return P / H + (P < E + 1 ? P : E + 1); }
 
@@ -174,6 +195,19 @@ template <int XT>
 __device__ __forceinline__ void store_out(void *out, bool f32, int64_t i, float v) {
   if (f32) ((float *)out)[i] = v;
   else ((typename Elem<XT>::type *)out)[i] = from_f32<typename Elem<XT>::type>(v);
+}
+
+// four neighbours of a row
+template <int XT>
+__device__ __forceinline__ void store4(void *out, bool f32, int64_t i, float a, float b, float c, float d) {
+  typedef typename Elem<XT>::type E;
+  if (f32) {
+    struct __attribute__((packed, aligned(4))) F4 { float v[4]; };
+    *reinterpret_cast<F4 *>((float *)out + i) = F4{{a, b, c, d}};
+  } else {
+    struct __attribute__((packed, aligned(sizeof(E)))) E4 { E v[4]; };
+    *reinterpret_cast<E4 *>((E *)out + i) = E4{{from_f32<E>(a), from_f32<E>(b), from_f32<E>(c), from_f32<E>(d)}};
+  }
 }
 
 }  // namespace xqmm

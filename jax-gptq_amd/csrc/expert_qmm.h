@@ -19,3 +19,7 @@ struct ExpertArgs {
 int expert_strip_f16(hipStream_t s, const ExpertArgs &a, int row_blocks);
 int expert_strip_bf16(hipStream_t s, const ExpertArgs &a, int row_blocks);
 int expert_strip_f32(hipStream_t s, const ExpertArgs &a, int row_blocks);
+// the same by tiles of 64 (row_blocks 4) or 128 (8) rows x 256 channels (expert_tile.h); ws: expert_tile_bytes
+int expert_tile_f16(hipStream_t s, const ExpertArgs &a, int row_blocks, void *ws);
+int expert_tile_bf16(hipStream_t s, const ExpertArgs &a, int row_blocks, void *ws);
+int expert_tile_f32(hipStream_t s, const ExpertArgs &a, int row_blocks, void *ws);

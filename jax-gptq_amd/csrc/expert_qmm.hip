@@ -5,7 +5,7 @@
 //   y[p, n]  = sum_k x[p, k] (c[k, n] - z[G(k), n]) s[G(k), n]      (transposed: x[p, n] summed over n)
 // Row p belongs to the expert e with offsets[e] <= p < offsets[e + 1]; rows from offsets[E] on are zero.  The row of x
 // is p itself or, with `order`, the token order[p] / top_k.
-#include "expert_qmm.h"
+#include "expert_tile.h"
 
 namespace {
 
@@ -121,6 +121,24 @@ static int strip_run(hipStream_t s, const ExpertArgs &a, int row_blocks) {
   return a.x_dtype == GPTQ_HIP_F16 ? expert_strip_f16(s, a, row_blocks) : expert_strip_bf16(s, a, row_blocks);
 }
 
+static int tile_run(hipStream_t s, const ExpertArgs &a, int row_blocks, void *ws) {
+  if (a.x_dtype == GPTQ_HIP_F32) return expert_tile_f32(s, a, row_blocks, ws);
+  return a.x_dtype == GPTQ_HIP_F16 ? expert_tile_f16(s, a, row_blocks, ws) : expert_tile_bf16(s, a, row_blocks, ws);
+}
+
+// Which kernel a product runs on.
+struct Choice {
+  enum Kind { SIMPLE, STRIP, TILE } kind;
+  int row_blocks;
+};
+static Choice choose(int64_t P, int E, int64_t C, int64_t group, int x_dtype, int transpose) {
+  if (transpose || (group && group % 32) || C < 8) return {Choice::SIMPLE, 0};
+  const int64_t rows = P / E;                   // of an expert, on average
+  if (rows <= 12) return {Choice::STRIP, 1};
+  if (rows <= 40 || C < 16) return P <= (int64_t)1 << 19 ? Choice{Choice::STRIP, 2} : Choice{Choice::SIMPLE, 0};
+  return {Choice::TILE, rows <= 96 || x_dtype == GPTQ_HIP_F32 ? 4 : 8};
+}
+
 // GPTQ_HIP_OK, or why the product is refused
 static int check_args(const ExpertArgs &a) {
   if (a.bits != 4 && a.bits != 8) return GPTQ_HIP_EINVAL;
@@ -145,7 +163,10 @@ extern "C" {
 
 size_t gptq_hip_expert_qmatmul_workspace_bytes(int64_t x_rows, int64_t rows, int64_t R, int64_t C, int bits,
                                                int64_t group_size, int n_experts, int x_dtype, int transpose_b) {
-  return 0;
+  if (n_experts < 1 || rows <= 0 || x_rows <= 0 || R <= 0 || group_size < 0) return 0;
+  const Choice c = choose(rows, n_experts, C, group_size, x_dtype, transpose_b);
+  if (c.kind != Choice::TILE) return 0;
+  return xqmm::staged_layout(x_rows, bits == 4 ? 2 * R : R, x_dtype, xqmm::tile_half(group_size)).bytes;
 }
 
 int gptq_hip_expert_qmatmul(void *stream, const void *x, int x_dtype, int64_t x_rows, const int32_t *order, int top_k,
@@ -157,8 +178,15 @@ int gptq_hip_expert_qmatmul(void *stream, const void *x, int x_dtype, int64_t x_
   if (int rc = check_args(a)) return rc;
   if (a.P == 0) return GPTQ_HIP_OK;
   hipStream_t s = as_stream(stream);
-  const bool matrix = (a.group == 0 || a.group % 32 == 0) && a.C >= 8;
-  if (matrix && !a.transpose && a.P <= 512 * a.E) return strip_run(s, a, a.P <= 12 * a.E ? 1 : 2);
+  const Choice c = choose(a.P, a.E, a.C, a.group, a.x_dtype, a.transpose);
+  if (c.kind == Choice::STRIP) return strip_run(s, a, c.row_blocks);
+  if (c.kind == Choice::TILE) {
+    if (!ws || ws_bytes < gptq_hip_expert_qmatmul_workspace_bytes(a.T, a.P, a.R, a.C, a.bits, a.group, a.E, a.x_dtype,
+                                                                  a.transpose))
+      return GPTQ_HIP_EWORKSPACE;
+    if ((uintptr_t)ws % 16) return GPTQ_HIP_EINVAL;
+    return tile_run(s, a, c.row_blocks, ws);
+  }
   return simple_run(s, a);
 }
 

@@ -182,7 +182,8 @@ __global__ __launch_bounds__(STRIP_WAVES * 64) void strip_kernel(ExpertArgs a) {
   using S = Strip<XT, BITS, ZB, KS, RB, CW>;
   constexpr int H = 16 * RB;
   __shared__ f32x4 red[STRIP_WAVES / 2][RB * CW][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15;
+  const int lane = threadIdx.x & 63, l16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Tile tile = find_tile(a.offsets, a.E, (int)a.P, H, blockIdx.y);
   if (tile.rows <= 0) return;
   const int64_t N = a.C, K = BITS == 4 ? 2 * a.R : a.R, n0 = (int64_t)blockIdx.x * 16 * CW;
