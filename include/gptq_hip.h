@@ -352,10 +352,12 @@ int gptq_hip_expert_combine_grad(void *stream, const void *y, const void *g, int
  * rows == x_rows * top_k.  Rows of nowhere give zeros and are not read.  Codes enter the products exactly, sums and
  * scales are fp32, the result is rounded once to out_dtype (x_dtype or F32).  A row with an infinity or a NaN may be
  * NaN throughout; other rows are untouched by it.  rows < 2^24, K <= 262140, C <= 2^20.
- * ws: gptq_hip_expert_qmatmul_workspace_bytes (contents need no preparation; calls that overlap in time need one
- * each). */
+ * ws, 16-byte aligned: gptq_hip_expert_qmatmul_workspace_bytes (contents need no preparation; calls that overlap in
+ * time need one each).  Plain kernels, an order of magnitude slower, take groups that are no multiple of 32, fewer
+ * than 8 channels (transposed: 16) and, transposed, an x that is not 16-byte aligned. */
 size_t gptq_hip_expert_qmatmul_workspace_bytes(int64_t x_rows, int64_t rows, int64_t R, int64_t C, int bits,
-                                               int64_t group_size, int n_experts, int x_dtype, int transpose_b);
+                                               int64_t group_size, int n_experts, int x_dtype, int zs_dtype,
+                                               int transpose_b);
 int gptq_hip_expert_qmatmul(void *stream, const void *x, int x_dtype, int64_t x_rows, const int32_t *order, int top_k,
                             int64_t rows, const int32_t *offsets, int n_experts, const uint8_t *packed, int64_t R,
                             int64_t C, const void *zero, const void *scale, int zs_dtype, int64_t group_size, int bits,

@@ -15,7 +15,8 @@ LIB = os.path.join(OUT_DIR, "libgptq_hip.so")
 SOURCES = ["api.hip", "codec.hip", "gemm_f32.hip", "gemm_f64.hip", "hessian.hip", "cholinv.hip", "solve.hip",
            "qmatmul.hip", "qmatmul_mid.hip", "qmatmul_reg.hip", "qmatmul_reg_bwd.hip", "qmatmul_wide.hip",
            "experts.hip", "expert_qmm.hip", "expert_strip_f16.hip", "expert_strip_bf16.hip", "expert_strip_f32.hip",
-           "expert_tile_f16.hip", "expert_tile_bf16.hip", "expert_tile_f32.hip"]
+           "expert_tile_f16.hip", "expert_tile_bf16.hip", "expert_tile_f32.hip", "expert_back_f16.hip", "expert_back_bf16.hip",
+           "expert_back_f32.hip"]
 FLAGS = ["-O3", "--offload-arch=gfx950", "-fPIC", "-std=c++17",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
          "-Wno-unused-result"]

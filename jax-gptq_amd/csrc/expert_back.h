@@ -1,0 +1,366 @@
+// The transposed product, the gradient of the activations: a workgroup computes 128 rows x 256 input features of one
+// expert, the contraction runs over the output channels n in stages.
+//
+//   y[p, k] = sum_n (x[p, n] s[G(k), n]) (o + c[k, n]) - sum_n (x[p, n] s[G(k), n]) (o + z[G(k), n])
+//
+// The scale varies along the contraction, so it goes to the activations: a = x s in fp32, cut to 16 bits and split
+// into two bf16 parts (fp32 activations: all 24 bits in three), which meet the exact codes in as many products; the
+// second sum is taken in fp32 over the very values that were multiplied.  The cut is 2^-16 of a term, far below the
+// rounding of a 16-bit result; one part of 8 or 11 bits would not be.
+// Bound by the matrix cores, two products per 16-bit operand pair, and by the instructions that make the parts: a
+// wavefront owns 64 rows x 128 features (one group of 128, or two or four smaller ones), so that the parts of its 64
+// rows are used for eight column blocks.  Rows, codes and tables travel to LDS without passing a register, several
+// stages deep, one barrier per stage, as in the untransposed tiles.
+#pragma once
+#include "expert_tile.h"
+
+namespace xqmm {
+
+// rows padded with zeros to whole stages, where they do not come that way
+template <typename U>
+__global__ __launch_bounds__(256) void pad_rows_kernel(const U *__restrict__ x, int64_t N, int64_t Np,
+                                                       U *__restrict__ out) {
+  const int64_t row = blockIdx.x;
+  for (int64_t n = threadIdx.x; n < Np; n += 256) out[row * Np + n] = n < N ? x[row * N + n] : U(0);
+}
+// 16-bit tables as fp32
+static __global__ __launch_bounds__(256) void widen_tables_kernel(const char *__restrict__ zero,
+                                                           const char *__restrict__ scale, int dtype, int64_t n,
+                                                           float *__restrict__ out) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  out[i] = table_value(zero, dtype, i);
+  out[n + i] = table_value(scale, dtype, i);
+}
+
+struct BackLayout {
+  bool pad, widen;
+  int64_t Np, tables;           // row pitch in elements; table elements of all experts
+  size_t tables_at, bytes;
+};
+static inline BackLayout back_layout(int64_t x_rows, int64_t R, int64_t N, int bits, int64_t group,
+                                     int E, int x_dtype, int zs_dtype) {
+  BackLayout l;
+  const int64_t K = bits == 4 ? 2 * R : R, size = x_dtype == GPTQ_HIP_F32 ? 4 : 2;
+  l.Np = round_up64(N, 64);
+  l.pad = l.Np != N;
+  l.widen = zs_dtype != GPTQ_HIP_F32;
+  l.tables = (int64_t)E * (group ? K / group : 1) * N;
+  l.tables_at = l.pad ? (size_t)round_up64(x_rows * l.Np * size, 256) : 0;
+  l.bytes = l.tables_at + (l.widen ? (size_t)round_up64(2 * l.tables * 4, 256) : 0);
+  return l;
+}
+
+struct BackArgs {
+  ExpertArgs a;
+  const char *x;                // rows of whole stages
+  const float *zero, *scale;
+  int64_t row_bytes;
+  int stages;
+};
+
+// NG: groups a wavefront's 128 features lie in
+template <int XT, int BITS, bool ALIGNED, int NG> struct BackShape {
+  static constexpr int WAVES = 4, THREADS = 256, BM = 128, BN = 256;
+  static constexpr int BK = XT == GPTQ_HIP_F32 ? 32 : 64;           // channels of a stage: 128 bytes of a row
+  static constexpr int STEPS = BK / 32;
+  static constexpr int PARTS = XT == GPTQ_HIP_F32 ? 3 : 2;
+  static constexpr int ROWS = BITS == 4 ? BN / 2 : BN;              // packed rows of the tile
+  static constexpr int TROWS = 2 * NG;                              // table rows of the tile
+  static constexpr int A = BM * 128, B = ROWS * BK, Z = TROWS * 256;
+  static constexpr int STAGE = A + B + 2 * Z;
+  static constexpr int STAGES = 3 * STAGE <= 80 * 1024 ? 3 : 2;     // two workgroups share a CU
+  static constexpr int LDS = STAGES * STAGE;
+  static constexpr int AI = A / 1024 / WAVES, BI = B / 1024 / WAVES, ZI = 2 * TROWS / WAVES;
+  static constexpr int LOADS = AI + BI + ZI;
+};
+
+template <int XT, int BITS, bool ALIGNED, int NG>
+__global__ __launch_bounds__(256, XT == GPTQ_HIP_F32 ? 1 : 2) void back_kernel(BackArgs t) {
+  using T = BackShape<XT, BITS, ALIGNED, NG>;
+  using O = Op<GPTQ_HIP_BF16>;
+  typedef __attribute__((address_space(3))) char lds_char;
+  constexpr bool CONVERT = XT == GPTQ_HIP_F32 || BITS == 8;         // codes as c itself, else as 128 + c
+  constexpr float OFFSET = CONVERT ? 0.f : 128.f;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const ExpertArgs &a = t.a;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave >> 1, wn = wave & 1;
+  const int64_t N = a.C, K = BITS == 4 ? 2 * a.R : a.R;
+  const bool f32 = a.out_dtype == GPTQ_HIP_F32;
+
+  // the tile, in the order of the untransposed tiles
+  const int row_tiles = count_tiles(a.offsets, a.E, (int)a.P, T::BM);
+  const int cols = (int)((K + T::BN - 1) / T::BN);
+  const int64_t total = (int64_t)row_tiles * cols, run = (total + 7) / 8;
+  const int64_t pos = blockIdx.x >> 3, item = (blockIdx.x & 7) * run + pos;
+  if (pos >= run || item >= total) return;
+  const int panel = (int)(item / ((int64_t)row_tiles * 4));
+  const int rest = (int)(item - (int64_t)panel * row_tiles * 4);
+  const int width = cols - 4 * panel < 4 ? cols - 4 * panel : 4;
+  const int64_t k0 = (int64_t)(4 * panel + rest % width) * T::BN;
+  const Tile tile = find_tile(a.offsets, a.E, (int)a.P, T::BM, rest / width);
+  if (tile.rows <= 0) return;
+  if (tile.expert == a.E) {                            // rows of nowhere
+    for (int i = threadIdx.x; i < tile.rows * T::BN; i += T::THREADS) {
+      const int64_t k = k0 + i % T::BN;
+      if (k < K) store_out<XT>(a.out, f32, (int64_t)(tile.row0 + i / T::BN) * K + k, 0.f);
+    }
+    return;
+  }
+
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_char *)lds;
+  const int64_t tables = a.group ? K / a.group : 1;
+  const uint8_t *packed = a.packed + (int64_t)tile.expert * a.R * N;
+  const int64_t r0 = BITS == 4 ? k0 / 2 : k0;
+
+  const char *arow[T::AI];
+#pragma unroll
+  for (int j = 0; j < T::AI; ++j) {
+    int m = 8 * (T::AI * wave + j) + (lane >> 3);
+    m = m < tile.rows ? m : tile.rows - 1;             // rows past the last repeat it and are not stored
+    arow[j] = t.x + x_row_of(a.order, a.top_k, a.T, tile.row0 + m) * t.row_bytes + ((lane & 7) ^ (lane >> 3)) * 16;
+  }
+  constexpr int CH = T::BK / 16;                       // 16-byte chunks of a packed row in a stage
+  const uint8_t *brow[T::BI];
+#pragma unroll
+  for (int j = 0; j < T::BI; ++j) {
+    int64_t r = r0 + (T::BI * wave + j) * (64 / CH) + lane / CH;
+    r = r < a.R ? r : a.R - 1;
+    brow[j] = packed + r * N;
+  }
+  const int bcol = 16 * (lane % CH);
+  const float *trow[T::ZI];
+#pragma unroll
+  for (int j = 0; j < T::ZI; ++j) {
+    const int i = T::ZI * wave + j, which = i / T::TROWS, g = i % T::TROWS;
+    int64_t row = 0;
+    if (a.group) {
+      row = (k0 + g * (128 / NG)) / a.group;
+      row = row < tables ? row : tables - 1;
+    }
+    trow[j] = (which ? t.scale : t.zero) + ((int64_t)tile.expert * tables + row) * N;
+  }
+  u32x4 breg[ALIGNED ? 1 : T::BI];
+
+  auto issue = [&](int stage, int slot) __attribute__((always_inline)) {
+    const uint32_t base = lds0 + slot * T::STAGE;
+    const int64_t n0 = (int64_t)stage * T::BK;
+#pragma unroll
+    for (int j = 0; j < T::AI; ++j)
+      to_lds_16(arow[j] + (int64_t)stage * 128, base + (T::AI * wave + j) * 1024);
+#pragma unroll
+    for (int j = 0; j < T::ZI; ++j) {
+      int64_t n = n0 + lane % T::BK;
+      n = n < N ? n : N - 1;                           // (past N the activations are zero)
+      to_lds_4(trow[j] + n, base + T::A + T::B + (T::ZI * wave + j) * 256);
+    }
+#pragma unroll
+    for (int j = 0; j < T::BI; ++j) {
+      int64_t n = n0 + bcol;
+      if constexpr (ALIGNED) {
+        n = n < N ? n : 0;
+        to_lds_16(brow[j] + n, base + T::A + (T::BI * wave + j) * 1024);
+      } else {
+        breg[j] = load_end16(brow[j], n, N);
+      }
+    }
+  };
+  auto land = [&](int slot) __attribute__((always_inline)) {
+    if constexpr (!ALIGNED) {
+#pragma unroll
+      for (int j = 0; j < T::BI; ++j)
+        *reinterpret_cast<u32x4 *>(lds + slot * T::STAGE + T::A + (T::BI * wave + j) * 1024 + lane * 16) = breg[j];
+    }
+  };
+
+  f32x4 acc[4][8];                                      // [row block][column block]
+  float sub[NG][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int c = 0; c < 8; ++c) acc[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int g = 0; g < NG; ++g) sub[g][i] = 0.f;
+  }
+
+  // Lane group g4 owns channels 16 g4 + 8 h .. + 7 of a stage of 64 in k-step h: 16 bytes of a packed row (stages of
+  // 32: channels 8 g4 .. + 7, 32 bytes of activations).
+  auto step = [&](const char *base, int h) __attribute__((always_inline)) {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      float z[8], s[8];
+      const char *zp = base + T::A + T::B + (wn * NG + g) * 256 + (T::BK == 64 ? (16 * g4 + 8 * h) : 8 * g4) * 4;
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        const f32x4 zv = *reinterpret_cast<const f32x4 *>(zp + 16 * v);
+        const f32x4 sv = *reinterpret_cast<const f32x4 *>(zp + T::Z + 16 * v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { z[4 * v + i] = zv[i] + OFFSET; s[4 * v + i] = sv[i]; }
+      }
+      u32x4 x[4][T::PARTS];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const char *row = base + (wm * 64 + 16 * i + l16) * 128;
+        float v[8];
+        if constexpr (XT == GPTQ_HIP_F32) {
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const f32x4 q = *reinterpret_cast<const f32x4 *>(row + ((2 * g4 + w) ^ (l16 & 7)) * 16);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[4 * w + e] = q[e];
+          }
+        } else {
+          const u32x4 q = *reinterpret_cast<const u32x4 *>(row + ((2 * g4 + h) ^ (l16 & 7)) * 16);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t w = q[e / 2];
+            const uint32_t half = (e & 1) ? w >> 16 : w & 0xFFFFu;
+            if (XT == GPTQ_HIP_BF16) v[e] = __builtin_bit_cast(float, (e & 1) ? w & 0xFFFF0000u : w << 16);
+            else v[e] = (float)__builtin_bit_cast(_Float16, (uint16_t)half);
+          }
+        }
+        uint32_t part[T::PARTS][8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float p = v[e] * s[e];
+          if (T::PARTS == 2) p = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, p) & 0xFFFFFF00u);
+          sub[g][i] = fmaf(p, z[e], sub[g][i]);
+          part[0][e] = __builtin_bit_cast(uint32_t, p);
+#pragma unroll
+          for (int c = 1; c < T::PARTS; ++c) {
+            p -= __builtin_bit_cast(float, part[c - 1][e] & 0xFFFF0000u);
+            part[c][e] = __builtin_bit_cast(uint32_t, p);
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < T::PARTS; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            x[i][c][e] = __builtin_amdgcn_perm(part[c][2 * e + 1], part[c][2 * e], 0x07060302u);
+      }
+      constexpr int RBS = (BITS == 4 ? 4 : 8) / NG;     // blocks of 16 packed rows
+#pragma unroll
+      for (int b = 0; b < RBS; ++b) {
+        const int row = wn * (T::ROWS / 2) + 16 * (g * RBS + b) + l16;
+        const uint2 w = *reinterpret_cast<const uint2 *>(base + T::A + row * T::BK +
+                                                         (T::BK == 64 ? 16 * g4 + 8 * h : 8 * g4));
+        constexpr int CB = BITS == 4 ? 2 : 1;
+        u32x4 op[CB];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t d = j < 2 ? w.x : w.y;
+          const int q = 2 * (j & 1);
+          if constexpr (CONVERT && BITS == 4) {
+            const uint32_t lo = d & 0x0F0F0F0Fu, hi = (d >> 4) & 0x0F0F0F0Fu;
+            op[0][j] = Codes<XT, BITS>::pair_f32(Codes<XT, BITS>::byte_f32(lo, q), Codes<XT, BITS>::byte_f32(lo, q + 1));
+            op[CB - 1][j] = Codes<XT, BITS>::pair_f32(Codes<XT, BITS>::byte_f32(hi, q), Codes<XT, BITS>::byte_f32(hi, q + 1));
+          } else if constexpr (CONVERT) {
+            op[0][j] = Codes<XT, BITS>::pair_f32(Codes<XT, BITS>::byte_f32(d, q), Codes<XT, BITS>::byte_f32(d, q + 1));
+          } else {
+            const uint32_t p = __builtin_amdgcn_perm(0u, d, q ? 0x0C030C02u : 0x0C010C00u);
+            op[0][j] = (p & 0x000F000Fu) | 0x43004300u;
+            op[CB - 1][j] = ((p >> 4) & 0x000F000Fu) | 0x43004300u;
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < CB; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int p = 0; p < T::PARTS; ++p) {
+              f32x4 &d = acc[i][(g * RBS + b) * CB + c];
+              d = O::mma(x[i][p], op[c], d);
+            }
+      }
+      // (one group's parts at a time: with those of the next made early the registers do not suffice)
+      if (NG > 1) __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  constexpr int AHEAD = T::STAGES - 1;
+#pragma unroll
+  for (int s = 0; s < AHEAD; ++s) {
+    issue(s < t.stages ? s : t.stages - 1, s);
+    land(s);
+  }
+  int slot = 0, into = AHEAD;
+  for (int s = 0; s < t.stages; ++s) {
+    wait_and_meet<ALIGNED ? (AHEAD - 1) * T::LOADS : 0>();
+    issue(s + AHEAD < t.stages ? s + AHEAD : t.stages - 1, into);
+    const char *base = lds + slot * T::STAGE;
+#pragma unroll
+    for (int h = 0; h < T::STEPS; ++h) step(base, h);
+    land(into);
+    slot = slot + 1 == T::STAGES ? 0 : slot + 1;
+    into = into + 1 == T::STAGES ? 0 : into + 1;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // no load may reach LDS after this workgroup's end
+
+  // the second sum lies with row l16 of each block, spread over the lane groups; results lie with rows 4 g4 + r
+#pragma unroll
+  for (int g = 0; g < NG; ++g)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      sub[g][i] += __shfl_xor(sub[g][i], 16);
+      sub[g][i] += __shfl_xor(sub[g][i], 32);
+    }
+  constexpr int CB = BITS == 4 ? 2 : 1, PERG = 8 / NG;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int m = wm * 64 + 16 * i + 4 * g4 + r;
+#pragma unroll
+      for (int c = 0; c < 8; c += CB) {
+        const float d = __shfl(sub[c / PERG][i], 4 * g4 + r);
+        const int64_t k = k0 + wn * 128 + 16 * c + CB * l16;
+        if (m >= tile.rows) continue;
+#pragma unroll
+        for (int j = 0; j < CB; ++j)
+          if (k + j < K) store_out<XT>(a.out, f32, (int64_t)(tile.row0 + m) * K + k + j, acc[i][c + j][r] - d);
+      }
+    }
+}
+
+template <int XT, int BITS, bool ALIGNED, int NG> static int back_one(hipStream_t s, const BackArgs &t) {
+  using T = BackShape<XT, BITS, ALIGNED, NG>;
+  const int64_t K = BITS == 4 ? 2 * t.a.R : t.a.R;
+  const int64_t blocks = round_up64(tile_bound(t.a.P, t.a.E, T::BM) * ceil_div64(K, T::BN), 8);
+  if (blocks * T::THREADS >= (int64_t)1 << 32) return GPTQ_HIP_EINVAL;
+  if (!gptq_raise_lds_limit((const void *)back_kernel<XT, BITS, ALIGNED, NG>, T::LDS)) return GPTQ_HIP_ELAUNCH;
+  back_kernel<XT, BITS, ALIGNED, NG><<<(unsigned)blocks, T::THREADS, T::LDS, s>>>(t);
+  GPTQ_CHECK_LAUNCH();
+  return GPTQ_HIP_OK;
+}
+template <int XT, int BITS, bool ALIGNED> static int back_groups(hipStream_t s, const BackArgs &t) {
+  if (t.a.group % 128 == 0) return back_one<XT, BITS, ALIGNED, 1>(s, t);
+  return t.a.group % 64 == 0 ? back_one<XT, BITS, ALIGNED, 2>(s, t) : back_one<XT, BITS, ALIGNED, 4>(s, t);
+}
+
+template <int XT> static int back_launch(hipStream_t s, const ExpertArgs &a, void *ws) {
+  const BackLayout l = back_layout(a.T, a.R, a.C, a.bits, a.group, a.E, a.x_dtype, a.zs_dtype);
+  constexpr int SZ = XT == GPTQ_HIP_F32 ? 4 : 2;
+  BackArgs t = {a, (const char *)a.x, (const float *)a.zero, (const float *)a.scale, l.Np * SZ,
+                (int)(l.Np * SZ / 128)};
+  if (l.pad) {
+    typedef typename std::conditional<SZ == 4, uint32_t, uint16_t>::type U;
+    pad_rows_kernel<U><<<(unsigned)a.T, 256, 0, s>>>((const U *)a.x, a.C, l.Np, (U *)ws);
+    GPTQ_CHECK_LAUNCH();
+    t.x = (const char *)ws;
+  }
+  if (l.widen) {
+    float *f = (float *)((char *)ws + l.tables_at);
+    widen_tables_kernel<<<(unsigned)ceil_div64(l.tables, 256), 256, 0, s>>>((const char *)a.zero, (const char *)a.scale,
+                                                                            a.zs_dtype, l.tables, f);
+    GPTQ_CHECK_LAUNCH();
+    t.zero = f;
+    t.scale = f + l.tables;
+  }
+  if (a.C % 16 == 0 && (uintptr_t)a.packed % 16 == 0)
+    return a.bits == 4 ? back_groups<XT, 4, true>(s, t) : back_groups<XT, 8, true>(s, t);
+  return a.bits == 4 ? back_groups<XT, 4, false>(s, t) : back_groups<XT, 8, false>(s, t);
+}
+
+}  // namespace xqmm

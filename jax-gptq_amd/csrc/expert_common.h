@@ -1,6 +1,7 @@
 // Device parts the experts' product kernels share: operand types, codes as matrix-core operands, the tile of a workgroup.
 #pragma once
 #include "expert_qmm.h"
+#include <type_traits>
 
 namespace xqmm {
 
@@ -23,6 +24,22 @@ __device__ __forceinline__ u32x4 load16u(const uint8_t *p) {
   struct __attribute__((packed, aligned(1))) U128b { uint32_t v[4]; };
   const U128b r = *reinterpret_cast<const U128b *>(p);
   return u32x4{r.v[0], r.v[1], r.v[2], r.v[3]};
+}
+// bytes n .. n + 15 of a row of N >= 16; past the row's end any bytes of it (its last 16, moved into place)
+__device__ __forceinline__ u32x4 load_end16(const uint8_t *row, int64_t n, int64_t N) {
+  if (n + 16 <= N) return load16u(row + n);
+  const int64_t over = n - (N - 16);
+  const u32x4 v = load16u(row + N - 16);
+  uint64_t lo = (uint64_t)v[1] << 32 | v[0], hi = (uint64_t)v[3] << 32 | v[2];
+  const int sh = (int)(over < 16 ? over : 15) * 8;
+  if (sh >= 64) {
+    lo = hi >> (sh - 64);
+    hi = 0;
+  } else if (sh > 0) {
+    lo = lo >> sh | hi << (64 - sh);
+    hi >>= sh;
+  }
+  return u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
 }
 // one value of a scale or zero table
 __device__ __forceinline__ float table_value(const char *p, int dtype, int64_t i) {

@@ -23,3 +23,7 @@ int expert_strip_f32(hipStream_t s, const ExpertArgs &a, int row_blocks);
 int expert_tile_f16(hipStream_t s, const ExpertArgs &a, int row_blocks, void *ws);
 int expert_tile_bf16(hipStream_t s, const ExpertArgs &a, int row_blocks, void *ws);
 int expert_tile_f32(hipStream_t s, const ExpertArgs &a, int row_blocks, void *ws);
+// the transposed product by tiles of 128 rows x 256 input features (expert_back.h)
+int expert_back_f16(hipStream_t s, const ExpertArgs &a, void *ws);
+int expert_back_bf16(hipStream_t s, const ExpertArgs &a, void *ws);
+int expert_back_f32(hipStream_t s, const ExpertArgs &a, void *ws);

@@ -5,7 +5,7 @@
 //   y[p, n]  = sum_k x[p, k] (c[k, n] - z[G(k), n]) s[G(k), n]      (transposed: x[p, n] summed over n)
 // Row p belongs to the expert e with offsets[e] <= p < offsets[e + 1]; rows from offsets[E] on are zero.  The row of x
 // is p itself or, with `order`, the token order[p] / top_k.
-#include "expert_tile.h"
+#include "expert_back.h"
 
 namespace {
 
@@ -126,13 +126,19 @@ static int tile_run(hipStream_t s, const ExpertArgs &a, int row_blocks, void *ws
   return a.x_dtype == GPTQ_HIP_F16 ? expert_tile_f16(s, a, row_blocks, ws) : expert_tile_bf16(s, a, row_blocks, ws);
 }
 
+static int back_run(hipStream_t s, const ExpertArgs &a, void *ws) {
+  if (a.x_dtype == GPTQ_HIP_F32) return expert_back_f32(s, a, ws);
+  return a.x_dtype == GPTQ_HIP_F16 ? expert_back_f16(s, a, ws) : expert_back_bf16(s, a, ws);
+}
+
 // Which kernel a product runs on.
 struct Choice {
-  enum Kind { SIMPLE, STRIP, TILE } kind;
+  enum Kind { SIMPLE, STRIP, TILE, BACK } kind;
   int row_blocks;
 };
 static Choice choose(int64_t P, int E, int64_t C, int64_t group, int x_dtype, int transpose) {
-  if (transpose || (group && group % 32) || C < 8) return {Choice::SIMPLE, 0};
+  if ((group && group % 32) || C < (transpose ? 16 : 8)) return {Choice::SIMPLE, 0};
+  if (transpose) return {Choice::BACK, 8};
   const int64_t rows = P / E;                   // of an expert, on average
   if (rows <= 12) return {Choice::STRIP, 1};
   if (rows <= 40 || C < 16) return P <= (int64_t)1 << 19 ? Choice{Choice::STRIP, 2} : Choice{Choice::SIMPLE, 0};
@@ -162,11 +168,15 @@ static int check_args(const ExpertArgs &a) {
 extern "C" {
 
 size_t gptq_hip_expert_qmatmul_workspace_bytes(int64_t x_rows, int64_t rows, int64_t R, int64_t C, int bits,
-                                               int64_t group_size, int n_experts, int x_dtype, int transpose_b) {
-  if (n_experts < 1 || rows <= 0 || x_rows <= 0 || R <= 0 || group_size < 0) return 0;
+                                               int64_t group_size, int n_experts, int x_dtype, int zs_dtype,
+                                               int transpose_b) {
+  if (n_experts < 1 || rows <= 0 || x_rows <= 0 || R <= 0 || C <= 0 || group_size < 0) return 0;
   const Choice c = choose(rows, n_experts, C, group_size, x_dtype, transpose_b);
-  if (c.kind != Choice::TILE) return 0;
-  return xqmm::staged_layout(x_rows, bits == 4 ? 2 * R : R, x_dtype, xqmm::tile_half(group_size)).bytes;
+  if (c.kind == Choice::TILE)
+    return xqmm::staged_layout(x_rows, bits == 4 ? 2 * R : R, x_dtype, xqmm::tile_half(group_size)).bytes;
+  if (c.kind == Choice::BACK)
+    return xqmm::back_layout(x_rows, R, C, bits, group_size, n_experts, x_dtype, zs_dtype).bytes;
+  return 0;
 }
 
 int gptq_hip_expert_qmatmul(void *stream, const void *x, int x_dtype, int64_t x_rows, const int32_t *order, int top_k,
@@ -180,13 +190,12 @@ int gptq_hip_expert_qmatmul(void *stream, const void *x, int x_dtype, int64_t x_
   hipStream_t s = as_stream(stream);
   const Choice c = choose(a.P, a.E, a.C, a.group, a.x_dtype, a.transpose);
   if (c.kind == Choice::STRIP) return strip_run(s, a, c.row_blocks);
-  if (c.kind == Choice::TILE) {
-    if (!ws || ws_bytes < gptq_hip_expert_qmatmul_workspace_bytes(a.T, a.P, a.R, a.C, a.bits, a.group, a.E, a.x_dtype,
-                                                                  a.transpose))
-      return GPTQ_HIP_EWORKSPACE;
-    if ((uintptr_t)ws % 16) return GPTQ_HIP_EINVAL;
-    return tile_run(s, a, c.row_blocks, ws);
-  }
+  const size_t need = gptq_hip_expert_qmatmul_workspace_bytes(a.T, a.P, a.R, a.C, a.bits, a.group, a.E, a.x_dtype,
+                                                              a.zs_dtype, a.transpose);
+  if (need && (!ws || ws_bytes < need)) return GPTQ_HIP_EWORKSPACE;
+  if (need && (uintptr_t)ws % 16) return GPTQ_HIP_EINVAL;
+  if (c.kind == Choice::TILE) return tile_run(s, a, c.row_blocks, ws);
+  if (c.kind == Choice::BACK && (uintptr_t)a.x % 16 == 0) return back_run(s, a, ws);
   return simple_run(s, a);
 }
 

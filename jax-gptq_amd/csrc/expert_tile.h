@@ -239,16 +239,8 @@ __global__ __launch_bounds__(256 * WM, 2) void tile_kernel(TileArgs t) {
       if constexpr (ZL) {
         n = n < N ? n : 0;
         to_lds_16(packed + r * N + n, base + T::A + i * 1024);
-      } else if (n + 16 <= N) {
-        breg[j] = load16u(packed + r * N + n);
-      } else {                                         // the row's end: its last 16 bytes, moved into place
-        const int64_t over = n - (N - 16);
-        const u32x4 v = load16u(packed + r * N + N - 16);
-        uint64_t lo = (uint64_t)v[1] << 32 | v[0], hi = (uint64_t)v[3] << 32 | v[2];
-        const int sh = (int)(over < 16 ? over : 15) * 8;
-        if (sh >= 64) { lo = hi >> (sh - 64); hi = 0; }
-        else if (sh > 0) { lo = lo >> sh | hi << (64 - sh); hi >>= sh; }
-        breg[j] = u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+      } else {
+        breg[j] = load_end16(packed + r * N, n, N);
       }
     }
 #pragma unroll

@@ -66,7 +66,7 @@ SIGNATURES = {
     "gptq_hip_expert_combine": (_i32, [_vp, _vp, _i32, _i64, _i32, _i64, _vp, _vp, _i32, _vp, _i32, _vp, _i32]),
     "gptq_hip_expert_combine_grad": (_i32, [_vp, _vp, _vp, _i32, _i64, _i32, _i64, _vp, _vp, _i32, _vp, _i32, _vp,
                                             _vp]),
-    "gptq_hip_expert_qmatmul_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i32, _i64, _i32, _i32, _i32]),
+    "gptq_hip_expert_qmatmul_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i32, _i64, _i32, _i32, _i32, _i32]),
     "gptq_hip_expert_qmatmul": (_i32, [_vp, _vp, _i32, _i64, _vp, _i32, _i64, _vp, _i32, _vp, _i64, _i64, _vp, _vp,
                                        _i32, _i64, _i32, _i32, _vp, _i32, _vp, _sz]),
     "gptq_hip_qmatmul_static": (_i32, [_vp, _vp, _i32, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _i32, _vp]),

@@ -296,7 +296,10 @@ def _expert_matmul_raw(x, packed, zero, scale, bits, group, plan, sorted_rows, t
     E, R, C = packed.shape
     x_rows, x_dtype, n_rows = x.shape[0], _DT[x.dtype], plan.n_rows
     out = torch.empty((n_rows, R * (8 // bits) if transpose_b else C), dtype=out_dtype, device=device)
-    nbytes = lib.gptq_hip_expert_qmatmul_workspace_bytes(x_rows, n_rows, R, C, bits, group, E, x_dtype, transpose_b)
+    if transpose_b and x.data_ptr() % 16:
+        x = x.clone()           # (the transposed kernels load 16 bytes at a time)
+    nbytes = lib.gptq_hip_expert_qmatmul_workspace_bytes(x_rows, n_rows, R, C, bits, group, E, x_dtype, _DT[zero.dtype],
+                                                         transpose_b)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     _launch(lib.gptq_hip_expert_qmatmul, device, "expert_qmatmul", x.data_ptr(), x_dtype, x_rows,
             None if sorted_rows else plan.order.data_ptr(), plan.top_k, n_rows, plan.offsets.data_ptr(), E,
