@@ -248,6 +248,7 @@ __global__ __launch_bounds__(256, XT == GPTQ_HIP_F32 ? 1 : 2) void back_kernel(B
                                                          (T::BK == 64 ? 16 * g4 + 8 * h : 8 * g4));
         constexpr int CB = BITS == 4 ? 2 : 1;
         u32x4 op[CB];
+        const uint32_t bias = opaque(0x43004300u);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t d = j < 2 ? w.x : w.y;
@@ -260,8 +261,8 @@ __global__ __launch_bounds__(256, XT == GPTQ_HIP_F32 ? 1 : 2) void back_kernel(B
             op[0][j] = Codes<XT, BITS>::pair_f32(Codes<XT, BITS>::byte_f32(d, q), Codes<XT, BITS>::byte_f32(d, q + 1));
           } else {
             const uint32_t p = __builtin_amdgcn_perm(0u, d, q ? 0x0C030C02u : 0x0C010C00u);
-            op[0][j] = (p & 0x000F000Fu) | 0x43004300u;
-            op[CB - 1][j] = ((p >> 4) & 0x000F000Fu) | 0x43004300u;
+            op[0][j] = (p & 0x000F000Fu) | bias;
+            op[CB - 1][j] = ((p >> 4) & 0x000F000Fu) | bias;
           }
         }
 #pragma unroll

@@ -74,6 +74,13 @@ template <> struct Op<GPTQ_HIP_F32> : Op<GPTQ_HIP_BF16> {
   static constexpr int PARTS = 3;
 };
 
+// A constant in a vector register, unknown to the compiler: "mask, then or" is one instruction then.  With both
+// constants in sight it is two, since an instruction reads one scalar register at most.
+__device__ __forceinline__ uint32_t opaque(uint32_t v) {
+  asm("" : "+v"(v));
+  return v;
+}
+
 // Packed rows of one k-step (32 input features) that a lane holds, and how their bytes become B operands.  Lane
 // (l16, g) owns features 8 g .. 8 g + 7 of the step: 4 packed rows of 4-bit codes, 8 of 8-bit codes.
 template <int XT, int BITS> struct Codes {
@@ -106,15 +113,16 @@ template <int XT, int BITS> struct Codes {
         b[i] = __builtin_bit_cast(uint32_t, v);
       }
     } else {
+      const uint32_t bias = opaque(XT == GPTQ_HIP_BF16 ? 0x43004300u : 0x54005400u);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const uint32_t p = __builtin_amdgcn_perm(r[2 * i + 1], r[2 * i], 0x0C040C00u + 0x00010001u * q);
         if (XT == GPTQ_HIP_BF16) {
-          b[2 * i] = (p & 0x000F000Fu) | 0x43004300u;
-          b[2 * i + 1] = ((p >> 4) & 0x000F000Fu) | 0x43004300u;
+          b[2 * i] = (p & 0x000F000Fu) | bias;
+          b[2 * i + 1] = ((p >> 4) & 0x000F000Fu) | bias;
         } else {
-          b[2 * i] = ((p << 4) & 0x00F000F0u) | 0x54005400u;
-          b[2 * i + 1] = (p & 0x00F000F0u) | 0x54005400u;
+          b[2 * i] = ((p << 4) & 0x00F000F0u) | bias;
+          b[2 * i + 1] = (p & 0x00F000F0u) | bias;
         }
       }
     }

@@ -137,11 +137,11 @@ struct Choice {
   int row_blocks;
 };
 static Choice choose(int64_t P, int E, int64_t C, int64_t group, int x_dtype, int transpose) {
-  if ((group && group % 32) || C < (transpose ? 16 : 8)) return {Choice::SIMPLE, 0};
+  if ((group && group % 32) || C < 16) return {Choice::SIMPLE, 0};
   if (transpose) return {Choice::BACK, 8};
   const int64_t rows = P / E;                   // of an expert, on average
-  if (rows <= 12) return {Choice::STRIP, 1};
-  if (rows <= 40 || C < 16) return P <= (int64_t)1 << 19 ? Choice{Choice::STRIP, 2} : Choice{Choice::SIMPLE, 0};
+  if (rows <= 12 && C >= 128) return {Choice::STRIP, 1};
+  if (rows <= 40 && C >= 128) return {Choice::STRIP, 2};
   return {Choice::TILE, rows <= 96 || x_dtype == GPTQ_HIP_F32 ? 4 : 8};
 }
 

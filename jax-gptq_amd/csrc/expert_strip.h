@@ -17,9 +17,10 @@ namespace xqmm {
 
 constexpr int STRIP_WAVES = 8;
 
-template <int XT, int BITS, int ZB, int KS, int RB, int CW> struct Strip {
+template <int XT, int BITS, int ZT, int KS, int RB, int CW> struct Strip {
   using C = Codes<XT, BITS>;
   using O = Op<XT>;
+  static constexpr int ZB = ZT == GPTQ_HIP_F32 ? 4 : 2; // bytes of a table's element
   static constexpr int SPAN = 32 * KS;                  // input features of a unit, all in one group
   static constexpr int DW = CW / 4;                     // dwords of a packed row
   static constexpr int XW = XT == GPTQ_HIP_F32 ? 2 : 1; // 16-byte words of 8 activations
@@ -30,56 +31,69 @@ template <int XT, int BITS, int ZB, int KS, int RB, int CW> struct Strip {
     u32x4 x[RB][KS][XW];
   };
   struct Ctx {
-    const uint8_t *w;             // the lane's bytes of packed row 0
-    const char *zero, *scale;     // the lane's channels in table row 0
-    const char *x[RB];            // the lane's rows of x
+    const uint8_t *w;             // packed row 0 of the expert (the same for all lanes, as all pointers but x)
+    const char *zero, *scale;     // table row 0
+    const char *x[RB];            // the lane's rows of x, at the lane group's first feature
     int64_t K, R, N;
+    uint32_t col, at_w, at_z;     // the lane's first channel; its bytes past `w` and past the tables' rows
     uint32_t magic;               // unit -> table row: 0 (all channels), 1 (a row each), else floor(2^32 / units a row) + 1
-    int g4, shift, bf_tables;
+    int g4;
   };
 
   // TAIL: the unit may reach past K.  Activations from there are zero, the other loads are kept inside.
   template <bool TAIL> static __device__ __forceinline__ void load(Unit &u, const Ctx &c, int unit) {
+    load_weights<TAIL>(u, c, unit);
+    load_rows<TAIL>(u, c, unit);
+  }
+  template <bool TAIL> static __device__ __forceinline__ void load_weights(Unit &u, const Ctx &c, int unit) {
+    const uint8_t *wu = c.w + (int64_t)unit * (BITS == 4 ? SPAN / 2 : SPAN) * c.N;
 #pragma unroll
     for (int t = 0; t < KS; ++t) {
-      const int64_t k = (int64_t)unit * SPAN + 32 * t + 8 * c.g4;
-      const int64_t r0 = BITS == 4 ? k >> 1 : k;
 #pragma unroll
       for (int i = 0; i < C::ROWS; ++i) {
-        int64_t r = r0 + i;
-        if (TAIL) r = r < c.R ? r : c.R - 1;
-        if (CW == 4) {
-          u.w[t][0][i] = reinterpret_cast<const U32u *>(c.w + r * c.N)->v;
+        const uint8_t *p;
+        if (TAIL) {
+          int64_t r = (int64_t)unit * (BITS == 4 ? SPAN / 2 : SPAN) + (BITS == 4 ? 16 : 32) * t + C::ROWS * c.g4 + i;
+          r = r < c.R ? r : c.R - 1;
+          p = c.w + r * c.N + c.col;
         } else {
-          const U64u v = *reinterpret_cast<const U64u *>(c.w + r * c.N);
+          p = wu + (int64_t)((BITS == 4 ? 16 : 32) * t + i) * c.N + c.at_w;
+        }
+        if (CW == 4) {
+          u.w[t][0][i] = reinterpret_cast<const U32u *>(p)->v;
+        } else {
+          const U64u v = *reinterpret_cast<const U64u *>(p);
 #pragma unroll
           for (int d = 0; d < DW; ++d) u.w[t][d][i] = v.v[d];
         }
       }
     }
     const uint32_t row = c.magic < 2 ? c.magic * (uint32_t)unit : __umulhi((uint32_t)unit, c.magic);
-    const int64_t at = (int64_t)row * c.N * ZB;
+    const char *zp = c.zero + (int64_t)row * c.N * ZB + c.at_z, *sp = c.scale + (int64_t)row * c.N * ZB + c.at_z;
     if (ZD == 2) {
-      const U64u a = *reinterpret_cast<const U64u *>(c.zero + at), b = *reinterpret_cast<const U64u *>(c.scale + at);
+      const U64u a = *reinterpret_cast<const U64u *>(zp), b = *reinterpret_cast<const U64u *>(sp);
 #pragma unroll
       for (int d = 0; d < 2; ++d) { u.z[d] = a.v[d]; u.s[d] = b.v[d]; }
     } else {
 #pragma unroll
       for (int d4 = 0; d4 < ZD / 4; ++d4) {
-        const u32x4 a = load16(c.zero + at + 16 * d4), b = load16(c.scale + at + 16 * d4);
+        const u32x4 a = load16(zp + 16 * d4), b = load16(sp + 16 * d4);
 #pragma unroll
         for (int d = 0; d < 4; ++d) { u.z[4 * d4 + d] = a[d]; u.s[4 * d4 + d] = b[d]; }
       }
     }
+  }
+  template <bool TAIL> static __device__ __forceinline__ void load_rows(Unit &u, const Ctx &c, int unit) {
+    constexpr int SZ = XT == GPTQ_HIP_F32 ? 4 : 2;
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
+      const char *xu = c.x[b] + (int64_t)unit * SPAN * SZ;
 #pragma unroll
       for (int t = 0; t < KS; ++t) {
         const int64_t k = (int64_t)unit * SPAN + 32 * t + 8 * c.g4;
-        constexpr int SZ = XT == GPTQ_HIP_F32 ? 4 : 2;
         if (!TAIL || k + 8 <= c.K) {
 #pragma unroll
-          for (int v = 0; v < XW; ++v) u.x[b][t][v] = load16(c.x[b] + k * SZ + 16 * v);
+          for (int v = 0; v < XW; ++v) u.x[b][t][v] = load16(xu + 32 * t * SZ + 16 * v);
         } else {
 #pragma unroll
           for (int v = 0; v < XW; ++v) {
@@ -87,11 +101,11 @@ template <int XT, int BITS, int ZB, int KS, int RB, int CW> struct Strip {
             for (int d = 0; d < 4; ++d) {
               uint32_t word = 0;
               if (SZ == 4) {
-                if (k + 4 * v + d < c.K) word = ((const uint32_t *)c.x[b])[k + 4 * v + d];
+                if (k + 4 * v + d < c.K) word = ((const uint32_t *)xu)[32 * t + 4 * v + d];
               } else {
-                const uint16_t *p = (const uint16_t *)c.x[b];
-                if (k + 2 * d < c.K) word = p[k + 2 * d];
-                if (k + 2 * d + 1 < c.K) word |= (uint32_t)p[k + 2 * d + 1] << 16;
+                const uint16_t *p = (const uint16_t *)xu + 32 * t;
+                if (k + 2 * d < c.K) word = p[2 * d];
+                if (k + 2 * d + 1 < c.K) word |= (uint32_t)p[2 * d + 1] << 16;
               }
               u.x[b][t][v][d] = word;
             }
@@ -109,35 +123,13 @@ template <int XT, int BITS, int ZB, int KS, int RB, int CW> struct Strip {
         v[q] = __builtin_bit_cast(float, raw[q]);
       } else {
         const uint32_t h = (raw[q / 2] >> (16 * (q & 1))) & 0xFFFFu;
-        v[q] = c.bf_tables ? __builtin_bit_cast(float, h << 16)
-                           : (float)__builtin_bit_cast(_Float16, (uint16_t)h);
-      }
-    }
-    if (c.shift >= 0) {             // the strip that N ends in (uniform): lanes past N - CW loaded from N - CW on
-#pragma unroll
-      for (int s = 1; s < CW; s <<= 1) {
-#pragma unroll
-        for (int q = 0; q + s < CW; ++q) v[q] = (c.shift & s) ? v[q + s] : v[q];
+        v[q] = ZT == GPTQ_HIP_BF16 ? __builtin_bit_cast(float, h << 16)
+                                   : (float)__builtin_bit_cast(_Float16, (uint16_t)h);
       }
     }
   }
 
   static __device__ __forceinline__ void multiply(Unit &u, const Ctx &c, f32x4 out[RB][CW]) {
-    if (c.shift >= 0) {
-#pragma unroll
-      for (int t = 0; t < KS; ++t)
-#pragma unroll
-        for (int i = 0; i < C::ROWS; ++i) {
-          if (DW == 1) {
-            u.w[t][0][i] >>= 8 * (c.shift & 3);
-          } else {
-            uint64_t v = (uint64_t)u.w[t][1][i] << 32 | u.w[t][0][i];
-            v >>= 8 * (c.shift & 7);
-            u.w[t][0][i] = (uint32_t)v;
-            u.w[t][DW - 1][i] = (uint32_t)(v >> 32);
-          }
-        }
-    }
     u32x4 a[RB][KS][O::PARTS];
     f32x4 sum[RB];
     const u32x4 ones = {O::ONE, O::ONE, O::ONE, O::ONE};
@@ -177,21 +169,24 @@ template <int XT, int BITS, int ZB, int KS, int RB, int CW> struct Strip {
   }
 };
 
-template <int XT, int BITS, int ZB, int KS, int RB, int CW>
+template <int XT, int BITS, int ZT, int KS, int RB, int CW>
 __global__ __launch_bounds__(STRIP_WAVES * 64) void strip_kernel(ExpertArgs a) {
-  using S = Strip<XT, BITS, ZB, KS, RB, CW>;
+  using S = Strip<XT, BITS, ZT, KS, RB, CW>;
+  constexpr int ZB = S::ZB;
   constexpr int H = 16 * RB;
   __shared__ f32x4 red[STRIP_WAVES / 2][RB * CW][64];
   const int lane = threadIdx.x & 63, l16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Tile tile = find_tile(a.offsets, a.E, (int)a.P, H, blockIdx.y);
   if (tile.rows <= 0) return;
-  const int64_t N = a.C, K = BITS == 4 ? 2 * a.R : a.R, n0 = (int64_t)blockIdx.x * 16 * CW;
+  const int64_t N = a.C, K = BITS == 4 ? 2 * a.R : a.R;
+  // (the last strip ends where N does; what it shares with the one before it is computed twice, to the same bits)
+  const int64_t n0 = (int64_t)blockIdx.x * 16 * CW + 16 * CW <= N ? (int64_t)blockIdx.x * 16 * CW : N - 16 * CW;
   const bool f32 = a.out_dtype == GPTQ_HIP_F32;
   if (tile.expert == a.E) {                            // rows of nowhere
     for (int i = threadIdx.x; i < tile.rows * 16 * CW; i += STRIP_WAVES * 64) {
       const int64_t n = n0 + i % (16 * CW);
-      if (n < N) store_out<XT>(a.out, f32, (int64_t)(tile.row0 + i / (16 * CW)) * N + n, 0.f);
+      store_out<XT>(a.out, f32, (int64_t)(tile.row0 + i / (16 * CW)) * N + n, 0.f);
     }
     return;
   }
@@ -203,24 +198,13 @@ __global__ __launch_bounds__(STRIP_WAVES * 64) void strip_kernel(ExpertArgs a) {
   const uint32_t per = a.group ? (uint32_t)(a.group / S::SPAN) : 0u;
   c.magic = per < 2 ? per : 0xFFFFFFFFu / per + 1u;    // (exact: a unit's number times `per` stays far below 2^32)
   c.g4 = lane >> 4;
-  c.bf_tables = a.zs_dtype == GPTQ_HIP_BF16;
-  int64_t col = n0 + CW * l16;
-  c.shift = n0 + 16 * CW > N ? 0 : -1;                 // -1: the whole strip lies inside
-  if (col + CW > N) {
-    const int64_t over = col - (N - CW);
-    c.shift = (int)(over < CW ? over : 0);             // (a lane wholly outside: its values are not stored)
-    col = N - CW;
-  }
-  c.w = a.packed + (int64_t)tile.expert * a.R * N + col;
-  c.zero = (const char *)a.zero + ((int64_t)tile.expert * tables * N + col) * ZB;
-  c.scale = (const char *)a.scale + ((int64_t)tile.expert * tables * N + col) * ZB;
-#pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    int m = 16 * b + l16;
-    m = m < tile.rows ? m : tile.rows - 1;             // rows past the last repeat it and are not stored
-    c.x[b] = (const char *)a.x + x_row_of(a.order, a.top_k, a.T, tile.row0 + m) * K * (XT == GPTQ_HIP_F32 ? 4 : 2);
-  }
-
+  const int64_t col = n0 + CW * l16;
+  c.w = a.packed + (int64_t)tile.expert * a.R * N;
+  c.zero = (const char *)a.zero + (int64_t)tile.expert * tables * N * ZB;
+  c.scale = (const char *)a.scale + (int64_t)tile.expert * tables * N * ZB;
+  c.col = (uint32_t)col;
+  c.at_w = (uint32_t)(S::C::ROWS * c.g4 * N + col);
+  c.at_z = (uint32_t)(col * ZB);
   f32x4 out[RB][CW];
 #pragma unroll
   for (int b = 0; b < RB; ++b)
@@ -231,10 +215,25 @@ __global__ __launch_bounds__(STRIP_WAVES * 64) void strip_kernel(ExpertArgs a) {
   constexpr int D = KS == 4 ? 2 : (KS == 2 && BITS == 4 && XT != GPTQ_HIP_F32 ? 3 : (KS == 2 ? 2 : 3));
   const int whole = (int)(K / S::SPAN);
   const int mine = whole > wave ? (whole - wave + STRIP_WAVES - 1) / STRIP_WAVES : 0;
+  typename S::Unit ring[D];
+  // (the first weights are on their way while the rows' numbers are fetched)
   if (mine > 0) {
-    typename S::Unit ring[D];
 #pragma unroll
-    for (int d = 0; d + 1 < D; ++d) S::template load<false>(ring[d], c, wave + STRIP_WAVES * (d < mine ? d : mine - 1));
+    for (int d = 0; d + 1 < D; ++d)
+      S::template load_weights<false>(ring[d], c, wave + STRIP_WAVES * (d < mine ? d : mine - 1));
+  }
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    int m = 16 * b + l16;
+    m = m < tile.rows ? m : tile.rows - 1;             // rows past the last repeat it and are not stored
+    c.x[b] = (const char *)a.x + (x_row_of(a.order, a.top_k, a.T, tile.row0 + m) * K + 8 * c.g4) *
+                                     (XT == GPTQ_HIP_F32 ? 4 : 2);
+  }
+
+  if (mine > 0) {
+#pragma unroll
+    for (int d = 0; d + 1 < D; ++d)
+      S::template load_rows<false>(ring[d], c, wave + STRIP_WAVES * (d < mine ? d : mine - 1));
     for (int i = 0; i < mine; i += D) {
 #pragma unroll
       for (int d = 0; d < D; ++d) {
@@ -272,7 +271,6 @@ __global__ __launch_bounds__(STRIP_WAVES * 64) void strip_kernel(ExpertArgs a) {
 #pragma unroll
     for (int w = 1; w < STRIP_WAVES / 2; ++w) v += red[w][t][l];
     const int64_t n = n0 + CW * (l & 15) + t % CW;
-    if (n >= N) continue;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int m = 16 * (t / CW) + 4 * (l >> 4) + r;
@@ -289,12 +287,17 @@ template <int XT, int RB, int CW> static int strip_launch(hipStream_t s, const E
   constexpr bool four = XT != GPTQ_HIP_F32;
   const bool r4 = four && a.bits == 4;
   const int ks = !a.group || a.group % 128 == 0 ? (r4 ? 4 : 2) : (a.group % 64 == 0 ? 2 : 1);
-  const int zb = a.zs_dtype == GPTQ_HIP_F32 ? 4 : 2;
-#define GPTQ_STRIP(B, Z, S) \
-  if (a.bits == B && zb == Z && ks == S) strip_kernel<XT, B, Z, S, RB, CW><<<grid, STRIP_WAVES * 64, 0, s>>>(a);
-  if constexpr (four) { GPTQ_STRIP(4, 4, 4) GPTQ_STRIP(4, 2, 4) }
-  GPTQ_STRIP(4, 4, 2) GPTQ_STRIP(4, 4, 1) GPTQ_STRIP(4, 2, 2) GPTQ_STRIP(4, 2, 1)
-  GPTQ_STRIP(8, 4, 2) GPTQ_STRIP(8, 4, 1) GPTQ_STRIP(8, 2, 2) GPTQ_STRIP(8, 2, 1)
+#define GPTQ_STRIP(B, S)                                                                                          \
+  if (a.bits == B && ks == S) {                                                                                   \
+    if (a.zs_dtype == GPTQ_HIP_F32)                                                                               \
+      strip_kernel<XT, B, GPTQ_HIP_F32, S, RB, CW><<<grid, STRIP_WAVES * 64, 0, s>>>(a);                          \
+    else if (a.zs_dtype == GPTQ_HIP_F16)                                                                          \
+      strip_kernel<XT, B, GPTQ_HIP_F16, S, RB, CW><<<grid, STRIP_WAVES * 64, 0, s>>>(a);                          \
+    else                                                                                                          \
+      strip_kernel<XT, B, GPTQ_HIP_BF16, S, RB, CW><<<grid, STRIP_WAVES * 64, 0, s>>>(a);                         \
+  }
+  if constexpr (four) { GPTQ_STRIP(4, 4) }
+  GPTQ_STRIP(4, 2) GPTQ_STRIP(4, 1) GPTQ_STRIP(8, 2) GPTQ_STRIP(8, 1)
 #undef GPTQ_STRIP
   GPTQ_CHECK_LAUNCH();
   return GPTQ_HIP_OK;
