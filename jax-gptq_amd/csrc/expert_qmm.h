@@ -19,10 +19,11 @@ struct ExpertArgs {
 int expert_strip_f16(hipStream_t s, const ExpertArgs &a, int row_blocks);
 int expert_strip_bf16(hipStream_t s, const ExpertArgs &a, int row_blocks);
 int expert_strip_f32(hipStream_t s, const ExpertArgs &a, int row_blocks);
-// the same by tiles of 64 (row_blocks 4) or 128 (8) rows x 256 channels (expert_tile.h); ws: expert_tile_bytes
-int expert_tile_f16(hipStream_t s, const ExpertArgs &a, int row_blocks, void *ws);
-int expert_tile_bf16(hipStream_t s, const ExpertArgs &a, int row_blocks, void *ws);
-int expert_tile_f32(hipStream_t s, const ExpertArgs &a, int row_blocks, void *ws);
+// the same by tiles (expert_tile.h) of these rows x channels; fp32 activations: the first and the third
+enum { TILE_32x128, TILE_64x128, TILE_64x256, TILE_128x256 };
+int expert_tile_f16(hipStream_t s, const ExpertArgs &a, int shape, void *ws);
+int expert_tile_bf16(hipStream_t s, const ExpertArgs &a, int shape, void *ws);
+int expert_tile_f32(hipStream_t s, const ExpertArgs &a, int shape, void *ws);
 // the transposed product by tiles of 128 rows x 256 input features (expert_back.h)
 int expert_back_f16(hipStream_t s, const ExpertArgs &a, void *ws);
 int expert_back_bf16(hipStream_t s, const ExpertArgs &a, void *ws);

@@ -121,9 +121,9 @@ static int strip_run(hipStream_t s, const ExpertArgs &a, int row_blocks) {
   return a.x_dtype == GPTQ_HIP_F16 ? expert_strip_f16(s, a, row_blocks) : expert_strip_bf16(s, a, row_blocks);
 }
 
-static int tile_run(hipStream_t s, const ExpertArgs &a, int row_blocks, void *ws) {
-  if (a.x_dtype == GPTQ_HIP_F32) return expert_tile_f32(s, a, row_blocks, ws);
-  return a.x_dtype == GPTQ_HIP_F16 ? expert_tile_f16(s, a, row_blocks, ws) : expert_tile_bf16(s, a, row_blocks, ws);
+static int tile_run(hipStream_t s, const ExpertArgs &a, int shape, void *ws) {
+  if (a.x_dtype == GPTQ_HIP_F32) return expert_tile_f32(s, a, shape, ws);
+  return a.x_dtype == GPTQ_HIP_F16 ? expert_tile_f16(s, a, shape, ws) : expert_tile_bf16(s, a, shape, ws);
 }
 
 static int back_run(hipStream_t s, const ExpertArgs &a, void *ws) {
@@ -134,15 +134,16 @@ static int back_run(hipStream_t s, const ExpertArgs &a, void *ws) {
 // Which kernel a product runs on.
 struct Choice {
   enum Kind { SIMPLE, STRIP, TILE, BACK } kind;
-  int row_blocks;
+  int shape;                // STRIP: blocks of 16 rows; TILE: TILE_*
 };
 static Choice choose(int64_t P, int E, int64_t C, int64_t group, int x_dtype, int transpose) {
   if ((group && group % 32) || C < 16) return {Choice::SIMPLE, 0};
   if (transpose) return {Choice::BACK, 8};
   const int64_t rows = P / E;                   // of an expert, on average
   if (rows <= 12 && C >= 128) return {Choice::STRIP, 1};
-  if (rows <= 40 && C >= 128) return {Choice::STRIP, 2};
-  return {Choice::TILE, rows <= 96 || x_dtype == GPTQ_HIP_F32 ? 4 : 8};
+  if (rows <= 24) return {Choice::TILE, TILE_32x128};
+  if (x_dtype == GPTQ_HIP_F32) return {Choice::TILE, rows <= 40 ? TILE_32x128 : TILE_64x256};
+  return {Choice::TILE, rows <= 80 ? TILE_64x128 : TILE_128x256};
 }
 
 // GPTQ_HIP_OK, or why the product is refused
@@ -189,12 +190,12 @@ int gptq_hip_expert_qmatmul(void *stream, const void *x, int x_dtype, int64_t x_
   if (a.P == 0) return GPTQ_HIP_OK;
   hipStream_t s = as_stream(stream);
   const Choice c = choose(a.P, a.E, a.C, a.group, a.x_dtype, a.transpose);
-  if (c.kind == Choice::STRIP) return strip_run(s, a, c.row_blocks);
+  if (c.kind == Choice::STRIP) return strip_run(s, a, c.shape);
   const size_t need = gptq_hip_expert_qmatmul_workspace_bytes(a.T, a.P, a.R, a.C, a.bits, a.group, a.E, a.x_dtype,
                                                               a.zs_dtype, a.transpose);
   if (need && (!ws || ws_bytes < need)) return GPTQ_HIP_EWORKSPACE;
   if (need && (uintptr_t)ws % 16) return GPTQ_HIP_EINVAL;
-  if (c.kind == Choice::TILE) return tile_run(s, a, c.row_blocks, ws);
+  if (c.kind == Choice::TILE) return tile_run(s, a, c.shape, ws);
   if (c.kind == Choice::BACK && (uintptr_t)a.x % 16 == 0) return back_run(s, a, ws);
   return simple_run(s, a);
 }

@@ -1,14 +1,15 @@
-// Many rows per expert: a workgroup computes BM x 256 outputs of one expert (BM = 128 or 64), K in stages of 64.
+// Many rows per expert: a workgroup computes a tile of one expert's outputs, K in stages of 64: 128 or 64 rows x 256
+// channels, or 64 or 32 rows x 128 channels with K in two halves, which fill the chip where the tiles are few.
 //
 //   y[p, n] = sum_G s[G, n] (sum_{k in G} x[p, k] (o + c[k, n]) - (o + z[G, n]) sum_{k in G} x[p, k])
 //
-// Bound by the matrix cores and the instructions that turn codes into their operands.  Everything a stage needs goes
-// from memory to LDS without passing a register, four stages deep: the activations of the tile's rows (16 KB at
-// BM = 128), the packed codes (8 KB; they stay packed in LDS), the group's scales and zeros and the rows' sums.  One
-// barrier per stage: wavefronts wait for their own loads of stage s, meet, and issue the loads of stage s + 3 into the
-// buffer that everybody has finished with.  Each wavefront owns 64 x 64 outputs: its four operands of codes are built
-// in registers and used for four row blocks.  fp32 sums of a group are scaled into a second set of accumulators, so
-// codes stay exact 16-bit operands whatever the scales are.
+// Bound by the matrix cores and the instructions that turn codes into their operands (many rows), by the bytes of the
+// weights (few).  Everything a stage needs goes from memory to LDS without passing a register, three or four stages
+// deep: the activations of the tile's rows, the packed codes (they stay packed in LDS), the group's scales and zeros
+// and the rows' sums.  One barrier per stage: wavefronts wait for their own loads of stage s, meet, and issue the loads
+// of a later stage into the buffer that everybody has finished with.  Each wavefront owns 64 (or 32) x 64 outputs: its
+// four operands of codes are built in registers and used for four (two) row blocks.  fp32 sums of a group are scaled
+// into a second set of accumulators, so codes stay exact 16-bit operands whatever the scales are.
 // A first kernel writes the activations once more, in the order of the operands (fp32: as three bf16 parts), padded to
 // whole stages, and the sums of every row over the part of its group up to the end of each stage.
 #pragma once
@@ -16,7 +17,7 @@
 
 namespace xqmm {
 
-constexpr int TILE_BK = 64, TILE_BN = 256, TILE_STAGES = 4;
+constexpr int TILE_BK = 64;
 constexpr int TILE_LONG = 512;            // without groups a sum is closed every 512 features all the same: short sums
                                           // keep the offset of the codes from costing precision
 
@@ -135,27 +136,34 @@ struct TileArgs {
 };
 
 // ZL: how tables lie in LDS: 4 or 2 bytes an element as they are in memory, 0: operands that start or end anywhere,
-// whose codes and tables pass through registers (tables converted to fp32)
-template <int XT, int BITS, int ZL, bool HALF, int WM>
-struct TileShape {
-  static constexpr int WAVES = 4 * WM, THREADS = 64 * WAVES, BM = 64 * WM;
+// whose codes and tables pass through registers (tables converted to fp32).
+// A wavefront owns 16 RBW rows x 64 channels; WM x WN wavefronts cover the tile, WK such sets take a part of K each.
+template <int XT, int BITS, int ZL, bool HALF, int RBW, int WM, int WN, int WK> struct TileShape {
+  static constexpr int SET = WM * WN, WAVES = SET * WK, THREADS = 64 * WAVES, BM = 16 * RBW * WM, BN = 64 * WN;
   static constexpr int PARTS = Op<XT>::PARTS;
-  static constexpr int BROWS = BITS == 4 ? 32 : 64;       // packed rows of a stage
-  static constexpr int HN = HALF ? 2 : 1;
-  static constexpr int A = PARTS * BM * 128, B = BROWS * 256, Z = HN * 1024, S = HN * BM * 4;
-  static constexpr int STAGE = A + B + 2 * Z + S;
-  static constexpr int STAGES = 4 * STAGE <= 160 * 1024 ? 4 : (3 * STAGE <= 160 * 1024 ? 3 : 2);
+  static constexpr int BROWS = BITS == 4 ? 32 : 64;       // packed rows of a part's stage
+  static constexpr int HN = HALF ? 2 : 1, MB = (BM + 63) / 64;
+  // one part's rows, codes, zeros and scales (of a group), sums; then all parts'
+  static constexpr int AP = PARTS * BM * 128, BP = BROWS * BN, ZP = 2 * BN * 4, SP = MB * 256;
+  static constexpr int A = WK * AP, B = WK * BP, Z = WK * HN * ZP, S = WK * HN * SP;
+  static constexpr int STAGE = A + B + Z + S;
+  // up to four stages; workgroups of four wavefronts leave room for a second one on the CU where that takes no more
+  // than a stage
+  static constexpr int ROOM = WAVES == 4 && 3 * STAGE <= 80 * 1024 ? 80 * 1024 : 160 * 1024;
+  static constexpr int STAGES = 4 * STAGE <= ROOM ? 4 : (3 * STAGE <= ROOM ? 3 : 2);
   static constexpr int LDS = STAGES * STAGE;
   // loads of a wavefront per stage
-  static constexpr int AI = 2 * PARTS, BI = BROWS / 4 / WAVES;
-  static constexpr int SUMS = HN * WM, ITEMS = SUMS + 2 * HN;        // sums by 64 rows, zeros, scales
+  static constexpr int AI = A / 1024 / WAVES, BI = B / 1024 / WAVES;
+  static constexpr int SI = WK * HN * MB, TI = WK * HN * (BN / 128), ITEMS = SI + TI;
   static constexpr int MI = (ITEMS + WAVES - 1) / WAVES;
   static constexpr int LOADS = AI + BI + MI;
+  static_assert(A % (1024 * WAVES) == 0 && B % (1024 * WAVES) == 0 && STAGES * STAGE <= 160 * 1024, "whole loads");
+  static_assert(WK == 1 || SET * RBW * 4 * 1024 <= LDS, "partial tiles fit");
 };
 
-template <int XT, int BITS, int ZL, bool HALF, int WM>
-__global__ __launch_bounds__(256 * WM, 2) void tile_kernel(TileArgs t) {
-  using T = TileShape<XT, BITS, ZL, HALF, WM>;
+template <int XT, int BITS, int ZL, bool HALF, int RBW, int WM, int WN, int WK>
+__global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) {
+  using T = TileShape<XT, BITS, ZL, HALF, RBW, WM, WN, WK>;
   using C = Codes<XT, BITS>;
   using O = Op<XT>;
   typedef __attribute__((address_space(3))) char lds_char;
@@ -163,27 +171,27 @@ __global__ __launch_bounds__(256 * WM, 2) void tile_kernel(TileArgs t) {
   const ExpertArgs &a = t.a;
   const int lane = threadIdx.x & 63, l16 = lane & 15, g4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave >> 2, wn = wave & 3;
+  const int part = wave / T::SET, wm = wave / WN % WM, wn = wave % WN;
   const int64_t N = a.C;
   const bool f32 = a.out_dtype == GPTQ_HIP_F32;
 
   // Which tile.  Workgroups go round the eight XCDs; each XCD takes a run of the list (panels of four column tiles, row
   // tile by row tile), so what runs on it at a time shares rows and weights in its L2.
   const int row_tiles = count_tiles(a.offsets, a.E, (int)a.P, T::BM);
-  const int cols = (int)((N + TILE_BN - 1) / TILE_BN);
+  const int cols = (int)((N + T::BN - 1) / T::BN);
   const int64_t total = (int64_t)row_tiles * cols, run = (total + 7) / 8;
   const int64_t pos = blockIdx.x >> 3, item = (blockIdx.x & 7) * run + pos;
   if (pos >= run || item >= total) return;
   const int panel = (int)(item / ((int64_t)row_tiles * 4));
   const int rest = (int)(item - (int64_t)panel * row_tiles * 4);
   const int width = cols - 4 * panel < 4 ? cols - 4 * panel : 4;
-  const int64_t n0 = (int64_t)(4 * panel + rest % width) * TILE_BN;
+  const int64_t n0 = (int64_t)(4 * panel + rest % width) * T::BN;
   const Tile tile = find_tile(a.offsets, a.E, (int)a.P, T::BM, rest / width);
   if (tile.rows <= 0) return;
   if (tile.expert == a.E) {                            // rows of nowhere
-    for (int i = threadIdx.x; i < tile.rows * TILE_BN; i += T::THREADS) {
-      const int64_t n = n0 + i % TILE_BN;
-      if (n < N) store_out<XT>(a.out, f32, (int64_t)(tile.row0 + i / TILE_BN) * N + n, 0.f);
+    for (int i = threadIdx.x; i < tile.rows * T::BN; i += T::THREADS) {
+      const int64_t n = n0 + i % T::BN;
+      if (n < N) store_out<XT>(a.out, f32, (int64_t)(tile.row0 + i / T::BN) * N + n, 0.f);
     }
     return;
   }
@@ -195,47 +203,59 @@ __global__ __launch_bounds__(256 * WM, 2) void tile_kernel(TileArgs t) {
   const int zsize = a.zs_dtype == GPTQ_HIP_F32 ? 4 : 2;
   const char *zero = (const char *)a.zero + (int64_t)tile.expert * tables * N * zsize;
   const char *scale = (const char *)a.scale + (int64_t)tile.expert * tables * N * zsize;
+  // part p takes stages p * span .. of K; the cut lies between groups
+  const int span = WK == 1 ? t.stages : ((t.stages + WK - 1) / WK + t.close - 1) / t.close * t.close;
+  auto stage_of = [&](int p, int s) -> int {           // (past the end: the last once more, not multiplied)
+    const int st = p * span + s;
+    return st < t.stages ? st : t.stages - 1;
+  };
 
-  // sources of this lane's loads
-  const char *arow[2];
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    int m = 8 * (2 * wave + j) + (lane >> 3);
+  // sources of this lane's loads.  The 16-byte chunks of a row of activations lie turned by the row's number, those of
+  // codes by their lane group, so that the reads of a wavefront meet all banks.
+  auto row_base = [&](int m) -> int64_t {
     m = m < tile.rows ? m : tile.rows - 1;             // rows past the last repeat it and are not stored
-    arow[j] = t.rows + x_row_of(a.order, a.top_k, a.T, tile.row0 + m) * t.row_bytes + ((lane & 7) ^ (lane >> 3)) * 16;
+    return x_row_of(a.order, a.top_k, a.T, tile.row0 + m);
+  };
+  const char *arow[T::AI];
+#pragma unroll
+  for (int j = 0; j < T::AI; ++j)
+    arow[j] = t.rows + row_base(8 * ((wave * T::AI + j) % (T::BM / 8)) + (lane >> 3)) * t.row_bytes +
+              ((lane & 7) ^ (lane >> 3)) * 16;
+  const float *srow[T::MI];
+#pragma unroll
+  for (int j = 0; j < T::MI; ++j) {
+    const int it = (wave + T::WAVES * j) % T::ITEMS;
+    srow[j] = t.sums;
+    if (it < T::SI) srow[j] = t.sums + row_base(64 * (it % T::MB) + lane) * t.per_row;
   }
-  const float *srow = nullptr;
-  {
-    const int sums_item = wave % T::ITEMS % WM;        // the 64 rows whose sums this wavefront may load
-    int m = 64 * sums_item + lane;
-    m = m < tile.rows ? m : tile.rows - 1;
-    srow = t.sums + x_row_of(a.order, a.top_k, a.T, tile.row0 + m) * t.per_row;
-  }
-  auto table_row = [&](int stage, int h) -> int64_t {
+  auto table_row = [&](int st, int h) -> int64_t {
     if (!t.grouped) return 0;
-    const uint32_t unit = HALF ? 2u * stage + h : (uint32_t)stage;
+    const uint32_t unit = HALF ? 2u * st + h : (uint32_t)st;
     const uint32_t per = HALF ? (uint32_t)(a.group / 32) : (uint32_t)t.close;
     const int64_t r = unit / per;
     return r < tables ? r : tables - 1;
   };
+  // lane group that reads packed row r of a stage
+  auto reader = [](int r) -> int { return BITS == 4 ? (r >> 2) & 3 : (r >> 3) & 3; };
+  constexpr int CH = T::BN / 16;                       // chunks of a row of codes
+  constexpr int TABLE_REGS = WK * T::HN * 2 * T::BN / T::THREADS;
   u32x4 breg[ZL ? 1 : T::BI];
-  float zreg[ZL ? 1 : 2 * T::HN * TILE_BN / T::THREADS];
+  float zreg[ZL ? 1 : TABLE_REGS];
 
-  auto issue = [&](int stage, int slot) __attribute__((always_inline)) {
+  auto issue = [&](int s, int slot) __attribute__((always_inline)) {
     const uint32_t base = lds0 + slot * T::STAGE;
 #pragma unroll
-    for (int p = 0; p < T::PARTS; ++p)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        to_lds_16(arow[j] + p * t.Kp * 2 + (int64_t)stage * 128, base + p * T::BM * 128 + (2 * wave + j) * 1024);
+    for (int j = 0; j < T::AI; ++j) {
+      const int i = wave * T::AI + j, p = i / (T::AP / 1024), q = i % (T::AP / 1024) / (T::BM / 8);
+      to_lds_16(arow[j] + q * t.Kp * 2 + (int64_t)stage_of(p, s) * 128, base + i * 1024);
+    }
 #pragma unroll
     for (int j = 0; j < T::BI; ++j) {
-      const int i = wave * T::BI + j, row = 4 * i + (lane >> 4);
-      const int turn = BITS == 4 ? (i & 3) : ((i >> 1) & 3);
-      int64_t r = (int64_t)stage * T::BROWS + row;
+      const int i = wave * T::BI + j, p = i / (T::BP / 1024);
+      const int at = i % (T::BP / 1024) * (64 / CH) + lane / CH, g = reader(at);
+      int64_t r = (int64_t)stage_of(p, s) * T::BROWS + (T::BN == 128 ? at ^ (g >> 1) : at);
       r = r < a.R ? r : a.R - 1;                       // (past K: any code, the activations are zero)
-      const int chunk = (lane & 15) ^ (4 * turn);
-      int64_t n = n0 + 16 * chunk;
+      int64_t n = n0 + 16 * ((lane % CH) ^ (T::BN == 128 ? 4 * (g & 1) : 4 * g));
       if constexpr (ZL) {
         n = n < N ? n : 0;
         to_lds_16(packed + r * N + n, base + T::A + i * 1024);
@@ -246,31 +266,27 @@ __global__ __launch_bounds__(256 * WM, 2) void tile_kernel(TileArgs t) {
 #pragma unroll
     for (int j = 0; j < T::MI; ++j) {
       const int it = (wave + T::WAVES * j) % T::ITEMS;   // (more wavefronts than items: the same bytes twice)
-      if (it < T::SUMS) {
-        // 64 rows: it % WM, half it / WM
-        const int h = it / WM;
-        const float *s = srow;
-        if (T::MI > 1 || T::ITEMS > T::WAVES) {
-          int m = 64 * (it % WM) + lane;
-          m = m < tile.rows ? m : tile.rows - 1;
-          s = t.sums + x_row_of(a.order, a.top_k, a.T, tile.row0 + m) * t.per_row;
-        }
-        to_lds_4(s + (HALF ? 2 * stage + h : stage), base + T::A + T::B + 2 * T::Z + (h * T::BM + 64 * (it % WM)) * 4);
+      if (it < T::SI) {
+        const int q = it / T::MB, h = q % T::HN, st = stage_of(q / T::HN, s);
+        to_lds_4(srow[j] + (HALF ? 2 * st + h : st), base + T::A + T::B + T::Z + it * 256);
       } else if constexpr (ZL != 0) {
-        const int which = (it - T::SUMS) / T::HN, h = (it - T::SUMS) % T::HN;
-        const char *src = which ? scale : zero;
-        int64_t n = ZB == 4 ? n0 + 4 * lane : n0 + 8 * (lane & 31);
+        // zeros, then scales: 1 KB each at 256 channels, half a load each at 128
+        const int i = it - T::SI, q = i / (T::BN / 128);
+        const int which = T::BN == 128 ? lane >> 5 : i & 1, l = T::BN == 128 ? lane & 31 : lane;
+        int64_t n = ZB == 4 ? n0 + 4 * l : n0 + 8 * (l % (T::BN / 8));
         n = n < N ? n : 0;
-        to_lds_16(src + (table_row(stage, h) * N + n) * ZB, base + T::A + T::B + which * T::Z + h * 1024);
+        to_lds_16((which ? scale : zero) + (table_row(stage_of(q / T::HN, s), q % T::HN) * N + n) * ZB,
+                  base + T::A + T::B + i * 1024);
       }
     }
     if constexpr (!ZL) {
 #pragma unroll
-      for (int j = 0; j < 2 * T::HN * TILE_BN / T::THREADS; ++j) {
-        const int i = threadIdx.x + j * T::THREADS, which = i / (T::HN * TILE_BN), h = i / TILE_BN % T::HN;
-        int64_t n = n0 + i % TILE_BN;
+      for (int j = 0; j < TABLE_REGS; ++j) {
+        const int i = threadIdx.x + j * T::THREADS, which = i / T::BN & 1, q = i / (2 * T::BN);
+        int64_t n = n0 + i % T::BN;
         n = n < N ? n : N - 1;
-        zreg[j] = table_value(which ? scale : zero, a.zs_dtype, table_row(stage, h) * N + n);
+        zreg[j] = table_value(which ? scale : zero, a.zs_dtype,
+                              table_row(stage_of(q / T::HN, s), q % T::HN) * N + n);
       }
     }
   };
@@ -281,26 +297,25 @@ __global__ __launch_bounds__(256 * WM, 2) void tile_kernel(TileArgs t) {
       for (int j = 0; j < T::BI; ++j)
         *reinterpret_cast<u32x4 *>(base + T::A + (wave * T::BI + j) * 1024 + lane * 16) = breg[j];
 #pragma unroll
-      for (int j = 0; j < 2 * T::HN * TILE_BN / T::THREADS; ++j) {
-        const int i = threadIdx.x + j * T::THREADS, which = i / (T::HN * TILE_BN), h = i / TILE_BN % T::HN;
-        *reinterpret_cast<float *>(base + T::A + T::B + which * T::Z + h * 1024 + (i % TILE_BN) * 4) = zreg[j];
-      }
+      for (int j = 0; j < TABLE_REGS; ++j)
+        *reinterpret_cast<float *>(base + T::A + T::B + (threadIdx.x + j * T::THREADS) * 4) = zreg[j];
     }
   };
 
-  f32x4 out[4][4], acc[4][4];                           // [row block][byte of the codes]
+  f32x4 out[RBW][4], acc[RBW][4];                       // [row block][byte of the codes]
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < RBW; ++i)
 #pragma unroll
     for (int q = 0; q < 4; ++q) out[i][q] = acc[i][q] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   auto close = [&](const char *base, int h) __attribute__((always_inline)) {
-    const char *zp = base + T::A + T::B + h * 1024;
+    const char *zp = base + T::A + T::B + (part * T::HN + h) * T::ZP;
+    const char *sums = base + T::A + T::B + T::Z + (part * T::HN + h) * T::SP;
     float z[4], s[4];
     const int col = wn * 64 + 4 * l16;
     if constexpr (ZB == 4) {
       const f32x4 zv = *reinterpret_cast<const f32x4 *>(zp + col * 4);
-      const f32x4 sv = *reinterpret_cast<const f32x4 *>(zp + T::Z + col * 4);
+      const f32x4 sv = *reinterpret_cast<const f32x4 *>(zp + T::BN * 4 + col * 4);
 #pragma unroll
       for (int q = 0; q < 4; ++q) { z[q] = zv[q]; s[q] = sv[q]; }
     } else {
@@ -308,15 +323,14 @@ __global__ __launch_bounds__(256 * WM, 2) void tile_kernel(TileArgs t) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const uint32_t zh = *reinterpret_cast<const uint16_t *>(zp + (col + q) * 2);
-        const uint32_t sh = *reinterpret_cast<const uint16_t *>(zp + T::Z + (col + q) * 2);
+        const uint32_t sh = *reinterpret_cast<const uint16_t *>(zp + T::BN * 4 + (col + q) * 2);
         z[q] = bf ? __builtin_bit_cast(float, zh << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)zh);
         s[q] = bf ? __builtin_bit_cast(float, sh << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)sh);
       }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const f32x4 sum = *reinterpret_cast<const f32x4 *>(base + T::A + T::B + 2 * T::Z +
-                                                         (h * T::BM + wm * 64 + 16 * i + 4 * g4) * 4);
+    for (int i = 0; i < RBW; ++i) {
+      const f32x4 sum = *reinterpret_cast<const f32x4 *>(sums + (wm * 16 * RBW + 16 * i + 4 * g4) * 4);
 #pragma unroll
       for (int q = 0; q < 4; ++q)
 #pragma unroll
@@ -325,24 +339,26 @@ __global__ __launch_bounds__(256 * WM, 2) void tile_kernel(TileArgs t) {
     }
   };
   auto step = [&](const char *base, int ks, bool fresh) __attribute__((always_inline)) {
-    u32x4 x[4][T::PARTS];
+    u32x4 x[RBW][T::PARTS];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < RBW; ++i)
 #pragma unroll
       for (int p = 0; p < T::PARTS; ++p)
-        x[i][p] = *reinterpret_cast<const u32x4 *>(base + p * T::BM * 128 + (wm * 64 + 16 * i + l16) * 128 +
+        x[i][p] = *reinterpret_cast<const u32x4 *>(base + part * T::AP + p * T::BM * 128 +
+                                                   (wm * 16 * RBW + 16 * i + l16) * 128 +
                                                    (((4 * ks + g4) ^ (l16 & 7)) * 16));
     uint32_t r[C::ROWS];
-    const int chunk = (wn * 4 + (l16 >> 2)) ^ (4 * g4);
+    const int chunk = (wn * 4 + (l16 >> 2)) ^ (T::BN == 128 ? 4 * (g4 & 1) : 4 * g4);
 #pragma unroll
-    for (int i = 0; i < C::ROWS; ++i)
-      r[i] = *reinterpret_cast<const uint32_t *>(base + T::A + ((BITS == 4 ? 16 : 32) * ks + C::ROWS * g4 + i) * 256 +
-                                                 chunk * 16 + (l16 & 3) * 4);
+    for (int i = 0; i < C::ROWS; ++i) {
+      const int row = (BITS == 4 ? 16 : 32) * ks + C::ROWS * g4 + (T::BN == 128 ? i ^ (g4 >> 1) : i);
+      r[i] = *reinterpret_cast<const uint32_t *>(base + T::A + part * T::BP + row * T::BN + chunk * 16 + (l16 & 3) * 4);
+    }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const u32x4 w = C::operand(r, q);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < RBW; ++i)
 #pragma unroll
         for (int p = 0; p < T::PARTS; ++p)
           acc[i][q] = O::mma(x[i][p], w, fresh && p == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[i][q]);
@@ -353,26 +369,28 @@ __global__ __launch_bounds__(256 * WM, 2) void tile_kernel(TileArgs t) {
   constexpr int AHEAD = T::STAGES - 1;
 #pragma unroll
   for (int s = 0; s < AHEAD; ++s) {
-    issue(s < t.stages ? s : t.stages - 1, s);
+    issue(s, s);
     land(s);
   }
   int in_group = 0, slot = 0, into = AHEAD;
-  for (int s = 0; s < t.stages; ++s) {
+  for (int s = 0; s < span; ++s) {
     wait_and_meet<ZL ? (AHEAD - 1) * T::LOADS : 0>();
-    issue(s + AHEAD < t.stages ? s + AHEAD : t.stages - 1, into);
+    issue(s + AHEAD, into);
     const char *base = lds + slot * T::STAGE;
-    if constexpr (HALF) {
-      step(base, 0, true);
-      close(base, 0);
-      step(base, 1, true);
-      close(base, 1);
-    } else {
-      if (in_group == 0) step(base, 0, true);
-      else step(base, 0, false);
-      step(base, 1, false);
-      if (++in_group == t.close || s + 1 == t.stages) {
+    if (WK == 1 || part * span + s < t.stages) {
+      if constexpr (HALF) {
+        step(base, 0, true);
         close(base, 0);
-        in_group = 0;
+        step(base, 1, true);
+        close(base, 1);
+      } else {
+        if (in_group == 0) step(base, 0, true);
+        else step(base, 0, false);
+        step(base, 1, false);
+        if (++in_group == t.close || part * span + s + 1 == t.stages) {
+          close(base, 0);
+          in_group = 0;
+        }
       }
     }
     land(into);
@@ -381,11 +399,28 @@ __global__ __launch_bounds__(256 * WM, 2) void tile_kernel(TileArgs t) {
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // no load may reach LDS after this workgroup's end
 
+  if constexpr (WK == 2) {                              // the second part hands its sums to the first
+    f32x4 *red = reinterpret_cast<f32x4 *>(lds) + (wave % T::SET) * RBW * 4 * 64 + lane;
+    __syncthreads();
+    if (part == 1) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < RBW; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) red[(i * 4 + q) * 64] = out[i][q];
+    }
+    __syncthreads();
+    if (part == 1) return;
+#pragma unroll
+    for (int i = 0; i < RBW; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) out[i][q] += red[(i * 4 + q) * 64];
+  }
+
+#pragma unroll
+  for (int i = 0; i < RBW; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int m = wm * 64 + 16 * i + 4 * g4 + r;
+      const int m = wm * 16 * RBW + 16 * i + 4 * g4 + r;
       if (m >= tile.rows) continue;
       const int64_t n = n0 + wn * 64 + 4 * l16, at = (int64_t)(tile.row0 + m) * N + n;
       if (n + 4 <= N) {
@@ -398,30 +433,41 @@ __global__ __launch_bounds__(256 * WM, 2) void tile_kernel(TileArgs t) {
     }
 }
 
-template <int XT, int BITS, int ZL, bool HALF, int WM> static int tile_one(hipStream_t s, const TileArgs &t) {
-  using T = TileShape<XT, BITS, ZL, HALF, WM>;
-  const int64_t blocks = round_up64(tile_bound(t.a.P, t.a.E, T::BM) * ceil_div64(t.a.C, TILE_BN), 8);
+template <int XT, int BITS, int ZL, bool HALF, int RBW, int WM, int WN, int WK>
+static int tile_one(hipStream_t s, const TileArgs &t) {
+  using T = TileShape<XT, BITS, ZL, HALF, RBW, WM, WN, WK>;
+  const void *kernel = (const void *)tile_kernel<XT, BITS, ZL, HALF, RBW, WM, WN, WK>;
+  const int64_t blocks = round_up64(tile_bound(t.a.P, t.a.E, T::BM) * ceil_div64(t.a.C, T::BN), 8);
   if (blocks * T::THREADS >= (int64_t)1 << 32) return GPTQ_HIP_EINVAL;
-  if (!gptq_raise_lds_limit((const void *)tile_kernel<XT, BITS, ZL, HALF, WM>, T::LDS)) return GPTQ_HIP_ELAUNCH;
-  tile_kernel<XT, BITS, ZL, HALF, WM><<<(unsigned)blocks, T::THREADS, T::LDS, s>>>(t);
+  if (!gptq_raise_lds_limit(kernel, T::LDS)) return GPTQ_HIP_ELAUNCH;
+  tile_kernel<XT, BITS, ZL, HALF, RBW, WM, WN, WK><<<(unsigned)blocks, T::THREADS, T::LDS, s>>>(t);
   GPTQ_CHECK_LAUNCH();
   return GPTQ_HIP_OK;
 }
-template <int XT, int BITS, int WM> static int tile_tables(hipStream_t s, const TileArgs &t, bool half, int zl) {
+template <int XT, int BITS, int RBW, int WM, int WN, int WK>
+static int tile_tables(hipStream_t s, const TileArgs &t, bool half, int zl) {
   if (half) {
-    if (zl == 4) return tile_one<XT, BITS, 4, true, WM>(s, t);
-    if (zl == 2) return tile_one<XT, BITS, 2, true, WM>(s, t);
-    return tile_one<XT, BITS, 0, true, WM>(s, t);
+    if (zl == 4) return tile_one<XT, BITS, 4, true, RBW, WM, WN, WK>(s, t);
+    if (zl == 2) return tile_one<XT, BITS, 2, true, RBW, WM, WN, WK>(s, t);
+    return tile_one<XT, BITS, 0, true, RBW, WM, WN, WK>(s, t);
   }
-  if (zl == 4) return tile_one<XT, BITS, 4, false, WM>(s, t);
-  if (zl == 2) return tile_one<XT, BITS, 2, false, WM>(s, t);
-  return tile_one<XT, BITS, 0, false, WM>(s, t);
+  if (zl == 4) return tile_one<XT, BITS, 4, false, RBW, WM, WN, WK>(s, t);
+  if (zl == 2) return tile_one<XT, BITS, 2, false, RBW, WM, WN, WK>(s, t);
+  return tile_one<XT, BITS, 0, false, RBW, WM, WN, WK>(s, t);
+}
+template <int XT, int BITS> static int tile_shape(hipStream_t s, const TileArgs &t, int shape, bool half, int zl) {
+  if (shape == TILE_32x128) return tile_tables<XT, BITS, 2, 1, 2, 2>(s, t, half, zl);
+  if constexpr (XT != GPTQ_HIP_F32) {
+    if (shape == TILE_64x128) return tile_tables<XT, BITS, 4, 1, 2, 2>(s, t, half, zl);
+    if (shape == TILE_128x256) return tile_tables<XT, BITS, 4, 2, 4, 1>(s, t, half, zl);
+  }
+  return tile_tables<XT, BITS, 4, 1, 4, 1>(s, t, half, zl);
 }
 
 // groups that are no multiple of a stage are closed after every k-step
 static inline bool tile_half(int64_t group) { return group % 64 != 0; }
 
-template <int XT> static int tile_launch(hipStream_t s, const ExpertArgs &a, int row_blocks, void *ws) {
+template <int XT> static int tile_launch(hipStream_t s, const ExpertArgs &a, int shape, void *ws) {
   const int64_t K = a.bits == 4 ? 2 * a.R : a.R;
   const bool half = tile_half(a.group);
   const Staged l = staged_layout(a.T, K, a.x_dtype, half);
@@ -435,14 +481,12 @@ template <int XT> static int tile_launch(hipStream_t s, const ExpertArgs &a, int
     stage_rows_kernel<XT, false><<<(unsigned)a.T, 256, l.per_row * 4, s>>>(a.x, K, l.Kp, l.per_row, l.row_bytes, half,
                                                                            group, rows, sums);
   GPTQ_CHECK_LAUNCH();
-  const TileArgs t = {a, rows, sums, l.row_bytes, l.Kp, l.per_row, (int)(l.Kp / TILE_BK), group / 64, a.group != 0};
+  const TileArgs t = {a, rows, sums, l.row_bytes, l.Kp, l.per_row, (int)(l.Kp / TILE_BK), half ? 1 : group / 64,
+                      a.group != 0};
   const bool aligned = a.C % 16 == 0 && (uintptr_t)a.packed % 16 == 0 && (uintptr_t)a.zero % 16 == 0 &&
                        (uintptr_t)a.scale % 16 == 0;
   const int zl = !aligned ? 0 : (a.zs_dtype == GPTQ_HIP_F32 ? 4 : 2);
-  if constexpr (XT != GPTQ_HIP_F32) {
-    if (row_blocks == 8) return a.bits == 4 ? tile_tables<XT, 4, 2>(s, t, half, zl) : tile_tables<XT, 8, 2>(s, t, half, zl);
-  }
-  return a.bits == 4 ? tile_tables<XT, 4, 1>(s, t, half, zl) : tile_tables<XT, 8, 1>(s, t, half, zl);
+  return a.bits == 4 ? tile_shape<XT, 4>(s, t, shape, half, zl) : tile_shape<XT, 8>(s, t, shape, half, zl);
 }
 
 }  // namespace xqmm

@@ -2,6 +2,6 @@
 // side).
 #include "expert_tile.h"
 
-int expert_tile_bf16(hipStream_t s, const ExpertArgs &a, int row_blocks, void *ws) {
-  return xqmm::tile_launch<GPTQ_HIP_BF16>(s, a, row_blocks, ws);
+int expert_tile_bf16(hipStream_t s, const ExpertArgs &a, int shape, void *ws) {
+  return xqmm::tile_launch<GPTQ_HIP_BF16>(s, a, shape, ws);
 }
