@@ -9,6 +9,7 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bfloat8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // loads of 4, 8, 16 bytes at any address that fits the element type
@@ -62,12 +63,18 @@ template <> struct Op<GPTQ_HIP_F16> {
   static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
   }
+  static __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+  }
 };
 template <> struct Op<GPTQ_HIP_BF16> {
   static constexpr int PARTS = 1;
   static constexpr uint32_t ONE = 0x3F803F80u;
   static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bfloat8, a), __builtin_bit_cast(bfloat8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bfloat8, a), __builtin_bit_cast(bfloat8, b), c, 0, 0, 0);
   }
 };
 template <> struct Op<GPTQ_HIP_F32> : Op<GPTQ_HIP_BF16> {
@@ -81,43 +88,46 @@ __device__ __forceinline__ uint32_t opaque(uint32_t v) {
   return v;
 }
 
-// Packed rows of one k-step (32 input features) that a lane holds, and how their bytes become B operands.  Lane
-// (l16, g) owns features 8 g .. 8 g + 7 of the step: 4 packed rows of 4-bit codes, 8 of 8-bit codes.
+// Packed rows that a lane holds for 8 input features, and how one byte of each becomes a B operand: 4 packed rows of
+// 4-bit codes, 8 of 8-bit codes.
 template <int XT, int BITS> struct Codes {
   static constexpr int ROWS = BITS == 4 ? 4 : 8;
   static constexpr bool CONVERT = XT == GPTQ_HIP_F32 || (XT == GPTQ_HIP_BF16 && BITS == 8);
   static constexpr float OFFSET = (CONVERT || BITS == 8) ? 0.f : (XT == GPTQ_HIP_BF16 ? 128.f : 64.f);
   // features in the order 0 2 1 3 4 6 5 7 (4-bit codes taken pairwise from two rows): the activations are dealt alike
-  static constexpr bool DEALT = BITS == 4 && !CONVERT;
+  static constexpr bool DEALT = BITS == 4;
 
   static __device__ __forceinline__ uint32_t pair_f32(float a, float b) {      // {bf16(a), bf16(b)}, exact here
     return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x07060302u);
   }
   static __device__ __forceinline__ float byte_f32(uint32_t w, int q) { return (float)((w >> (8 * q)) & 255u); }
 
-  // B operand of byte q (0 .. 3) of the dwords r[0 .. ROWS - 1]
-  static __device__ __forceinline__ u32x4 operand(const uint32_t *r, int q) {
+  // the byte permutation that takes byte q (0 .. 3) of two rows into the halves of a word
+  static __device__ __forceinline__ uint32_t select(int q) { return 0x0C040C00u + 0x00010001u * (uint32_t)q; }
+  // B operand of the selected byte of the dwords r[0 .. ROWS - 1]
+  static __device__ __forceinline__ u32x4 operand(const uint32_t *r, uint32_t sel) {
     u32x4 b;
-    if (CONVERT && BITS == 4) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        b[i] = pair_f32(byte_f32(r[i] & 0x0F0F0F0Fu, q), byte_f32((r[i] >> 4) & 0x0F0F0F0Fu, q));
-    } else if (CONVERT) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) b[i] = pair_f32(byte_f32(r[2 * i], q), byte_f32(r[2 * i + 1], q));
-    } else if (BITS == 8) {
+    if (BITS == 8) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t p = __builtin_amdgcn_perm(r[2 * i + 1], r[2 * i], 0x0C040C00u + 0x00010001u * q);
-        const half2 v = __builtin_bit_cast(half2, p | 0x64006400u) - half2{(_Float16)1024.f, (_Float16)1024.f};
-        b[i] = __builtin_bit_cast(uint32_t, v);
+        const uint32_t p = __builtin_amdgcn_perm(r[2 * i + 1], r[2 * i], sel);
+        if (CONVERT) {
+          b[i] = pair_f32(byte_f32(p, 0), byte_f32(p, 2));
+        } else {
+          const half2 v = __builtin_bit_cast(half2, p | 0x64006400u) - half2{(_Float16)1024.f, (_Float16)1024.f};
+          b[i] = __builtin_bit_cast(uint32_t, v);
+        }
       }
     } else {
       const uint32_t bias = opaque(XT == GPTQ_HIP_BF16 ? 0x43004300u : 0x54005400u);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const uint32_t p = __builtin_amdgcn_perm(r[2 * i + 1], r[2 * i], 0x0C040C00u + 0x00010001u * q);
-        if (XT == GPTQ_HIP_BF16) {
+        const uint32_t p = __builtin_amdgcn_perm(r[2 * i + 1], r[2 * i], sel);
+        if (CONVERT) {
+          const uint32_t lo = p & 0x000F000Fu, hi = (p >> 4) & 0x000F000Fu;
+          b[2 * i] = pair_f32(byte_f32(lo, 0), byte_f32(lo, 2));
+          b[2 * i + 1] = pair_f32(byte_f32(hi, 0), byte_f32(hi, 2));
+        } else if (XT == GPTQ_HIP_BF16) {
           b[2 * i] = (p & 0x000F000Fu) | bias;
           b[2 * i + 1] = ((p >> 4) & 0x000F000Fu) | bias;
         } else {
@@ -222,16 +232,15 @@ __device__ __forceinline__ void store_out(void *out, bool f32, int64_t i, float 
   else ((typename Elem<XT>::type *)out)[i] = from_f32<typename Elem<XT>::type>(v);
 }
 
-// four neighbours of a row
-template <int XT>
-__device__ __forceinline__ void store4(void *out, bool f32, int64_t i, float a, float b, float c, float d) {
+// two neighbours of a row
+template <int XT> __device__ __forceinline__ void store2(void *out, bool f32, int64_t i, float a, float b) {
   typedef typename Elem<XT>::type E;
   if (f32) {
-    struct __attribute__((packed, aligned(4))) F4 { float v[4]; };
-    *reinterpret_cast<F4 *>((float *)out + i) = F4{{a, b, c, d}};
+    struct __attribute__((packed, aligned(4))) F2 { float v[2]; };
+    *reinterpret_cast<F2 *>((float *)out + i) = F2{{a, b}};
   } else {
-    struct __attribute__((packed, aligned(sizeof(E)))) E4 { E v[4]; };
-    *reinterpret_cast<E4 *>((E *)out + i) = E4{{from_f32<E>(a), from_f32<E>(b), from_f32<E>(c), from_f32<E>(d)}};
+    struct __attribute__((packed, aligned(sizeof(E)))) E2 { E v[2]; };
+    *reinterpret_cast<E2 *>((E *)out + i) = E2{{from_f32<E>(a), from_f32<E>(b)}};
   }
 }
 

@@ -9,7 +9,7 @@
 // no partial result leaves it: no workspace, no counter, no second launch.
 // Codes enter the matrix cores exactly; the group's sum of activations comes from one more product against ones; the
 // scale and the zero point (with the codes' offset) are applied to the fp32 sums group by group.
-// A lane loads CW consecutive bytes of a packed row; byte q of all lanes' rows is channel CW l16 + q: product tile q.
+// In a k-step of 32 features lane (l16, g) owns features 8 g .. 8 g + 7; it loads CW consecutive bytes of a packed row; byte q of all lanes' rows is channel CW l16 + q: product tile q.
 #pragma once
 #include "expert_common.h"
 
@@ -139,7 +139,11 @@ template <int XT, int BITS, int ZT, int KS, int RB, int CW> struct Strip {
 #pragma unroll
       for (int t = 0; t < KS; ++t) {
         if constexpr (XT == GPTQ_HIP_F32) parts3(u.x[b][t][0], u.x[b][t][XW - 1], a[b][t]);
-        else a[b][t][0] = C::DEALT ? deal(u.x[b][t][0]) : u.x[b][t][0];
+        else a[b][t][0] = u.x[b][t][0];
+        if (C::DEALT) {
+#pragma unroll
+          for (int p = 0; p < O::PARTS; ++p) a[b][t][p] = deal(a[b][t][p]);
+        }
 #pragma unroll
         for (int p = 0; p < O::PARTS; ++p) sum[b] = O::mma(a[b][t][p], ones, sum[b]);
       }
@@ -154,7 +158,7 @@ template <int XT, int BITS, int ZT, int KS, int RB, int CW> struct Strip {
       for (int b = 0; b < RB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int t = 0; t < KS; ++t) {
-        const u32x4 w = C::operand(u.w[t][q / 4], q & 3);
+        const u32x4 w = C::operand(u.w[t][q / 4], C::select(q & 3));
 #pragma unroll
         for (int b = 0; b < RB; ++b)
 #pragma unroll

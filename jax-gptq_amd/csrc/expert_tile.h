@@ -98,7 +98,8 @@ __global__ __launch_bounds__(256) void stage_rows_kernel(const void *__restrict_
         u32x4 part[3];
         parts3(v[0], v[1], part);
 #pragma unroll
-        for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4 *>(dst + p * Kp * 2 + k * 2) = part[p];
+        for (int p = 0; p < 3; ++p)
+          *reinterpret_cast<u32x4 *>(dst + p * Kp * 2 + k * 2) = DEALT ? deal(part[p]) : part[p];
       } else {
         *reinterpret_cast<u32x4 *>(dst + k * 2) = DEALT ? deal(v[0]) : v[0];
       }
@@ -146,19 +147,21 @@ template <int XT, int BITS, int ZL, bool HALF, int RBW, int WM, int WN, int WK> 
   // one part's rows, codes, zeros and scales (of a group), sums; then all parts'
   static constexpr int AP = PARTS * BM * 128, BP = BROWS * BN, ZP = 2 * BN * 4, SP = MB * 256;
   static constexpr int A = WK * AP, B = WK * BP, Z = WK * HN * ZP, S = WK * HN * SP;
-  static constexpr int STAGE = A + B + Z + S;
+  // a stage's rows and codes, and its tables, in rings of their own: rows and codes are in registers half a stage before
+  // the tables are needed, so their place is free one stage earlier
+  static constexpr int DATA = A + B, TABLE = Z + S, STAGE = DATA + TABLE;
   // up to four stages; workgroups of four wavefronts leave room for a second one on the CU where that takes no more
   // than a stage
-  static constexpr int ROOM = WAVES == 4 && 3 * STAGE <= 80 * 1024 ? 80 * 1024 : 160 * 1024;
+  static constexpr int ROOM = (WAVES == 4 && 2 * STAGE + TABLE <= 80 * 1024 ? 80 * 1024 : 160 * 1024) - TABLE;
   static constexpr int STAGES = 4 * STAGE <= ROOM ? 4 : (3 * STAGE <= ROOM ? 3 : 2);
-  static constexpr int LDS = STAGES * STAGE;
+  static constexpr int LDS = STAGES * STAGE + TABLE;
   // loads of a wavefront per stage
   static constexpr int AI = A / 1024 / WAVES, BI = B / 1024 / WAVES;
   static constexpr int SI = WK * HN * MB, TI = WK * HN * (BN / 128), ITEMS = SI + TI;
   static constexpr int MI = (ITEMS + WAVES - 1) / WAVES;
   static constexpr int LOADS = AI + BI + MI;
-  static_assert(A % (1024 * WAVES) == 0 && B % (1024 * WAVES) == 0 && STAGES * STAGE <= 160 * 1024, "whole loads");
-  static_assert(WK == 1 || SET * RBW * 4 * 1024 <= LDS, "partial tiles fit");
+  static_assert(A % (1024 * WAVES) == 0 && B % (1024 * WAVES) == 0 && LDS <= 160 * 1024, "whole loads");
+  static_assert(RBW % 2 == 0 && (WK == 1 || SET * RBW * 4 * 1024 <= LDS), "partial tiles fit");
 };
 
 template <int XT, int BITS, int ZL, bool HALF, int RBW, int WM, int WN, int WK>
@@ -169,7 +172,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
   typedef __attribute__((address_space(3))) char lds_char;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const ExpertArgs &a = t.a;
-  const int lane = threadIdx.x & 63, l16 = lane & 15, g4 = lane >> 4;
+  const int lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int part = wave / T::SET, wm = wave / WN % WM, wn = wave % WN;
   const int64_t N = a.C;
@@ -242,8 +245,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
   u32x4 breg[ZL ? 1 : T::BI];
   float zreg[ZL ? 1 : TABLE_REGS];
 
-  auto issue = [&](int s, int slot) __attribute__((always_inline)) {
-    const uint32_t base = lds0 + slot * T::STAGE;
+  auto issue = [&](int s, int slot, int table) __attribute__((always_inline)) {
+    const uint32_t base = lds0 + slot * T::DATA, tbase = lds0 + T::STAGES * T::DATA + table * T::TABLE;
 #pragma unroll
     for (int j = 0; j < T::AI; ++j) {
       const int i = wave * T::AI + j, p = i / (T::AP / 1024), q = i % (T::AP / 1024) / (T::BM / 8);
@@ -268,7 +271,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
       const int it = (wave + T::WAVES * j) % T::ITEMS;   // (more wavefronts than items: the same bytes twice)
       if (it < T::SI) {
         const int q = it / T::MB, h = q % T::HN, st = stage_of(q / T::HN, s);
-        to_lds_4(srow[j] + (HALF ? 2 * st + h : st), base + T::A + T::B + T::Z + it * 256);
+        to_lds_4(srow[j] + (HALF ? 2 * st + h : st), tbase + T::Z + it * 256);
       } else if constexpr (ZL != 0) {
         // zeros, then scales: 1 KB each at 256 channels, half a load each at 128
         const int i = it - T::SI, q = i / (T::BN / 128);
@@ -276,7 +279,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
         int64_t n = ZB == 4 ? n0 + 4 * l : n0 + 8 * (l % (T::BN / 8));
         n = n < N ? n : 0;
         to_lds_16((which ? scale : zero) + (table_row(stage_of(q / T::HN, s), q % T::HN) * N + n) * ZB,
-                  base + T::A + T::B + i * 1024);
+                  tbase + i * 1024);
       }
     }
     if constexpr (!ZL) {
@@ -290,146 +293,191 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
       }
     }
   };
-  auto land = [&](int slot) __attribute__((always_inline)) {      // what passed through registers
+  auto land = [&](int slot, int table) __attribute__((always_inline)) {      // what passed through registers
     if constexpr (!ZL) {
-      char *base = lds + slot * T::STAGE;
+      char *base = lds + slot * T::DATA;
 #pragma unroll
       for (int j = 0; j < T::BI; ++j)
         *reinterpret_cast<u32x4 *>(base + T::A + (wave * T::BI + j) * 1024 + lane * 16) = breg[j];
 #pragma unroll
       for (int j = 0; j < TABLE_REGS; ++j)
-        *reinterpret_cast<float *>(base + T::A + T::B + (threadIdx.x + j * T::THREADS) * 4) = zreg[j];
+        *reinterpret_cast<float *>(lds + T::STAGES * T::DATA + table * T::TABLE + (threadIdx.x + j * T::THREADS) * 4) =
+            zreg[j];
     }
   };
 
-  f32x4 out[RBW][4], acc[RBW][4];                       // [row block][byte of the codes]
+  // 32 x 32 products over 16 features: row (column) l32, features 8 hi .. + 7; sums lie with column l32, rows
+  // 8 (r / 4) + 4 hi + r % 4.  Column block c of a wavefront's 64 channels: channel 4 (l32 % 16) + 2 (l32 / 16) + c, so
+  // that a dword of codes serves two lanes and a lane's two channels are neighbours.
+  constexpr int RB = RBW / 2;
+  const int mycol = 4 * (l32 & 15) + 2 * (l32 >> 4);
+  const uint32_t sel[2] = {C::select(2 * (l32 >> 4)), C::select(2 * (l32 >> 4) + 1)};
+  f32x16 out[RB][2], acc[RB][2];                        // [row block][column block]
 #pragma unroll
-  for (int i = 0; i < RBW; ++i)
+  for (int i = 0; i < RB; ++i)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) out[i][q] = acc[i][q] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) out[i][c][r] = acc[i][c][r] = 0.f;
 
-  auto close = [&](const char *base, int h) __attribute__((always_inline)) {
-    const char *zp = base + T::A + T::B + (part * T::HN + h) * T::ZP;
-    const char *sums = base + T::A + T::B + T::Z + (part * T::HN + h) * T::SP;
-    float z[4], s[4];
-    const int col = wn * 64 + 4 * l16;
+  auto close = [&](int table, int h) __attribute__((always_inline)) {
+    const char *zp = lds + T::STAGES * T::DATA + table * T::TABLE + (part * T::HN + h) * T::ZP;
+    const char *sums = lds + T::STAGES * T::DATA + table * T::TABLE + T::Z + (part * T::HN + h) * T::SP;
+    float z[2], s[2];
+    const int col = wn * 64 + mycol;
     if constexpr (ZB == 4) {
-      const f32x4 zv = *reinterpret_cast<const f32x4 *>(zp + col * 4);
-      const f32x4 sv = *reinterpret_cast<const f32x4 *>(zp + T::BN * 4 + col * 4);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) { z[q] = zv[q]; s[q] = sv[q]; }
+      const float2 zv = *reinterpret_cast<const float2 *>(zp + col * 4);
+      const float2 sv = *reinterpret_cast<const float2 *>(zp + T::BN * 4 + col * 4);
+      z[0] = zv.x; z[1] = zv.y; s[0] = sv.x; s[1] = sv.y;
     } else {
       const bool bf = a.zs_dtype == GPTQ_HIP_BF16;
+      const uint32_t zw = *reinterpret_cast<const uint32_t *>(zp + col * 2);
+      const uint32_t sw = *reinterpret_cast<const uint32_t *>(zp + T::BN * 4 + col * 2);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const uint32_t zh = *reinterpret_cast<const uint16_t *>(zp + (col + q) * 2);
-        const uint32_t sh = *reinterpret_cast<const uint16_t *>(zp + T::BN * 4 + (col + q) * 2);
-        z[q] = bf ? __builtin_bit_cast(float, zh << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)zh);
-        s[q] = bf ? __builtin_bit_cast(float, sh << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)sh);
+      for (int c = 0; c < 2; ++c) {
+        const uint32_t zh = (zw >> (16 * c)) & 0xFFFFu, sh = (sw >> (16 * c)) & 0xFFFFu;
+        z[c] = bf ? __builtin_bit_cast(float, zh << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)zh);
+        s[c] = bf ? __builtin_bit_cast(float, sh << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)sh);
       }
     }
 #pragma unroll
-    for (int i = 0; i < RBW; ++i) {
-      const f32x4 sum = *reinterpret_cast<const f32x4 *>(sums + (wm * 16 * RBW + 16 * i + 4 * g4) * 4);
+    for (int i = 0; i < RB; ++i)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
+      for (int j = 0; j < 4; ++j) {
+        const f32x4 sum = *reinterpret_cast<const f32x4 *>(sums + (wm * 16 * RBW + 32 * i + 8 * j + 4 * hi) * 4);
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          out[i][q][r] = fmaf(s[q], fmaf(-(z[q] + C::OFFSET), sum[r], acc[i][q][r]), out[i][q][r]);
-    }
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            out[i][c][4 * j + r] = fmaf(s[c], fmaf(-(z[c] + C::OFFSET), sum[r], acc[i][c][4 * j + r]), out[i][c][4 * j + r]);
+      }
   };
-  auto step = [&](const char *base, int ks, bool fresh) __attribute__((always_inline)) {
-    u32x4 x[RBW][T::PARTS];
+  struct Step {                                         // operands of 32 features: rows, and codes as they are
+    u32x4 x[2][RB][T::PARTS];
+    uint32_t r[2][C::ROWS];
+  };
+  auto fetch = [&](Step &f, int slot, int ks) __attribute__((always_inline)) {
+    const char *base = lds + slot * T::DATA;
 #pragma unroll
-    for (int i = 0; i < RBW; ++i)
+    for (int v = 0; v < 2; ++v) {
+      const int g = 2 * v + hi;                         // 8 features g of the 32; (16 features per product)
+      const int chunk = (wn * 4 + ((l32 & 15) >> 2)) ^ (T::BN == 128 ? 4 * (g & 1) : 4 * g);
 #pragma unroll
-      for (int p = 0; p < T::PARTS; ++p)
-        x[i][p] = *reinterpret_cast<const u32x4 *>(base + part * T::AP + p * T::BM * 128 +
-                                                   (wm * 16 * RBW + 16 * i + l16) * 128 +
-                                                   (((4 * ks + g4) ^ (l16 & 7)) * 16));
-    uint32_t r[C::ROWS];
-    const int chunk = (wn * 4 + (l16 >> 2)) ^ (T::BN == 128 ? 4 * (g4 & 1) : 4 * g4);
+      for (int i = 0; i < C::ROWS; ++i) {
+        const int row = (BITS == 4 ? 16 : 32) * ks + C::ROWS * g + (T::BN == 128 ? i ^ (g >> 1) : i);
+        f.r[v][i] =
+            *reinterpret_cast<const uint32_t *>(base + T::A + part * T::BP + row * T::BN + chunk * 16 + (l32 & 3) * 4);
+      }
 #pragma unroll
-    for (int i = 0; i < C::ROWS; ++i) {
-      const int row = (BITS == 4 ? 16 : 32) * ks + C::ROWS * g4 + (T::BN == 128 ? i ^ (g4 >> 1) : i);
-      r[i] = *reinterpret_cast<const uint32_t *>(base + T::A + part * T::BP + row * T::BN + chunk * 16 + (l16 & 3) * 4);
-    }
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const u32x4 w = C::operand(r, q);
-#pragma unroll
-      for (int i = 0; i < RBW; ++i)
+      for (int i = 0; i < RB; ++i)
 #pragma unroll
         for (int p = 0; p < T::PARTS; ++p)
-          acc[i][q] = O::mma(x[i][p], w, fresh && p == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[i][q]);
+          f.x[v][i][p] = *reinterpret_cast<const u32x4 *>(base + part * T::AP + p * T::BM * 128 +
+                                                          (wm * 16 * RBW + 32 * i + l32) * 128 +
+                                                          (((4 * ks + g) ^ (l32 & 7)) * 16));
     }
   };
-
-  // stages past the last load it again: every stage then has the same number of loads in flight
-  constexpr int AHEAD = T::STAGES - 1;
+  auto multiply = [&](Step &f, bool fresh) __attribute__((always_inline)) {
+    f32x16 none;
 #pragma unroll
-  for (int s = 0; s < AHEAD; ++s) {
-    issue(s, s);
-    land(s);
-  }
-  int in_group = 0, slot = 0, into = AHEAD;
-  for (int s = 0; s < span; ++s) {
-    wait_and_meet<ZL ? (AHEAD - 1) * T::LOADS : 0>();
-    issue(s + AHEAD, into);
-    const char *base = lds + slot * T::STAGE;
-    if (WK == 1 || part * span + s < t.stages) {
-      if constexpr (HALF) {
-        step(base, 0, true);
-        close(base, 0);
-        step(base, 1, true);
-        close(base, 1);
-      } else {
-        if (in_group == 0) step(base, 0, true);
-        else step(base, 0, false);
-        step(base, 1, false);
-        if (++in_group == t.close || part * span + s + 1 == t.stages) {
-          close(base, 0);
-          in_group = 0;
-        }
+    for (int r = 0; r < 16; ++r) none[r] = 0.f;
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const u32x4 w = C::operand(f.r[v], sel[c]);
+#pragma unroll
+        for (int i = 0; i < RB; ++i)
+#pragma unroll
+          for (int p = 0; p < T::PARTS; ++p)
+            acc[i][c] = O::mma32(f.x[v][i][p], w, fresh && v == 0 && p == 0 ? none : acc[i][c]);
       }
+  };
+
+  // The operands of a k-step are fetched from LDS while the one before is multiplied; the second half of a stage
+  // starts with the barrier that publishes the next stage and frees this one's rows and codes.
+  // (fp32: two sets of operands do not fit the registers, a k-step's are fetched when the one before is done.)
+  constexpr bool EARLY = T::PARTS == 1;
+  constexpr int NS = T::STAGES;
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    issue(s, s, s);
+    land(s, s);
+  }
+  wait_and_meet<ZL ? (NS - 1) * T::LOADS : 0>();
+  Step f0, f1;
+  fetch(f0, 0, 0);
+  int slot = 0, table = 0, fresh_table = NS;
+  auto stage = [&](int s, bool fresh, bool last) __attribute__((always_inline)) {
+    const bool live = WK == 1 || part * span + s < t.stages;
+    if (EARLY) fetch(f1, slot, 1);
+    if (live) {
+      multiply(f0, HALF || fresh);
+      if constexpr (HALF) close(table, 0);
     }
-    land(into);
-    slot = slot + 1 == T::STAGES ? 0 : slot + 1;
-    into = into + 1 == T::STAGES ? 0 : into + 1;
+    if (!EARLY) fetch(f1, slot, 1);
+    wait_and_meet<ZL ? (NS - 2) * T::LOADS : 0>();
+    issue(s + NS, slot, fresh_table);
+    const int next = slot + 1 == NS ? 0 : slot + 1;
+    if (EARLY) fetch(f0, next, 0);
+    if (live) {
+      multiply(f1, HALF);
+      if (HALF || last || part * span + s + 1 == t.stages) close(table, HALF ? 1 : 0);
+    }
+    if (!EARLY) fetch(f0, next, 0);
+    land(slot, fresh_table);
+    slot = next;
+    table = table == NS ? 0 : table + 1;
+    fresh_table = fresh_table == NS ? 0 : fresh_table + 1;
+  };
+  if constexpr (HALF) {
+    for (int s = 0; s < span; ++s) stage(s, true, true);
+  } else {
+    for (int s = 0; s < span;) {
+      stage(s, true, t.close == 1);
+      ++s;
+      for (int j = 2; j <= t.close && s < span; ++j, ++s) stage(s, false, j == t.close);
+    }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // no load may reach LDS after this workgroup's end
 
   if constexpr (WK == 2) {                              // the second part hands its sums to the first
-    f32x4 *red = reinterpret_cast<f32x4 *>(lds) + (wave % T::SET) * RBW * 4 * 64 + lane;
+    f32x4 *red = reinterpret_cast<f32x4 *>(lds) + (wave % T::SET) * RB * 2 * 4 * 64 + lane;
     __syncthreads();
     if (part == 1) {
 #pragma unroll
-      for (int i = 0; i < RBW; ++i)
+      for (int i = 0; i < RB; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) red[(i * 4 + q) * 64] = out[i][q];
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            red[((i * 2 + c) * 4 + j) * 64] =
+                f32x4{out[i][c][4 * j], out[i][c][4 * j + 1], out[i][c][4 * j + 2], out[i][c][4 * j + 3]};
     }
     __syncthreads();
     if (part == 1) return;
 #pragma unroll
-    for (int i = 0; i < RBW; ++i)
+    for (int i = 0; i < RB; ++i)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) out[i][q] += red[(i * 4 + q) * 64];
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const f32x4 v = red[((i * 2 + c) * 4 + j) * 64];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) out[i][c][4 * j + r] += v[r];
+        }
   }
 
+  const int64_t n = n0 + wn * 64 + mycol;
 #pragma unroll
-  for (int i = 0; i < RBW; ++i)
+  for (int i = 0; i < RB; ++i)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int m = wm * 16 * RBW + 16 * i + 4 * g4 + r;
-      if (m >= tile.rows) continue;
-      const int64_t n = n0 + wn * 64 + 4 * l16, at = (int64_t)(tile.row0 + m) * N + n;
-      if (n + 4 <= N) {
-        store4<XT>(a.out, f32, at, out[i][0][r], out[i][1][r], out[i][2][r], out[i][3][r]);
-      } else {
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (n + q < N) store_out<XT>(a.out, f32, at + q, out[i][q][r]);
-      }
+    for (int r = 0; r < 16; ++r) {
+      const int m = wm * 16 * RBW + 32 * i + 8 * (r / 4) + 4 * hi + r % 4;
+      if (m >= tile.rows || n >= N) continue;
+      const int64_t at = (int64_t)(tile.row0 + m) * N + n;
+      if (n + 1 < N) store2<XT>(a.out, f32, at, out[i][0][r], out[i][1][r]);
+      else store_out<XT>(a.out, f32, at, out[i][0][r]);
     }
 }
 
