@@ -15,12 +15,12 @@ struct ExpertArgs {
   int top_k, E, bits, x_dtype, zs_dtype, out_dtype, transpose;
 };
 
-// rows of one expert by strips of channels (expert_strip.h), 16 * row_blocks rows at a time
-int expert_strip_f16(hipStream_t s, const ExpertArgs &a, int row_blocks);
-int expert_strip_bf16(hipStream_t s, const ExpertArgs &a, int row_blocks);
-int expert_strip_f32(hipStream_t s, const ExpertArgs &a, int row_blocks);
-// the same by tiles (expert_tile.h) of these rows x channels; fp32 activations: the first and the third
-enum { TILE_32x128, TILE_64x128, TILE_64x256, TILE_128x256 };
+// 16 rows of one expert at a time by strips of channels (expert_strip.h)
+int expert_strip_f16(hipStream_t s, const ExpertArgs &a);
+int expert_strip_bf16(hipStream_t s, const ExpertArgs &a);
+int expert_strip_f32(hipStream_t s, const ExpertArgs &a);
+// the same by tiles (expert_tile.h) of these rows x channels; K2: K in two halves, side by side
+enum { TILE_32x128_K2, TILE_32x256, TILE_64x256, TILE_64x256_K2 };
 int expert_tile_f16(hipStream_t s, const ExpertArgs &a, int shape, void *ws);
 int expert_tile_bf16(hipStream_t s, const ExpertArgs &a, int shape, void *ws);
 int expert_tile_f32(hipStream_t s, const ExpertArgs &a, int shape, void *ws);

@@ -116,9 +116,9 @@ static int simple_run(hipStream_t s, const ExpertArgs &a) {
 
 static bool float_type(int dt) { return dt == GPTQ_HIP_F32 || dt == GPTQ_HIP_F16 || dt == GPTQ_HIP_BF16; }
 
-static int strip_run(hipStream_t s, const ExpertArgs &a, int row_blocks) {
-  if (a.x_dtype == GPTQ_HIP_F32) return expert_strip_f32(s, a, row_blocks);
-  return a.x_dtype == GPTQ_HIP_F16 ? expert_strip_f16(s, a, row_blocks) : expert_strip_bf16(s, a, row_blocks);
+static int strip_run(hipStream_t s, const ExpertArgs &a) {
+  if (a.x_dtype == GPTQ_HIP_F32) return expert_strip_f32(s, a);
+  return a.x_dtype == GPTQ_HIP_F16 ? expert_strip_f16(s, a) : expert_strip_bf16(s, a);
 }
 
 static int tile_run(hipStream_t s, const ExpertArgs &a, int shape, void *ws) {
@@ -134,16 +134,27 @@ static int back_run(hipStream_t s, const ExpertArgs &a, void *ws) {
 // Which kernel a product runs on.
 struct Choice {
   enum Kind { SIMPLE, STRIP, TILE, BACK } kind;
-  int shape;                // STRIP: blocks of 16 rows; TILE: TILE_*
+  int shape;                // TILE_*
 };
+// By the rows of an expert, on average, and by whether tiles of 256 channels, one row of them per expert, fill the 256
+// CUs.  Each kernel costs the same for 1 row as for all that its tile holds, so a wider tile pays once the rows fill
+// half of it or so; where columns are few, strips of 128 channels and halves of K bring more workgroups.  Measured, us a
+// call (strip / 32 x 128 in halves of K / 32 x 256 / 64 x 256 / 64 x 256 in halves of K):
+//   8 experts 4096 x 11008:  4 rows 53 66 67 83 93,  24: 100 81 71 83 95,  48: 161 113 108 92 105,  128: - 237 206 172 197
+//   64 experts 2048 x 1424:  4 rows 49 43 43 52 61,  24: 92 56 47 57 67,   48: 145 79 70 62 73,     128: - 170 143 117 137
+//   8 experts 11008 x 4096:  4 rows 45 76 125 152 112,  24: 88 97 126 153 117,  48: 133 107 130 155 119,
+//                            96: - 184 164 158 132,  128: - 228 259 201 225
 static Choice choose(int64_t P, int E, int64_t C, int64_t group, int x_dtype, int transpose) {
   if ((group && group % 32) || C < 16) return {Choice::SIMPLE, 0};
-  if (transpose) return {Choice::BACK, 8};
-  const int64_t rows = P / E;                   // of an expert, on average
-  if (rows <= 12 && C >= 128) return {Choice::STRIP, 1};
-  if (rows <= 24) return {Choice::TILE, TILE_32x128};
-  if (x_dtype == GPTQ_HIP_F32) return {Choice::TILE, rows <= 40 ? TILE_32x128 : TILE_64x256};
-  return {Choice::TILE, rows <= 80 ? TILE_64x128 : TILE_128x256};
+  if (transpose) return {Choice::BACK, 0};
+  const int64_t rows = P / E;
+  if ((P < E ? P : E) * ceil_div64(C, 256) >= 256) {
+    if (rows < 8 && C >= 128) return {Choice::STRIP, 0};
+    return {Choice::TILE, rows <= 24 ? TILE_32x256 : TILE_64x256};
+  }
+  if (rows <= 24 && C >= 128) return {Choice::STRIP, 0};
+  if (rows <= 48) return {Choice::TILE, TILE_32x128_K2};
+  return {Choice::TILE, rows <= 96 && x_dtype != GPTQ_HIP_F32 ? TILE_64x256_K2 : TILE_64x256};
 }
 
 // GPTQ_HIP_OK, or why the product is refused
@@ -190,7 +201,7 @@ int gptq_hip_expert_qmatmul(void *stream, const void *x, int x_dtype, int64_t x_
   if (a.P == 0) return GPTQ_HIP_OK;
   hipStream_t s = as_stream(stream);
   const Choice c = choose(a.P, a.E, a.C, a.group, a.x_dtype, a.transpose);
-  if (c.kind == Choice::STRIP) return strip_run(s, a, c.shape);
+  if (c.kind == Choice::STRIP) return strip_run(s, a);
   const size_t need = gptq_hip_expert_qmatmul_workspace_bytes(a.T, a.P, a.R, a.C, a.bits, a.group, a.E, a.x_dtype,
                                                               a.zs_dtype, a.transpose);
   if (need && (!ws || ws_bytes < need)) return GPTQ_HIP_EWORKSPACE;

@@ -1,6 +1,6 @@
-// Few rows per expert: y[p, n] for 16 RB rows of one expert and a strip of 16 CW channels, over all of K.
+// Few rows per expert: y[p, n] for 16 rows of one expert and a strip of 16 CW channels, over all of K.
 //
-//   y[p, n] = sum_G s[G, n] (sum_{k in G} x[p, k] c[k, n] - (z[G, n]) sum_{k in G} x[p, k])
+//   y[p, n] = sum_G s[G, n] (sum_{k in G} x[p, k] (o + c[k, n]) - (o + z[G, n]) sum_{k in G} x[p, k])
 //
 // Bound by the weights' bytes (every expert that any row picked is read once from HBM as long as its rows fit one
 // tile).  Each of the eight wavefronts takes every eighth unit of 32 KS input features and multiplies all rows of the
@@ -9,15 +9,18 @@
 // no partial result leaves it: no workspace, no counter, no second launch.
 // Codes enter the matrix cores exactly; the group's sum of activations comes from one more product against ones; the
 // scale and the zero point (with the codes' offset) are applied to the fp32 sums group by group.
-// In a k-step of 32 features lane (l16, g) owns features 8 g .. 8 g + 7; it loads CW consecutive bytes of a packed row; byte q of all lanes' rows is channel CW l16 + q: product tile q.
+// In a k-step of 32 features lane (l16, g) owns features 8 g .. 8 g + 7; it loads CW consecutive bytes of a packed row;
+// byte q of all lanes' rows is channel CW l16 + q: product tile q.  Weights go to registers as they are needed there;
+// the activations of 16 rows, which as operands would be 16-byte pieces of 16 places, go to LDS in whole lines.
 #pragma once
-#include "expert_common.h"
+#include "expert_tile.h"
 
 namespace xqmm {
 
 constexpr int STRIP_WAVES = 8;
 
-template <int XT, int BITS, int ZT, int KS, int RB, int CW> struct Strip {
+// DMA: the rows' features travel through LDS (16-byte aligned rows); else through registers.
+template <int XT, int BITS, int ZT, int KS, int CW, bool DMA> struct Strip {
   using C = Codes<XT, BITS>;
   using O = Op<XT>;
   static constexpr int ZB = ZT == GPTQ_HIP_F32 ? 4 : 2; // bytes of a table's element
@@ -28,23 +31,29 @@ template <int XT, int BITS, int ZT, int KS, int RB, int CW> struct Strip {
   struct Unit {
     uint32_t w[KS][DW][C::ROWS];
     uint32_t z[ZD], s[ZD];
-    u32x4 x[RB][KS][XW];
+    u32x4 x[DMA ? 1 : KS][XW];
   };
+  // a unit's 16 rows in LDS, a wavefront's own: 16-byte chunks of a row lie turned by its number, so that the reads of
+  // 8 neighbouring lanes (rows) meet all banks
+  static constexpr int SZ = XT == GPTQ_HIP_F32 ? 4 : 2, CPR = SPAN * SZ / 16, PIECE = 16 * SPAN * SZ;
+  static __device__ __forceinline__ int turn(int row) { return CPR >= 8 ? row & 7 : (row >> 2) & 3; }
   struct Ctx {
     const uint8_t *w;             // packed row 0 of the expert (the same for all lanes, as all pointers but x)
     const char *zero, *scale;     // table row 0
-    const char *x[RB];            // the lane's rows of x, at the lane group's first feature
+    const char *x;                // the lane's row of x, at the lane group's first feature
+    const char *row[PIECE / 1024];   // DMA: the rows whose chunks the lane fetches, at those chunks
     int64_t K, R, N;
     uint32_t col, at_w, at_z;     // the lane's first channel; its bytes past `w` and past the tables' rows
     uint32_t magic;               // unit -> table row: 0 (all channels), 1 (a row each), else floor(2^32 / units a row) + 1
     int g4;
   };
 
-  // TAIL: the unit may reach past K.  Activations from there are zero, the other loads are kept inside.
-  template <bool TAIL> static __device__ __forceinline__ void load(Unit &u, const Ctx &c, int unit) {
-    load_weights<TAIL>(u, c, unit);
-    load_rows<TAIL>(u, c, unit);
+  // the rows' features of a unit on their way to LDS; the loads of the unit's weights come behind them
+  static __device__ __forceinline__ void send_rows(const Ctx &c, int unit, uint32_t lds) {
+#pragma unroll
+    for (int i = 0; i < PIECE / 1024; ++i) to_lds_16(c.row[i] + (int64_t)unit * SPAN * SZ, lds + i * 1024);
   }
+  // TAIL: the unit may reach past K.  Activations from there are zero, the other loads are kept inside.
   template <bool TAIL> static __device__ __forceinline__ void load_weights(Unit &u, const Ctx &c, int unit) {
     const uint8_t *wu = c.w + (int64_t)unit * (BITS == 4 ? SPAN / 2 : SPAN) * c.N;
 #pragma unroll
@@ -83,40 +92,48 @@ template <int XT, int BITS, int ZT, int KS, int RB, int CW> struct Strip {
       }
     }
   }
-  template <bool TAIL> static __device__ __forceinline__ void load_rows(Unit &u, const Ctx &c, int unit) {
-    constexpr int SZ = XT == GPTQ_HIP_F32 ? 4 : 2;
+  template <bool TAIL> static __device__ __forceinline__ void load_rows(u32x4 (*x)[XW], const Ctx &c, int unit) {
+    const char *xu = c.x + (int64_t)unit * SPAN * SZ;
 #pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      const char *xu = c.x[b] + (int64_t)unit * SPAN * SZ;
+    for (int t = 0; t < KS; ++t) {
+      const int64_t k = (int64_t)unit * SPAN + 32 * t + 8 * c.g4;
+      if (!TAIL || k + 8 <= c.K) {
 #pragma unroll
-      for (int t = 0; t < KS; ++t) {
-        const int64_t k = (int64_t)unit * SPAN + 32 * t + 8 * c.g4;
-        if (!TAIL || k + 8 <= c.K) {
+        for (int v = 0; v < XW; ++v) x[t][v] = load16(xu + 32 * t * SZ + 16 * v);
+      } else {
 #pragma unroll
-          for (int v = 0; v < XW; ++v) u.x[b][t][v] = load16(xu + 32 * t * SZ + 16 * v);
-        } else {
+        for (int v = 0; v < XW; ++v) {
 #pragma unroll
-          for (int v = 0; v < XW; ++v) {
-#pragma unroll
-            for (int d = 0; d < 4; ++d) {
-              uint32_t word = 0;
-              if (SZ == 4) {
-                if (k + 4 * v + d < c.K) word = ((const uint32_t *)xu)[32 * t + 4 * v + d];
-              } else {
-                const uint16_t *p = (const uint16_t *)xu + 32 * t;
-                if (k + 2 * d < c.K) word = p[2 * d];
-                if (k + 2 * d + 1 < c.K) word |= (uint32_t)p[2 * d + 1] << 16;
-              }
-              u.x[b][t][v][d] = word;
+          for (int d = 0; d < 4; ++d) {
+            uint32_t word = 0;
+            if (SZ == 4) {
+              if (k + 4 * v + d < c.K) word = ((const uint32_t *)xu)[32 * t + 4 * v + d];
+            } else {
+              const uint16_t *p = (const uint16_t *)xu + 32 * t;
+              if (k + 2 * d < c.K) word = p[2 * d];
+              if (k + 2 * d + 1 < c.K) word |= (uint32_t)p[2 * d + 1] << 16;
             }
+            x[t][v][d] = word;
           }
         }
       }
     }
   }
+  // A unit's features from LDS.  They have arrived: a load of the unit's weights, issued behind them, has (naming its
+  // register makes the compiler wait for it, and loads return in order).
+  static __device__ __forceinline__ void read_rows(u32x4 (*x)[XW], const Unit &u, const Ctx &c, const char *lds, int l16) {
+    asm volatile("" : : "v"(u.w[KS - 1][DW - 1][C::ROWS - 1]) : "memory");
+#pragma unroll
+    for (int t = 0; t < KS; ++t)
+#pragma unroll
+      for (int v = 0; v < XW; ++v) {
+        const int chunk = (4 * t + c.g4) * XW + v;
+        x[t][v] = *reinterpret_cast<const u32x4 *>(lds + l16 * SPAN * SZ + (chunk ^ turn(l16)) * 16);
+      }
+  }
 
   // the lane's channels of a table row in fp32
-  static __device__ __forceinline__ void table(const uint32_t *raw, const Ctx &c, float *v) {
+  static __device__ __forceinline__ void table(const uint32_t *raw, float *v) {
 #pragma unroll
     for (int q = 0; q < CW; ++q) {
       if (ZB == 4) {
@@ -129,59 +146,51 @@ template <int XT, int BITS, int ZT, int KS, int RB, int CW> struct Strip {
     }
   }
 
-  static __device__ __forceinline__ void multiply(Unit &u, const Ctx &c, f32x4 out[RB][CW]) {
-    u32x4 a[RB][KS][O::PARTS];
-    f32x4 sum[RB];
+  static __device__ __forceinline__ void multiply(const Unit &u, u32x4 (*x)[XW], const Ctx &c, f32x4 out[CW]) {
+    u32x4 a[KS][O::PARTS];
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
     const u32x4 ones = {O::ONE, O::ONE, O::ONE, O::ONE};
 #pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      sum[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < KS; ++t) {
+      if constexpr (XT == GPTQ_HIP_F32) parts3(x[t][0], x[t][XW - 1], a[t]);
+      else a[t][0] = x[t][0];
 #pragma unroll
-      for (int t = 0; t < KS; ++t) {
-        if constexpr (XT == GPTQ_HIP_F32) parts3(u.x[b][t][0], u.x[b][t][XW - 1], a[b][t]);
-        else a[b][t][0] = u.x[b][t][0];
-        if (C::DEALT) {
-#pragma unroll
-          for (int p = 0; p < O::PARTS; ++p) a[b][t][p] = deal(a[b][t][p]);
-        }
-#pragma unroll
-        for (int p = 0; p < O::PARTS; ++p) sum[b] = O::mma(a[b][t][p], ones, sum[b]);
+      for (int p = 0; p < O::PARTS; ++p) {
+        if (C::DEALT) a[t][p] = deal(a[t][p]);
+        sum = O::mma(a[t][p], ones, sum);
       }
     }
     float z[CW], s[CW];
-    table(u.z, c, z);
-    table(u.s, c, s);
+    table(u.z, z);
+    table(u.s, s);
 #pragma unroll
     for (int q = 0; q < CW; ++q) {
-      f32x4 acc[RB];
-#pragma unroll
-      for (int b = 0; b < RB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int t = 0; t < KS; ++t) {
         const u32x4 w = C::operand(u.w[t][q / 4], C::select(q & 3));
 #pragma unroll
-        for (int b = 0; b < RB; ++b)
-#pragma unroll
-          for (int p = 0; p < O::PARTS; ++p) acc[b] = O::mma(a[b][t][p], w, acc[b]);
+        for (int p = 0; p < O::PARTS; ++p) acc = O::mma(a[t][p], w, acc);
       }
       const float zq = -(z[q] + C::OFFSET), sq = s[q];
 #pragma unroll
-      for (int b = 0; b < RB; ++b)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) out[b][q][r] = fmaf(sq, fmaf(zq, sum[b][r], acc[b][r]), out[b][q][r]);
+      for (int r = 0; r < 4; ++r) out[q][r] = fmaf(sq, fmaf(zq, sum[r], acc[r]), out[q][r]);
     }
   }
 };
 
-template <int XT, int BITS, int ZT, int KS, int RB, int CW>
+template <int XT, int BITS, int ZT, int KS, int CW, bool DMA>
 __global__ __launch_bounds__(STRIP_WAVES * 64) void strip_kernel(ExpertArgs a) {
-  using S = Strip<XT, BITS, ZT, KS, RB, CW>;
+  using S = Strip<XT, BITS, ZT, KS, CW, DMA>;
   constexpr int ZB = S::ZB;
-  constexpr int H = 16 * RB;
-  __shared__ f32x4 red[STRIP_WAVES / 2][RB * CW][64];
+  // register sets and pieces of LDS that the units of a wavefront go round
+  constexpr int D = KS == 4 ? 2 : (BITS == 4 && XT != GPTQ_HIP_F32 ? 3 : 2);
+  constexpr int ROWS_LDS = DMA ? STRIP_WAVES * D * S::PIECE : 0, RED_LDS = STRIP_WAVES / 2 * CW * 1024;
+  typedef __attribute__((address_space(3))) char lds_char;
+  __shared__ __attribute__((aligned(16))) char lds[ROWS_LDS > RED_LDS ? ROWS_LDS : RED_LDS];
   const int lane = threadIdx.x & 63, l16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Tile tile = find_tile(a.offsets, a.E, (int)a.P, H, blockIdx.y);
+  const Tile tile = find_tile(a.offsets, a.E, (int)a.P, 16, blockIdx.y);
   if (tile.rows <= 0) return;
   const int64_t N = a.C, K = BITS == 4 ? 2 * a.R : a.R;
   // (the last strip ends where N does; what it shares with the one before it is computed twice, to the same bits)
@@ -209,102 +218,117 @@ __global__ __launch_bounds__(STRIP_WAVES * 64) void strip_kernel(ExpertArgs a) {
   c.col = (uint32_t)col;
   c.at_w = (uint32_t)(S::C::ROWS * c.g4 * N + col);
   c.at_z = (uint32_t)(col * ZB);
-  f32x4 out[RB][CW];
+  auto row_of = [&](int m) -> const char * {
+    m = m < tile.rows ? m : tile.rows - 1;             // rows past the last repeat it and are not stored
+    return (const char *)a.x + x_row_of(a.order, a.top_k, a.T, tile.row0 + m) * K * S::SZ;
+  };
+  const uint32_t piece0 = (uint32_t)(uintptr_t)(lds_char *)lds + wave * D * S::PIECE;
+  if (DMA) {
 #pragma unroll
-  for (int b = 0; b < RB; ++b)
-#pragma unroll
-    for (int q = 0; q < CW; ++q) out[b][q] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < S::PIECE / 1024; ++i) {
+      const int row = i * (64 / S::CPR) + lane / S::CPR;
+      c.row[i] = row_of(row) + ((lane % S::CPR) ^ S::turn(row)) * 16;
+    }
+  }
+  c.x = row_of(l16) + 8 * c.g4 * S::SZ;
 
-  // units wave, wave + 8, ... through a ring of D register sets; the one that K ends in (no groups then) by itself
-  constexpr int D = KS == 4 ? 2 : (KS == 2 && BITS == 4 && XT != GPTQ_HIP_F32 ? 3 : (KS == 2 ? 2 : 3));
+  f32x4 out[CW];
+#pragma unroll
+  for (int q = 0; q < CW; ++q) out[q] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  // units wave, wave + 8, ...; the one that K ends in (no groups then) by itself
   const int whole = (int)(K / S::SPAN);
   const int mine = whole > wave ? (whole - wave + STRIP_WAVES - 1) / STRIP_WAVES : 0;
-  typename S::Unit ring[D];
-  // (the first weights are on their way while the rows' numbers are fetched)
   if (mine > 0) {
+    typename S::Unit ring[D];
+    // (past the end: the last unit once more, not multiplied)
+    auto load = [&](int d, int i) __attribute__((always_inline)) {
+      const int unit = wave + STRIP_WAVES * (i < mine ? i : mine - 1);
+      if constexpr (DMA) S::send_rows(c, unit, piece0 + d * S::PIECE);
+      S::template load_weights<false>(ring[d], c, unit);
+      if constexpr (!DMA) S::template load_rows<false>(ring[d].x, c, unit);
+    };
 #pragma unroll
-    for (int d = 0; d + 1 < D; ++d)
-      S::template load_weights<false>(ring[d], c, wave + STRIP_WAVES * (d < mine ? d : mine - 1));
-  }
-#pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    int m = 16 * b + l16;
-    m = m < tile.rows ? m : tile.rows - 1;             // rows past the last repeat it and are not stored
-    c.x[b] = (const char *)a.x + (x_row_of(a.order, a.top_k, a.T, tile.row0 + m) * K + 8 * c.g4) *
-                                     (XT == GPTQ_HIP_F32 ? 4 : 2);
-  }
-
-  if (mine > 0) {
-#pragma unroll
-    for (int d = 0; d + 1 < D; ++d)
-      S::template load_rows<false>(ring[d], c, wave + STRIP_WAVES * (d < mine ? d : mine - 1));
+    for (int d = 0; d + 1 < D; ++d) load(d, d);
     for (int i = 0; i < mine; i += D) {
 #pragma unroll
       for (int d = 0; d < D; ++d) {
-        // (past the end: the last unit once more, not multiplied)
-        const int next = i + d + D - 1 < mine ? i + d + D - 1 : mine - 1;
-        S::template load<false>(ring[(d + D - 1) % D], c, wave + STRIP_WAVES * next);
-        if (i + d < mine) S::multiply(ring[d], c, out);
+        load((d + D - 1) % D, i + d + D - 1);
+        if (i + d < mine) {
+          if constexpr (DMA) {
+            u32x4 x[KS][S::XW];
+            S::read_rows(x, ring[d], c, lds + (wave * D + d) * S::PIECE, l16);
+            S::multiply(ring[d], x, c, out);
+          } else {
+            S::multiply(ring[d], ring[d].x, c, out);
+          }
+        }
       }
     }
+    if (DMA) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // (the last loads reach LDS before it is used again)
   }
   if (K % S::SPAN && whole % STRIP_WAVES == wave) {
     typename S::Unit u;
-    S::template load<true>(u, c, whole);
-    S::multiply(u, c, out);
+    u32x4 x[KS][S::XW];
+    S::template load_weights<true>(u, c, whole);
+    S::template load_rows<true>(x, c, whole);
+    S::multiply(u, x, c, out);
   }
 
   // the eight partial tiles: the upper four wavefronts hand theirs to the lower four, whose sums are then added up
+  f32x4 *red = reinterpret_cast<f32x4 *>(lds);
+  __syncthreads();
   if (wave >= STRIP_WAVES / 2) {
 #pragma unroll
-    for (int b = 0; b < RB; ++b)
-#pragma unroll
-      for (int q = 0; q < CW; ++q) red[wave - STRIP_WAVES / 2][b * CW + q][lane] = out[b][q];
+    for (int q = 0; q < CW; ++q) red[((wave - STRIP_WAVES / 2) * CW + q) * 64 + lane] = out[q];
   }
   __syncthreads();
   if (wave < STRIP_WAVES / 2) {
 #pragma unroll
-    for (int b = 0; b < RB; ++b)
-#pragma unroll
-      for (int q = 0; q < CW; ++q) red[wave][b * CW + q][lane] += out[b][q];
+    for (int q = 0; q < CW; ++q) red[(wave * CW + q) * 64 + lane] += out[q];
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < RB * CW * 64; i += STRIP_WAVES * 64) {
-    const int l = i & 63, t = i >> 6;
-    f32x4 v = red[0][t][l];
+  for (int i = threadIdx.x; i < CW * 64; i += STRIP_WAVES * 64) {
+    const int l = i & 63, q = i >> 6;
+    f32x4 v = red[i];
 #pragma unroll
-    for (int w = 1; w < STRIP_WAVES / 2; ++w) v += red[w][t][l];
-    const int64_t n = n0 + CW * (l & 15) + t % CW;
+    for (int w = 1; w < STRIP_WAVES / 2; ++w) v += red[w * CW * 64 + i];
+    const int64_t n = n0 + CW * (l & 15) + q;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int m = 16 * (t / CW) + 4 * (l >> 4) + r;
+      const int m = 4 * (l >> 4) + r;
       if (m < tile.rows) store_out<XT>(a.out, f32, (int64_t)(tile.row0 + m) * N + n, v[r]);
     }
   }
 }
 
-// RB: blocks of 16 rows in a tile
-template <int XT, int RB, int CW> static int strip_launch(hipStream_t s, const ExpertArgs &a) {
-  const int64_t tiles = tile_bound(a.P, a.E, 16 * RB);
-  const dim3 grid((unsigned)ceil_div64(a.C, 16 * CW), (unsigned)tiles);
-  // the longest unit that lies in one group; four k-steps where the registers hold two such units
-  constexpr bool four = XT != GPTQ_HIP_F32;
-  const bool r4 = four && a.bits == 4;
-  const int ks = !a.group || a.group % 128 == 0 ? (r4 ? 4 : 2) : (a.group % 64 == 0 ? 2 : 1);
+template <int XT, int CW, bool DMA> static int strip_tables(hipStream_t s, const ExpertArgs &a, dim3 grid, int ks) {
 #define GPTQ_STRIP(B, S)                                                                                          \
   if (a.bits == B && ks == S) {                                                                                   \
     if (a.zs_dtype == GPTQ_HIP_F32)                                                                               \
-      strip_kernel<XT, B, GPTQ_HIP_F32, S, RB, CW><<<grid, STRIP_WAVES * 64, 0, s>>>(a);                          \
+      strip_kernel<XT, B, GPTQ_HIP_F32, S, CW, DMA><<<grid, STRIP_WAVES * 64, 0, s>>>(a);                         \
     else if (a.zs_dtype == GPTQ_HIP_F16)                                                                          \
-      strip_kernel<XT, B, GPTQ_HIP_F16, S, RB, CW><<<grid, STRIP_WAVES * 64, 0, s>>>(a);                          \
+      strip_kernel<XT, B, GPTQ_HIP_F16, S, CW, DMA><<<grid, STRIP_WAVES * 64, 0, s>>>(a);                         \
     else                                                                                                          \
-      strip_kernel<XT, B, GPTQ_HIP_BF16, S, RB, CW><<<grid, STRIP_WAVES * 64, 0, s>>>(a);                         \
+      strip_kernel<XT, B, GPTQ_HIP_BF16, S, CW, DMA><<<grid, STRIP_WAVES * 64, 0, s>>>(a);                        \
   }
-  if constexpr (four) { GPTQ_STRIP(4, 4) }
+  if constexpr (XT != GPTQ_HIP_F32) { GPTQ_STRIP(4, 4) }
   GPTQ_STRIP(4, 2) GPTQ_STRIP(4, 1) GPTQ_STRIP(8, 2) GPTQ_STRIP(8, 1)
 #undef GPTQ_STRIP
   GPTQ_CHECK_LAUNCH();
   return GPTQ_HIP_OK;
+}
+
+template <int XT> static int strip_launch(hipStream_t s, const ExpertArgs &a) {
+  constexpr int CW = 8;          // rows of 128 bytes: half as wide, every 128-byte line of memory is fetched twice (18.5
+                                 // against 10.5 us for the bare loads of 45 MB); 256 bytes, 13 - 14 us
+  const int64_t K = a.bits == 4 ? 2 * a.R : a.R;
+  const dim3 grid((unsigned)ceil_div64(a.C, 16 * CW), (unsigned)tile_bound(a.P, a.E, 16));
+  // the longest unit that lies in one group; four k-steps where the registers hold two such units
+  const bool r4 = XT != GPTQ_HIP_F32 && a.bits == 4;
+  const int ks = !a.group || a.group % 128 == 0 ? (r4 ? 4 : 2) : (a.group % 64 == 0 ? 2 : 1);
+  const bool dma = (uintptr_t)a.x % 16 == 0 && K * (XT == GPTQ_HIP_F32 ? 4 : 2) % 16 == 0;
+  return dma ? strip_tables<XT, CW, true>(s, a, grid, ks) : strip_tables<XT, CW, false>(s, a, grid, ks);
 }
 
 }  // namespace xqmm

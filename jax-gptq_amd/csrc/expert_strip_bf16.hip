@@ -2,7 +2,4 @@
 // side).
 #include "expert_strip.h"
 
-int expert_strip_bf16(hipStream_t s, const ExpertArgs &a, int row_blocks) {
-  if (row_blocks == 1) return xqmm::strip_launch<GPTQ_HIP_BF16, 1, 8>(s, a);
-  return xqmm::strip_launch<GPTQ_HIP_BF16, 2, 8>(s, a);
-}
+int expert_strip_bf16(hipStream_t s, const ExpertArgs &a) { return xqmm::strip_launch<GPTQ_HIP_BF16>(s, a); }

@@ -161,7 +161,7 @@ template <int XT, int BITS, int ZL, bool HALF, int RBW, int WM, int WN, int WK> 
   static constexpr int MI = (ITEMS + WAVES - 1) / WAVES;
   static constexpr int LOADS = AI + BI + MI;
   static_assert(A % (1024 * WAVES) == 0 && B % (1024 * WAVES) == 0 && LDS <= 160 * 1024, "whole loads");
-  static_assert(RBW % 2 == 0 && (WK == 1 || SET * RBW * 4 * 1024 <= LDS), "partial tiles fit");
+  static_assert(RBW % 2 == 0 && (WK == 1 || (WK - 1) * SET * RBW * 4 * 1024 <= LDS), "partial tiles fit");
 };
 
 template <int XT, int BITS, int ZL, bool HALF, int RBW, int WM, int WN, int WK>
@@ -441,31 +441,33 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // no load may reach LDS after this workgroup's end
 
-  if constexpr (WK == 2) {                              // the second part hands its sums to the first
-    f32x4 *red = reinterpret_cast<f32x4 *>(lds) + (wave % T::SET) * RB * 2 * 4 * 64 + lane;
+  if constexpr (WK > 1) {                               // the other parts hand their sums to the first
+    f32x4 *red = reinterpret_cast<f32x4 *>(lds) + wave % T::SET * RB * 8 * 64 + lane;
     __syncthreads();
-    if (part == 1) {
+    if (part > 0) {
 #pragma unroll
       for (int i = 0; i < RB; ++i)
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            red[((i * 2 + c) * 4 + j) * 64] =
+            red[((part - 1) * T::SET * RB * 8 + (i * 2 + c) * 4 + j) * 64] =
                 f32x4{out[i][c][4 * j], out[i][c][4 * j + 1], out[i][c][4 * j + 2], out[i][c][4 * j + 3]};
     }
     __syncthreads();
-    if (part == 1) return;
+    if (part > 0) return;
 #pragma unroll
     for (int i = 0; i < RB; ++i)
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const f32x4 v = red[((i * 2 + c) * 4 + j) * 64];
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) out[i][c][4 * j + r] += v[r];
-        }
+          for (int p = 0; p < WK - 1; ++p) {
+            const f32x4 v = red[(p * T::SET * RB * 8 + (i * 2 + c) * 4 + j) * 64];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) out[i][c][4 * j + r] += v[r];
+          }
   }
 
   const int64_t n = n0 + wn * 64 + mycol;
@@ -504,10 +506,10 @@ static int tile_tables(hipStream_t s, const TileArgs &t, bool half, int zl) {
   return tile_one<XT, BITS, 0, false, RBW, WM, WN, WK>(s, t);
 }
 template <int XT, int BITS> static int tile_shape(hipStream_t s, const TileArgs &t, int shape, bool half, int zl) {
-  if (shape == TILE_32x128) return tile_tables<XT, BITS, 2, 1, 2, 2>(s, t, half, zl);
-  if constexpr (XT != GPTQ_HIP_F32) {
-    if (shape == TILE_64x128) return tile_tables<XT, BITS, 4, 1, 2, 2>(s, t, half, zl);
-    if (shape == TILE_128x256) return tile_tables<XT, BITS, 4, 2, 4, 1>(s, t, half, zl);
+  if (shape == TILE_32x128_K2) return tile_tables<XT, BITS, 2, 1, 2, 2>(s, t, half, zl);
+  if (shape == TILE_32x256) return tile_tables<XT, BITS, 2, 1, 4, 1>(s, t, half, zl);
+  if constexpr (XT != GPTQ_HIP_F32) {                   // (three parts of 64 rows and both halves do not fit LDS)
+    if (shape == TILE_64x256_K2) return tile_tables<XT, BITS, 4, 1, 4, 2>(s, t, half, zl);
   }
   return tile_tables<XT, BITS, 4, 1, 4, 1>(s, t, half, zl);
 }
