@@ -84,7 +84,7 @@ __global__ __launch_bounds__(256, XT == GPTQ_HIP_F32 ? 1 : 2) void back_kernel(B
   constexpr float OFFSET = CONVERT ? 0.f : 128.f;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const ExpertArgs &a = t.a;
-  const int lane = threadIdx.x & 63, l16 = lane & 15, g4 = lane >> 4;
+  const int lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave >> 1, wn = wave & 1;
   const int64_t N = a.C, K = BITS == 4 ? 2 * a.R : a.R;
@@ -130,7 +130,9 @@ __global__ __launch_bounds__(256, XT == GPTQ_HIP_F32 ? 1 : 2) void back_kernel(B
     r = r < a.R ? r : a.R - 1;
     brow[j] = packed + r * N;
   }
-  const int bcol = 16 * (lane % CH);
+  // (rows of 64 bytes: chunks lie turned by every fourth row, so that reads of 8 neighbouring rows meet all banks)
+  auto turn = [](int row) -> int { return CH == 4 ? (row >> 2) & 3 : 0; };
+  const int bcol = 16 * ((lane % CH) ^ turn(lane / CH));
   const float *trow[T::ZI];
 #pragma unroll
   for (int j = 0; j < T::ZI; ++j) {
@@ -175,23 +177,28 @@ __global__ __launch_bounds__(256, XT == GPTQ_HIP_F32 ? 1 : 2) void back_kernel(B
     }
   };
 
-  f32x4 acc[4][8];                                      // [row block][column block]
-  float sub[NG][4];
+  // 32 x 32 products over 16 channels: row (column) l32, 8 channels a lane; sums lie with column l32, rows
+  // 8 (r / 4) + 4 hi + r % 4.  A lane's packed row gives it two columns at 4 bits (low and high codes), one at 8.
+  constexpr int CB = BITS == 4 ? 2 : 1;
+  f32x16 acc[2][4];                                     // [row block][column block]
+  float sub[NG][2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 2; ++i) {
 #pragma unroll
-    for (int c = 0; c < 8; ++c) acc[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][c][r] = 0.f;
 #pragma unroll
     for (int g = 0; g < NG; ++g) sub[g][i] = 0.f;
   }
 
-  // Lane group g4 owns channels 16 g4 + 8 h .. + 7 of a stage of 64 in k-step h: 16 bytes of a packed row (stages of
-  // 32: channels 8 g4 .. + 7, 32 bytes of activations).
-  auto step = [&](const char *base, int h) __attribute__((always_inline)) {
+  // Channels 32 u + 16 hi .. + 15 of a stage are the lane's in two products w: 16 bytes of a packed row.
+  auto step = [&](const char *base, int u, int w) __attribute__((always_inline)) {
+    const int n = 32 * u + 16 * hi + 8 * w;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       float z[8], s[8];
-      const char *zp = base + T::A + T::B + (wn * NG + g) * 256 + (T::BK == 64 ? (16 * g4 + 8 * h) : 8 * g4) * 4;
+      const char *zp = base + T::A + T::B + (wn * NG + g) * 256 + n * 4;
 #pragma unroll
       for (int v = 0; v < 2; ++v) {
         const f32x4 zv = *reinterpret_cast<const f32x4 *>(zp + 16 * v);
@@ -199,39 +206,37 @@ __global__ __launch_bounds__(256, XT == GPTQ_HIP_F32 ? 1 : 2) void back_kernel(B
 #pragma unroll
         for (int i = 0; i < 4; ++i) { z[4 * v + i] = zv[i] + OFFSET; s[4 * v + i] = sv[i]; }
       }
-      u32x4 x[4][T::PARTS];
+      u32x4 x[2][T::PARTS];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const char *row = base + (wm * 64 + 16 * i + l16) * 128;
-        float v[8];
-        if constexpr (XT == GPTQ_HIP_F32) {
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            const f32x4 q = *reinterpret_cast<const f32x4 *>(row + ((2 * g4 + w) ^ (l16 & 7)) * 16);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[4 * w + e] = q[e];
-          }
-        } else {
-          const u32x4 q = *reinterpret_cast<const u32x4 *>(row + ((2 * g4 + h) ^ (l16 & 7)) * 16);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const uint32_t w = q[e / 2];
-            const uint32_t half = (e & 1) ? w >> 16 : w & 0xFFFFu;
-            if (XT == GPTQ_HIP_BF16) v[e] = __builtin_bit_cast(float, (e & 1) ? w & 0xFFFF0000u : w << 16);
-            else v[e] = (float)__builtin_bit_cast(_Float16, (uint16_t)half);
-          }
-        }
+      for (int i = 0; i < 2; ++i) {
+        const char *row = base + (wm * 64 + 32 * i + l32) * 128;
         uint32_t part[T::PARTS][8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float p = v[e] * s[e];
-          if (T::PARTS == 2) p = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, p) & 0xFFFFFF00u);
-          sub[g][i] = fmaf(p, z[e], sub[g][i]);
-          part[0][e] = __builtin_bit_cast(uint32_t, p);
+        for (int e4 = 0; e4 < 2; ++e4) {                // 4 channels at a time (fp32), or of 8 (16 bits)
+          u32x4 q;
+          if (XT == GPTQ_HIP_F32) q = *reinterpret_cast<const u32x4 *>(row + ((n / 4 + e4) ^ (l32 & 7)) * 16);
+          else q = *reinterpret_cast<const u32x4 *>(row + ((n / 8) ^ (l32 & 7)) * 16);
 #pragma unroll
-          for (int c = 1; c < T::PARTS; ++c) {
-            p -= __builtin_bit_cast(float, part[c - 1][e] & 0xFFFF0000u);
-            part[c][e] = __builtin_bit_cast(uint32_t, p);
+          for (int k = 0; k < 4; ++k) {
+            const int e = 4 * e4 + k;
+            const uint32_t word = XT == GPTQ_HIP_F32 ? q[k] : q[e / 2];
+            float p;
+            if (XT == GPTQ_HIP_F32) {
+              p = __builtin_bit_cast(float, word) * s[e];
+            } else if (XT == GPTQ_HIP_BF16) {
+              p = __builtin_bit_cast(float, (e & 1) ? word & 0xFFFF0000u : word << 16) * s[e];
+            } else {                                    // (conversion and product in one instruction)
+              const uint16_t h = (uint16_t)((e & 1) ? word >> 16 : word);
+              p = fmaf((float)__builtin_bit_cast(_Float16, h), s[e], 0.f);
+            }
+            if (T::PARTS == 2) p = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, p) & 0xFFFFFF00u);
+            sub[g][i] = fmaf(p, z[e], sub[g][i]);
+            part[0][e] = __builtin_bit_cast(uint32_t, p);
+#pragma unroll
+            for (int c = 1; c < T::PARTS; ++c) {
+              p -= __builtin_bit_cast(float, part[c - 1][e] & 0xFFFF0000u);
+              part[c][e] = __builtin_bit_cast(uint32_t, p);
+            }
           }
         }
 #pragma unroll
@@ -240,23 +245,24 @@ __global__ __launch_bounds__(256, XT == GPTQ_HIP_F32 ? 1 : 2) void back_kernel(B
           for (int e = 0; e < 4; ++e)
             x[i][c][e] = __builtin_amdgcn_perm(part[c][2 * e + 1], part[c][2 * e], 0x07060302u);
       }
-      constexpr int RBS = (BITS == 4 ? 4 : 8) / NG;     // blocks of 16 packed rows
+      // blocks of 32 packed rows with columns in this group; a block of 4-bit codes and groups of 32 columns lies in two
+      // groups, each takes its half of the lanes
+      constexpr int RBS = 4 / CB, HALF_BLOCK = NG > RBS;
 #pragma unroll
-      for (int b = 0; b < RBS; ++b) {
-        const int row = wn * (T::ROWS / 2) + 16 * (g * RBS + b) + l16;
-        const uint2 w = *reinterpret_cast<const uint2 *>(base + T::A + row * T::BK +
-                                                         (T::BK == 64 ? 16 * g4 + 8 * h : 8 * g4));
-        constexpr int CB = BITS == 4 ? 2 : 1;
+      for (int b = HALF_BLOCK ? g / 2 : g * RBS / NG; b < (HALF_BLOCK ? g / 2 + 1 : (g + 1) * RBS / NG); ++b) {
+        const int row = wn * (T::ROWS / 2) + 32 * b + l32;
+        const uint2 d2 = *reinterpret_cast<const uint2 *>(
+            base + T::A + row * T::BK + (((n / 16) ^ turn(row)) * 16) + 8 * w);
         u32x4 op[CB];
         const uint32_t bias = opaque(0x43004300u);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t d = j < 2 ? w.x : w.y;
+          const uint32_t d = j < 2 ? d2.x : d2.y;
           const int q = 2 * (j & 1);
           if constexpr (CONVERT && BITS == 4) {
-            const uint32_t lo = d & 0x0F0F0F0Fu, hi = (d >> 4) & 0x0F0F0F0Fu;
+            const uint32_t lo = d & 0x0F0F0F0Fu, up = (d >> 4) & 0x0F0F0F0Fu;
             op[0][j] = Codes<XT, BITS>::pair_f32(Codes<XT, BITS>::byte_f32(lo, q), Codes<XT, BITS>::byte_f32(lo, q + 1));
-            op[CB - 1][j] = Codes<XT, BITS>::pair_f32(Codes<XT, BITS>::byte_f32(hi, q), Codes<XT, BITS>::byte_f32(hi, q + 1));
+            op[CB - 1][j] = Codes<XT, BITS>::pair_f32(Codes<XT, BITS>::byte_f32(up, q), Codes<XT, BITS>::byte_f32(up, q + 1));
           } else if constexpr (CONVERT) {
             op[0][j] = Codes<XT, BITS>::pair_f32(Codes<XT, BITS>::byte_f32(d, q), Codes<XT, BITS>::byte_f32(d, q + 1));
           } else {
@@ -265,15 +271,19 @@ __global__ __launch_bounds__(256, XT == GPTQ_HIP_F32 ? 1 : 2) void back_kernel(B
             op[CB - 1][j] = ((p >> 4) & 0x000F000Fu) | bias;
           }
         }
+        if (HALF_BLOCK) {
+          const uint32_t keep = (l32 >> 4) == (g & 1) ? 0xFFFFFFFFu : 0u;
+#pragma unroll
+          for (int c = 0; c < CB; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) op[c][j] &= keep;
+        }
 #pragma unroll
         for (int c = 0; c < CB; ++c)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int p = 0; p < T::PARTS; ++p) {
-              f32x4 &d = acc[i][(g * RBS + b) * CB + c];
-              d = O::mma(x[i][p], op[c], d);
-            }
+            for (int p = 0; p < T::PARTS; ++p) acc[i][b * CB + c] = O::mma32(x[i][p], op[c], acc[i][b * CB + c]);
       }
       // (one group's parts at a time: with those of the next made early the registers do not suffice)
       if (NG > 1) __builtin_amdgcn_sched_barrier(0);
@@ -292,35 +302,37 @@ __global__ __launch_bounds__(256, XT == GPTQ_HIP_F32 ? 1 : 2) void back_kernel(B
     issue(s + AHEAD < t.stages ? s + AHEAD : t.stages - 1, into);
     const char *base = lds + slot * T::STAGE;
 #pragma unroll
-    for (int h = 0; h < T::STEPS; ++h) step(base, h);
+    for (int h = 0; h < 2 * T::STEPS; ++h) step(base, h / 2, h % 2);
     land(into);
     slot = slot + 1 == T::STAGES ? 0 : slot + 1;
     into = into + 1 == T::STAGES ? 0 : into + 1;
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // no load may reach LDS after this workgroup's end
 
-  // the second sum lies with row l16 of each block, spread over the lane groups; results lie with rows 4 g4 + r
+  // the second sum lies with row l32 of each block, half of it in either half of the wavefront
 #pragma unroll
   for (int g = 0; g < NG; ++g)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      sub[g][i] += __shfl_xor(sub[g][i], 16);
-      sub[g][i] += __shfl_xor(sub[g][i], 32);
-    }
-  constexpr int CB = BITS == 4 ? 2 : 1, PERG = 8 / NG;
+    for (int i = 0; i < 2; ++i) sub[g][i] += __shfl_xor(sub[g][i], 32);
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int m = wm * 64 + 16 * i + 4 * g4 + r;
+    for (int r = 0; r < 16; ++r) {
+      const int in = 8 * (r / 4) + 4 * hi + r % 4, m = wm * 64 + 32 * i + in;
 #pragma unroll
-      for (int c = 0; c < 8; c += CB) {
-        const float d = __shfl(sub[c / PERG][i], 4 * g4 + r);
-        const int64_t k = k0 + wn * 128 + 16 * c + CB * l16;
-        if (m >= tile.rows) continue;
-#pragma unroll
-        for (int j = 0; j < CB; ++j)
-          if (k + j < K) store_out<XT>(a.out, f32, (int64_t)(tile.row0 + m) * K + k + j, acc[i][c + j][r] - d);
+      for (int b = 0; b < 4 / CB; ++b) {
+        float d;
+        if constexpr (NG > 4 / CB) {                    // two groups in a block
+          const float d0 = __shfl(sub[2 * b][i], in), d1 = __shfl(sub[2 * b + 1][i], in);
+          d = l32 < 16 ? d0 : d1;
+        } else {
+          d = __shfl(sub[b * NG * CB / 4][i], in);
+        }
+        const int64_t k = k0 + wn * 128 + CB * (32 * b + l32);
+        if (m >= tile.rows || k >= K) continue;
+        const int64_t at = (int64_t)(tile.row0 + m) * K + k;
+        if constexpr (CB == 2) store2<XT>(a.out, f32, at, acc[i][2 * b][r] - d, acc[i][2 * b + 1][r] - d);
+        else store_out<XT>(a.out, f32, at, acc[i][b][r] - d);
       }
     }
 }
