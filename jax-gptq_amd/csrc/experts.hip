@@ -10,9 +10,9 @@
 namespace {
 
 constexpr int MAX_EXPERTS = 1024;
-constexpr int SORT_CHUNK = 8192;       // pairs of one workgroup where there are several
+constexpr int SORT_CHUNK = 4096;       // pairs of one workgroup where there are several
 constexpr int SORT_MAX_GROUPS = 256;   // each of them reads the counts of all
-constexpr int SORT_LDS_WORDS = 12288;  // counters of a workgroup: one per wavefront and bucket
+constexpr int SORT_LDS_WORDS = 11264;  // counters of a workgroup: one per wavefront and bucket
 
 // bucket of a pair: its expert, or E for an id that names none (compared in 64 bits: 2^32 is not expert 0)
 template <typename ID>
@@ -55,11 +55,12 @@ __global__ __launch_bounds__(1024) void sort_kernel(const ID *__restrict__ ids, 
                                                     const int *__restrict__ counts, int n_chunks,
                                                     int *__restrict__ order, int *__restrict__ position,
                                                     int *__restrict__ offsets) {
-  extern __shared__ int hist[];          // [wavefronts][E + 1]
+  extern __shared__ int hist[];          // [wavefronts][E + 1], then two more rows where there are several chunks
   __shared__ int wave_sum[16];
   const int waves = blockDim.x >> 6, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int nb = E + 1;
-  for (int i = threadIdx.x; i < waves * nb; i += blockDim.x) hist[i] = 0;
+  int *all = hist + waves * nb, *before = all + nb;      // pairs of every bucket in all chunks and in those before
+  for (int i = threadIdx.x; i < (counts ? waves + 2 : waves) * nb; i += blockDim.x) hist[i] = 0;
   __syncthreads();
   const int64_t lo = (int64_t)blockIdx.x * chunk;
   const int64_t hi = lo + chunk < P ? lo + chunk : P;
@@ -68,6 +69,15 @@ __global__ __launch_bounds__(1024) void sort_kernel(const ID *__restrict__ ids, 
   const int64_t whi = wlo + per < hi ? wlo + per : hi;
   int *mine = hist + w * nb;
   for (int64_t i = wlo + lane; i < whi; i += 64) atomicAdd(&mine[bucket_of(ids[i], E)], 1);
+  if (counts) {
+    for (int i = threadIdx.x; i < n_chunks * nb; i += blockDim.x) {
+      const int v = counts[i], b = i % nb;
+      if (v) {
+        atomicAdd(&all[b], v);
+        if (i / nb < (int)blockIdx.x) atomicAdd(&before[b], v);
+      }
+    }
+  }
   __syncthreads();
 
   // thread t: `each` consecutive buckets, their totals summed, scanned over the workgroup
@@ -76,11 +86,8 @@ __global__ __launch_bounds__(1024) void sort_kernel(const ID *__restrict__ ids, 
   const int b1 = b0 + each < nb ? b0 + each : nb;
   int total = 0;
   for (int b = b0; b < b1; ++b) {
-    if (counts) {
-      for (int c = 0; c < n_chunks; ++c) total += counts[(int64_t)c * nb + b];
-    } else {
-      for (int v = 0; v < waves; ++v) total += hist[v * nb + b];
-    }
+    if (counts) total += all[b];
+    else for (int v = 0; v < waves; ++v) total += hist[v * nb + b];
   }
   int scan = total;
   for (int d = 1; d < 64; d <<= 1) {
@@ -93,23 +100,13 @@ __global__ __launch_bounds__(1024) void sort_kernel(const ID *__restrict__ ids, 
   for (int v = 0; v < w; ++v) base += wave_sum[v];
   for (int b = b0; b < b1; ++b) {
     if (blockIdx.x == 0) offsets[b] = base;      // bucket E: where the rows of nowhere begin
-    int at = base;
-    if (counts) {
-      int before = 0, all = 0;
-      for (int c = 0; c < n_chunks; ++c) {
-        const int v = counts[(int64_t)c * nb + b];
-        all += v;
-        if (c < (int)blockIdx.x) before += v;
-      }
-      at += before;
-      base += all;
-    }
+    int at = counts ? base + before[b] : base;
     for (int v = 0; v < waves; ++v) {
       const int n = hist[v * nb + b];
       hist[v * nb + b] = at;
       at += n;
     }
-    if (!counts) base = at;
+    base = counts ? base + all[b] : at;
   }
   __syncthreads();
 
@@ -152,27 +149,32 @@ __global__ __launch_bounds__(256) void gather_kernel(const T *__restrict__ x, in
                                                      const int *__restrict__ offsets, int E, int64_t P,
                                                      T *__restrict__ out) {
   using V = Vec<T>;
+  constexpr int EACH = 2;                          // pieces of a thread: both are loaded before either is stored
   const int64_t t = blockIdx.x;
-  const int64_t c = ((int64_t)blockIdx.y * 256 + threadIdx.x) * V::N;
-  if (c >= K) return;
   const int live = offsets[E];
-  const bool whole = c + V::N <= K;
-  typename V::Raw r;
-  if (whole) {
-    r = V::load(x + t * K + c);
-  } else {
-    for (int i = 0; i < V::N; ++i) r.v[i] = c + i < K ? x[t * K + c + i] : from_f32<T>(0.f);
+  int64_t c[EACH];
+  typename V::Raw r[EACH], zero;
+#pragma unroll
+  for (int u = 0; u < EACH; ++u) {
+    c[u] = (((int64_t)blockIdx.y * EACH + u) * 256 + threadIdx.x) * V::N;
+    if (c[u] + V::N <= K) {
+      r[u] = V::load(x + t * K + c[u]);
+    } else {
+      for (int i = 0; i < V::N; ++i) r[u].v[i] = c[u] + i < K ? x[t * K + c[u] + i] : from_f32<T>(0.f);
+    }
   }
-  typename V::Raw zero;
   for (int i = 0; i < V::N; ++i) zero.v[i] = from_f32<T>(0.f);
   for (int j = 0; j < top_k; ++j) {
     const int64_t p = position[t * top_k + j];
     if (p < 0 || p >= P) continue;
-    const typename V::Raw &s = p < live ? r : zero;
-    if (whole) {
-      V::store(out + p * K + c, s);
-    } else {
-      for (int i = 0; c + i < K; ++i) out[p * K + c + i] = s.v[i];
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) {
+      const typename V::Raw &s = p < live ? r[u] : zero;
+      if (c[u] + V::N <= K) {
+        V::store(out + p * K + c[u], s);
+      } else {
+        for (int i = 0; c[u] + i < K; ++i) out[p * K + c[u] + i] = s.v[i];
+      }
     }
   }
 }
@@ -194,14 +196,29 @@ __global__ __launch_bounds__(256) void combine_kernel(const T *__restrict__ y, i
   const bool whole = c + V::N <= N;
   float acc[V::N];
   for (int i = 0; i < V::N; ++i) acc[i] = 0.f;
-  for (int j = 0; j < top_k; ++j) {
-    const int64_t p = position[t * top_k + j];
-    if (p < 0 || p >= live) continue;
-    const float w = weight_at(weights, t * top_k + j);
-    if (whole) {
-      const typename V::Raw r = V::load(y + p * N + c);
-      for (int i = 0; i < V::N; ++i) acc[i] = fmaf(w, to_f32(r.v[i]), acc[i]);
-    } else {
+  if (whole) {
+    // four rows' loads in flight; a pair that goes nowhere reads row 0 in its place, which is left out of the sum
+    for (int j0 = 0; j0 < top_k; j0 += 4) {
+      typename V::Raw r[4];
+      bool in[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t p = j0 + j < top_k ? position[t * top_k + j0 + j] : -1;
+        in[j] = p >= 0 && p < live;
+        r[j] = V::load(y + (in[j] ? p : 0) * N + c);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (!in[j]) continue;
+        const float w = weight_at(weights, t * top_k + j0 + j);
+        for (int i = 0; i < V::N; ++i) acc[i] = fmaf(w, to_f32(r[j].v[i]), acc[i]);
+      }
+    }
+  } else {
+    for (int j = 0; j < top_k; ++j) {
+      const int64_t p = position[t * top_k + j];
+      if (p < 0 || p >= live) continue;
+      const float w = weight_at(weights, t * top_k + j);
       for (int i = 0; c + i < N; ++i) acc[i] = fmaf(w, to_f32(y[p * N + c + i]), acc[i]);
     }
   }
@@ -271,14 +288,14 @@ static int check_rows(int64_t T, int top_k, int64_t width, int E) {
   if (T >= (int64_t)1 << 24 || T * top_k > (int64_t)1 << 30 || width > (int64_t)1 << 25) return GPTQ_HIP_EINVAL;
   return GPTQ_HIP_OK;
 }
-template <typename T> static dim3 row_grid(int64_t rows, int64_t width) {
-  return dim3((unsigned)rows, (unsigned)ceil_div64(width, 256 * (16 / (int64_t)sizeof(T))));
+template <typename T> static dim3 row_grid(int64_t rows, int64_t width, int each) {
+  return dim3((unsigned)rows, (unsigned)ceil_div64(width, each * 256 * (16 / (int64_t)sizeof(T))));
 }
 
 template <typename T, typename TO, typename TW>
 static int combine_launch(hipStream_t s, const void *y, int64_t T_, int top_k, int64_t N, const int *position,
                           const int *offsets, int E, const void *weights, void *out) {
-  const dim3 grid = row_grid<T>(T_, N);
+  const dim3 grid = row_grid<T>(T_, N, 1);
   combine_kernel<T, TO, TW><<<grid, 256, 0, s>>>((const T *)y, top_k, N, position, offsets, E, T_ * top_k,
                                                  (const TW *)weights, (TO *)out);
   GPTQ_CHECK_LAUNCH();
@@ -328,7 +345,7 @@ static int sort_launch(hipStream_t s, const void *ids, int64_t P, int E, int *or
   const int n = (int)ceil_div64(P, chunk), waves = sort_waves(chunk, E);
   sort_count_kernel<ID><<<n, 1024, (size_t)(E + 1) * 4, s>>>(p, P, chunk, E, counts);
   GPTQ_CHECK_LAUNCH();
-  sort_kernel<ID><<<n, waves * 64, (size_t)waves * (E + 1) * 4, s>>>(p, P, chunk, E, counts, n, order, position,
+  sort_kernel<ID><<<n, waves * 64, (size_t)(waves + 2) * (E + 1) * 4, s>>>(p, P, chunk, E, counts, n, order, position,
                                                                      offsets);
   GPTQ_CHECK_LAUNCH();
   return GPTQ_HIP_OK;
@@ -366,11 +383,11 @@ int gptq_hip_expert_gather(void *stream, const void *x, int dtype, int64_t token
   hipStream_t s = as_stream(stream);
   const int64_t P = tokens * top_k;
   if (dtype == GPTQ_HIP_F32) {
-    const dim3 grid = row_grid<float>(tokens, K);
+    const dim3 grid = row_grid<float>(tokens, K, 2);
     gather_kernel<float><<<grid, 256, 0, s>>>((const float *)x, top_k, K, position, offsets, n_experts, P,
                                               (float *)out);
   } else {                                        // 16-bit rows are copied as they are
-    const dim3 grid = row_grid<__half>(tokens, K);
+    const dim3 grid = row_grid<__half>(tokens, K, 2);
     gather_kernel<__half><<<grid, 256, 0, s>>>((const __half *)x, top_k, K, position, offsets, n_experts, P,
                                                (__half *)out);
   }
