@@ -90,18 +90,9 @@ __global__ __launch_bounds__(256, XT == GPTQ_HIP_F32 ? 1 : 2) void back_kernel(B
   const int64_t N = a.C, K = BITS == 4 ? 2 * a.R : a.R;
   const bool f32 = a.out_dtype == GPTQ_HIP_F32;
 
-  // the tile, in the order of the untransposed tiles
-  const int row_tiles = count_tiles(a.offsets, a.E, (int)a.P, T::BM);
-  const int cols = (int)((K + T::BN - 1) / T::BN);
-  const int64_t total = (int64_t)row_tiles * cols, run = (total + 7) / 8;
-  const int64_t pos = blockIdx.x >> 3, item = (blockIdx.x & 7) * run + pos;
-  if (pos >= run || item >= total) return;
-  const int panel = (int)(item / ((int64_t)row_tiles * 4));
-  const int rest = (int)(item - (int64_t)panel * row_tiles * 4);
-  const int width = cols - 4 * panel < 4 ? cols - 4 * panel : 4;
-  const int64_t k0 = (int64_t)(4 * panel + rest % width) * T::BN;
-  const Tile tile = find_tile(a.offsets, a.E, (int)a.P, T::BM, rest / width);
+  const Item tile = find_item<4>(a.offsets, a.E, (int)a.P, T::BM, (uint32_t)((K + T::BN - 1) / T::BN));
   if (tile.rows <= 0) return;
+  const int64_t k0 = (int64_t)tile.col * T::BN;
   if (tile.expert == a.E) {                            // rows of nowhere
     for (int i = threadIdx.x; i < tile.rows * T::BN; i += T::THREADS) {
       const int64_t k = k0 + i % T::BN;
@@ -340,10 +331,10 @@ __global__ __launch_bounds__(256, XT == GPTQ_HIP_F32 ? 1 : 2) void back_kernel(B
 template <int XT, int BITS, bool ALIGNED, int NG> static int back_one(hipStream_t s, const BackArgs &t) {
   using T = BackShape<XT, BITS, ALIGNED, NG>;
   const int64_t K = BITS == 4 ? 2 * t.a.R : t.a.R;
-  const int64_t blocks = round_up64(tile_bound(t.a.P, t.a.E, T::BM) * ceil_div64(K, T::BN), 8);
-  if (blocks * T::THREADS >= (int64_t)1 << 32) return GPTQ_HIP_EINVAL;
+  const unsigned blocks = item_grid(t.a.P, t.a.E, T::BM, ceil_div64(K, T::BN), T::THREADS);
+  if (!blocks) return GPTQ_HIP_EINVAL;
   if (!gptq_raise_lds_limit((const void *)back_kernel<XT, BITS, ALIGNED, NG>, T::LDS)) return GPTQ_HIP_ELAUNCH;
-  back_kernel<XT, BITS, ALIGNED, NG><<<(unsigned)blocks, T::THREADS, T::LDS, s>>>(t);
+  back_kernel<XT, BITS, ALIGNED, NG><<<blocks, T::THREADS, T::LDS, s>>>(t);
   GPTQ_CHECK_LAUNCH();
   return GPTQ_HIP_OK;
 }

@@ -166,54 +166,73 @@ __device__ __forceinline__ void parts3(const u32x4 &lo4, const u32x4 &hi4, u32x4
   }
 }
 
-// Which rows a workgroup owns: tiles of H rows are counted expert by expert (the rows of nowhere as one more), and
-// tile number `tile` is found by a scan over the experts, 64 at a time.  Every wavefront does it for itself.
-struct Tile {
-  int expert, row0, rows;        // rows == 0: there is no such tile
+// Which rows and columns a workgroup owns.  Tiles of H rows are counted expert by expert (the rows of nowhere as one
+// more) and each comes with `cols` columns; PANEL columns at a time (0: all), all tiles of them, make the list of items.
+// Workgroups go round the eight XCDs; each XCD takes a run of the list, so what runs on it at a time shares rows and
+// weights (and lines that two neighbouring strips begin in) in its L2.  The counts come from a scan over the experts, 64
+// at a time; every wavefront does it for itself.
+struct Item {
+  int expert, row0, rows, col;        // rows == 0: nothing to do
 };
-__device__ __forceinline__ Tile find_tile(const int *__restrict__ offsets, int E, int P, int H, int tile) {
+template <int PANEL>
+__device__ __forceinline__ Item find_item(const int *__restrict__ offsets, int E, int P, int H, uint32_t cols) {
   const int lane = threadIdx.x & 63;
-  int before = 0;
-  for (int e0 = 0; e0 <= E; e0 += 64) {
-    const int e = e0 + lane;
-    int lo = 0, hi = 0;
+  auto tiles_of = [&](int e, int &lo, int &hi) -> int {
+    lo = hi = 0;
     if (e <= E) {
       lo = offsets[e];
       hi = e < E ? offsets[e + 1] : P;
     }
-    const int n = (hi - lo + H - 1) / H;
-    int scan = n;
+    return (hi - lo + H - 1) / H;
+  };
+  auto scan_of = [&](int n) -> int {
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-      const int up = __shfl_up(scan, d);
-      if (lane >= d) scan += up;
+      const int up = __shfl_up(n, d);
+      if (lane >= d) n += up;
+    }
+    return n;
+  };
+  int lo, hi, n = tiles_of(lane, lo, hi), scan = scan_of(n), total = __shfl(scan, 63);
+  if (E >= 64) {
+    int more = 0, l, h;
+    for (int e = 64 + lane; e <= E; e += 64) more += tiles_of(e, l, h);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) more += __shfl_xor(more, d);
+    total += more;
+  }
+  const uint32_t tiles = (uint32_t)__builtin_amdgcn_readfirstlane(total), items = tiles * cols, run = (items + 7) / 8;
+  const uint32_t pos = blockIdx.x >> 3, item = (blockIdx.x & 7) * run + pos;
+  if (pos >= run || item >= items) return {0, 0, 0, 0};
+  const uint32_t panel = PANEL ? item / (tiles * PANEL) : 0u, rest = item - panel * tiles * PANEL;
+  const uint32_t left = cols - PANEL * panel, width = PANEL && left > (uint32_t)PANEL ? (uint32_t)PANEL : left;
+  const int tile = (int)(rest / width), col = (int)(PANEL * panel + rest % width);
+  int before = 0;
+  for (int e0 = 0;; e0 += 64) {
+    if (e0 > 0) {
+      n = tiles_of(e0 + lane, lo, hi);
+      scan = scan_of(n);
     }
     const uint64_t past = __ballot(before + scan > tile);
     if (past) {
       const int who = __ffsll((unsigned long long)past) - 1;
       const int first = before + __shfl(scan - n, who);
-      const int l = __shfl(lo, who), h = __shfl(hi, who);
-      const int row0 = l + (tile - first) * H;
-      int rows = h - row0;
-      rows = rows < H ? rows : H;
+      const int l = __shfl(lo, who), h = __shfl(hi, who), row0 = l + (tile - first) * H;
+      const int rows = h - row0 < H ? h - row0 : H;
       return {__builtin_amdgcn_readfirstlane(e0 + who), __builtin_amdgcn_readfirstlane(row0),
-              __builtin_amdgcn_readfirstlane(rows)};
+              __builtin_amdgcn_readfirstlane(rows), col};
     }
     before += __shfl(scan, 63);
+    if (e0 + 64 > E) return {0, 0, 0, 0};
   }
-  return {0, 0, 0};
-}
-// how many tiles there are
-__device__ __forceinline__ int count_tiles(const int *__restrict__ offsets, int E, int P, int H) {
-  const int lane = threadIdx.x & 63;
-  int n = 0;
-  for (int e = lane; e <= E; e += 64) n += ((e < E ? offsets[e + 1] : P) - offsets[e] + H - 1) / H;
-#pragma unroll
-  for (int d = 32; d; d >>= 1) n += __shfl_xor(n, d);
-  return __builtin_amdgcn_readfirstlane(n);
 }
 // tiles there can be
 static inline int64_t tile_bound(int64_t P, int E, int H) { return P / H + (P < E + 1 ? P : E + 1); }
+// workgroups of `threads` for all items there can be; 0: too many for a launch
+static inline unsigned item_grid(int64_t P, int E, int H, int64_t cols, int threads) {
+  const int64_t blocks = round_up64(tile_bound(P, E, H) * cols, 8);
+  return blocks * threads >= (int64_t)1 << 32 ? 0u : (unsigned)blocks;
+}
 
 // the row of x that row p reads
 __device__ __forceinline__ int64_t x_row_of(const int *__restrict__ order, int top_k, int64_t T, int64_t p) {

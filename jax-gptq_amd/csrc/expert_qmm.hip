@@ -140,16 +140,16 @@ struct Choice {
 // CUs.  Each kernel costs the same for 1 row as for all that its tile holds, so a wider tile pays once the rows fill
 // half of it or so; where columns are few, strips of 128 channels and halves of K bring more workgroups.  Measured, us a
 // call (strip / 32 x 128 in halves of K / 32 x 256 / 64 x 256 / 64 x 256 in halves of K):
-//   8 experts 4096 x 11008:  4 rows 53 66 67 83 93,  24: 100 81 71 83 95,  48: 161 113 108 92 105,  128: - 237 206 172 197
-//   64 experts 2048 x 1424:  4 rows 49 43 43 52 61,  24: 92 56 47 57 67,   48: 145 79 70 62 73,     128: - 170 143 117 137
-//   8 experts 11008 x 4096:  4 rows 45 76 125 152 112,  24: 88 97 126 153 117,  48: 133 107 130 155 119,
+//   8 experts 4096 x 11008:  4 rows 55 66 67 83 93,  16: 76 73 68 84 94,  48: 161 113 108 92 105,  128: - 237 206 172 197
+//   64 experts 2048 x 1424:  4 rows 37 43 43 52 61,  16: 52 52 44 55 64,   48: 145 79 70 62 73,     128: - 170 143 117 137
+//   8 experts 11008 x 4096:  4 rows 45 76 125 152 112,  24: 87 97 126 153 117,  48: 133 107 130 155 119,
 //                            96: - 184 164 158 132,  128: - 228 259 201 225
 static Choice choose(int64_t P, int E, int64_t C, int64_t group, int x_dtype, int transpose) {
   if ((group && group % 32) || C < 16) return {Choice::SIMPLE, 0};
   if (transpose) return {Choice::BACK, 0};
   const int64_t rows = P / E;
   if ((P < E ? P : E) * ceil_div64(C, 256) >= 256) {
-    if (rows < 8 && C >= 128) return {Choice::STRIP, 0};
+    if (rows <= 8 && C >= 128) return {Choice::STRIP, 0};
     return {Choice::TILE, rows <= 24 ? TILE_32x256 : TILE_64x256};
   }
   if (rows <= 24 && C >= 128) return {Choice::STRIP, 0};

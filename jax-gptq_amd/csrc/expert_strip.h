@@ -4,7 +4,7 @@
 //
 // Bound by the weights' bytes (every expert that any row picked is read once from HBM as long as its rows fit one
 // tile).  Each of the eight wavefronts takes every eighth unit of 32 KS input features and multiplies all rows of the
-// tile with the whole strip: nothing is shared while K runs, so there is no barrier, and a wavefront has the next
+// tile with the whole strip (sixteen wavefronts, for the calls that have few workgroups: a quarter slower): nothing is shared while K runs, so there is no barrier, and a wavefront has the next
 // units' loads (weights, tables, activations) in flight while it multiplies one.  A workgroup covers K by itself, so
 // no partial result leaves it: no workspace, no counter, no second launch.
 // Codes enter the matrix cores exactly; the group's sum of activations comes from one more product against ones; the
@@ -14,6 +14,7 @@
 // the activations of 16 rows, which as operands would be 16-byte pieces of 16 places, go to LDS in whole lines.
 #pragma once
 #include "expert_tile.h"
+#include <math.h>
 
 namespace xqmm {
 
@@ -184,17 +185,17 @@ __global__ __launch_bounds__(STRIP_WAVES * 64) void strip_kernel(ExpertArgs a) {
   using S = Strip<XT, BITS, ZT, KS, CW, DMA>;
   constexpr int ZB = S::ZB;
   // register sets and pieces of LDS that the units of a wavefront go round
-  constexpr int D = KS == 4 ? 2 : (BITS == 4 && XT != GPTQ_HIP_F32 ? 3 : 2);
+  constexpr int D = KS == 1 ? 3 : 2;
   constexpr int ROWS_LDS = DMA ? STRIP_WAVES * D * S::PIECE : 0, RED_LDS = STRIP_WAVES / 2 * CW * 1024;
   typedef __attribute__((address_space(3))) char lds_char;
   __shared__ __attribute__((aligned(16))) char lds[ROWS_LDS > RED_LDS ? ROWS_LDS : RED_LDS];
   const int lane = threadIdx.x & 63, l16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Tile tile = find_tile(a.offsets, a.E, (int)a.P, 16, blockIdx.y);
-  if (tile.rows <= 0) return;
   const int64_t N = a.C, K = BITS == 4 ? 2 * a.R : a.R;
+  const Item tile = find_item<0>(a.offsets, a.E, (int)a.P, 16, (uint32_t)((N + 16 * CW - 1) / (16 * CW)));
+  if (tile.rows <= 0) return;
   // (the last strip ends where N does; what it shares with the one before it is computed twice, to the same bits)
-  const int64_t n0 = (int64_t)blockIdx.x * 16 * CW + 16 * CW <= N ? (int64_t)blockIdx.x * 16 * CW : N - 16 * CW;
+  const int64_t n0 = (int64_t)tile.col * 16 * CW + 16 * CW <= N ? (int64_t)tile.col * 16 * CW : N - 16 * CW;
   const bool f32 = a.out_dtype == GPTQ_HIP_F32;
   if (tile.expert == a.E) {                            // rows of nowhere
     for (int i = threadIdx.x; i < tile.rows * 16 * CW; i += STRIP_WAVES * 64) {
@@ -236,7 +237,7 @@ __global__ __launch_bounds__(STRIP_WAVES * 64) void strip_kernel(ExpertArgs a) {
 #pragma unroll
   for (int q = 0; q < CW; ++q) out[q] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  // units wave, wave + 8, ...; the one that K ends in (no groups then) by itself
+  // units wave, wave + STRIP_WAVES, ...; the one that K ends in (no groups then) by itself
   const int whole = (int)(K / S::SPAN);
   const int mine = whole > wave ? (whole - wave + STRIP_WAVES - 1) / STRIP_WAVES : 0;
   if (mine > 0) {
@@ -275,7 +276,7 @@ __global__ __launch_bounds__(STRIP_WAVES * 64) void strip_kernel(ExpertArgs a) {
     S::multiply(u, x, c, out);
   }
 
-  // the eight partial tiles: the upper four wavefronts hand theirs to the lower four, whose sums are then added up
+  // the partial tiles: the upper half of the wavefronts hand theirs to the lower, whose sums are then added up
   f32x4 *red = reinterpret_cast<f32x4 *>(lds);
   __syncthreads();
   if (wave >= STRIP_WAVES / 2) {
@@ -302,17 +303,19 @@ __global__ __launch_bounds__(STRIP_WAVES * 64) void strip_kernel(ExpertArgs a) {
   }
 }
 
-template <int XT, int CW, bool DMA> static int strip_tables(hipStream_t s, const ExpertArgs &a, dim3 grid, int ks) {
+template <int XT, int CW, bool DMA>
+static int strip_tables(hipStream_t s, const ExpertArgs &a, int ks) {
+  const unsigned grid = item_grid(a.P, a.E, 16, ceil_div64(a.C, 16 * CW), STRIP_WAVES * 64);
+  if (!grid) return GPTQ_HIP_EINVAL;
 #define GPTQ_STRIP(B, S)                                                                                          \
   if (a.bits == B && ks == S) {                                                                                   \
     if (a.zs_dtype == GPTQ_HIP_F32)                                                                               \
-      strip_kernel<XT, B, GPTQ_HIP_F32, S, CW, DMA><<<grid, STRIP_WAVES * 64, 0, s>>>(a);                         \
+      strip_kernel<XT, B, GPTQ_HIP_F32, S, CW, DMA><<<grid, STRIP_WAVES * 64, 0, s>>>(a);                        \
     else if (a.zs_dtype == GPTQ_HIP_F16)                                                                          \
-      strip_kernel<XT, B, GPTQ_HIP_F16, S, CW, DMA><<<grid, STRIP_WAVES * 64, 0, s>>>(a);                         \
+      strip_kernel<XT, B, GPTQ_HIP_F16, S, CW, DMA><<<grid, STRIP_WAVES * 64, 0, s>>>(a);                        \
     else                                                                                                          \
-      strip_kernel<XT, B, GPTQ_HIP_BF16, S, CW, DMA><<<grid, STRIP_WAVES * 64, 0, s>>>(a);                        \
+      strip_kernel<XT, B, GPTQ_HIP_BF16, S, CW, DMA><<<grid, STRIP_WAVES * 64, 0, s>>>(a);                       \
   }
-  if constexpr (XT != GPTQ_HIP_F32) { GPTQ_STRIP(4, 4) }
   GPTQ_STRIP(4, 2) GPTQ_STRIP(4, 1) GPTQ_STRIP(8, 2) GPTQ_STRIP(8, 1)
 #undef GPTQ_STRIP
   GPTQ_CHECK_LAUNCH();
@@ -320,15 +323,17 @@ template <int XT, int CW, bool DMA> static int strip_tables(hipStream_t s, const
 }
 
 template <int XT> static int strip_launch(hipStream_t s, const ExpertArgs &a) {
-  constexpr int CW = 8;          // rows of 128 bytes: half as wide, every 128-byte line of memory is fetched twice (18.5
-                                 // against 10.5 us for the bare loads of 45 MB); 256 bytes, 13 - 14 us
   const int64_t K = a.bits == 4 ? 2 * a.R : a.R;
-  const dim3 grid((unsigned)ceil_div64(a.C, 16 * CW), (unsigned)tile_bound(a.P, a.E, 16));
-  // the longest unit that lies in one group; four k-steps where the registers hold two such units
-  const bool r4 = XT != GPTQ_HIP_F32 && a.bits == 4;
-  const int ks = !a.group || a.group % 128 == 0 ? (r4 ? 4 : 2) : (a.group % 64 == 0 ? 2 : 1);
-  const bool dma = (uintptr_t)a.x % 16 == 0 && K * (XT == GPTQ_HIP_F32 ? 4 : 2) % 16 == 0;
-  return dma ? strip_tables<XT, CW, true>(s, a, grid, ks) : strip_tables<XT, CW, false>(s, a, grid, ks);
+  // 64 features lie in one group, or 32; units of 128 keep one workgroup on a CU where two fit and are no faster
+  const int ks = a.group % 64 == 0 ? 2 : 1;
+  if ((uintptr_t)a.x % 16 || K * (XT == GPTQ_HIP_F32 ? 4 : 2) % 16) return strip_tables<XT, 8, false>(s, a, ks);
+  // Strips of 64 channels: two neighbours share the lines of memory they begin and end in, on the same XCD; more
+  // workgroups, less for each (8 experts 11008 x 4096, one token: 20 us, in strips of 128 channels 29; 64 experts
+  // 2048 x 1424, 32 tokens of 2: 19 against 22).  Strips of 128 read the activations half as often, which decides where
+  // they take one round of workgroups on the 256 CUs (11008 x 4096, 16 tokens of 2: 45 against 61 us).
+  const double busy = a.E * (1.0 - exp(-(double)a.P / a.E)), strips = busy * ceil_div64(a.C, 128);
+  const bool wide = strips > 128 && strips <= 256 && a.P < 8 * a.E;
+  return wide ? strip_tables<XT, 8, true>(s, a, ks) : strip_tables<XT, 4, true>(s, a, ks);
 }
 
 }  // namespace xqmm

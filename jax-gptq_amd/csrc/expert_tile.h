@@ -178,19 +178,9 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
   const int64_t N = a.C;
   const bool f32 = a.out_dtype == GPTQ_HIP_F32;
 
-  // Which tile.  Workgroups go round the eight XCDs; each XCD takes a run of the list (panels of four column tiles, row
-  // tile by row tile), so what runs on it at a time shares rows and weights in its L2.
-  const int row_tiles = count_tiles(a.offsets, a.E, (int)a.P, T::BM);
-  const int cols = (int)((N + T::BN - 1) / T::BN);
-  const int64_t total = (int64_t)row_tiles * cols, run = (total + 7) / 8;
-  const int64_t pos = blockIdx.x >> 3, item = (blockIdx.x & 7) * run + pos;
-  if (pos >= run || item >= total) return;
-  const int panel = (int)(item / ((int64_t)row_tiles * 4));
-  const int rest = (int)(item - (int64_t)panel * row_tiles * 4);
-  const int width = cols - 4 * panel < 4 ? cols - 4 * panel : 4;
-  const int64_t n0 = (int64_t)(4 * panel + rest % width) * T::BN;
-  const Tile tile = find_tile(a.offsets, a.E, (int)a.P, T::BM, rest / width);
+  const Item tile = find_item<4>(a.offsets, a.E, (int)a.P, T::BM, (uint32_t)((N + T::BN - 1) / T::BN));
   if (tile.rows <= 0) return;
+  const int64_t n0 = (int64_t)tile.col * T::BN;
   if (tile.expert == a.E) {                            // rows of nowhere
     for (int i = threadIdx.x; i < tile.rows * T::BN; i += T::THREADS) {
       const int64_t n = n0 + i % T::BN;
@@ -487,10 +477,10 @@ template <int XT, int BITS, int ZL, bool HALF, int RBW, int WM, int WN, int WK>
 static int tile_one(hipStream_t s, const TileArgs &t) {
   using T = TileShape<XT, BITS, ZL, HALF, RBW, WM, WN, WK>;
   const void *kernel = (const void *)tile_kernel<XT, BITS, ZL, HALF, RBW, WM, WN, WK>;
-  const int64_t blocks = round_up64(tile_bound(t.a.P, t.a.E, T::BM) * ceil_div64(t.a.C, T::BN), 8);
-  if (blocks * T::THREADS >= (int64_t)1 << 32) return GPTQ_HIP_EINVAL;
+  const unsigned blocks = item_grid(t.a.P, t.a.E, T::BM, ceil_div64(t.a.C, T::BN), T::THREADS);
+  if (!blocks) return GPTQ_HIP_EINVAL;
   if (!gptq_raise_lds_limit(kernel, T::LDS)) return GPTQ_HIP_ELAUNCH;
-  tile_kernel<XT, BITS, ZL, HALF, RBW, WM, WN, WK><<<(unsigned)blocks, T::THREADS, T::LDS, s>>>(t);
+  tile_kernel<XT, BITS, ZL, HALF, RBW, WM, WN, WK><<<blocks, T::THREADS, T::LDS, s>>>(t);
   GPTQ_CHECK_LAUNCH();
   return GPTQ_HIP_OK;
 }
