@@ -31,6 +31,10 @@ __device__ __forceinline__ void to_lds_16(const void *src, uint32_t dst) {
 __device__ __forceinline__ void to_lds_4(const void *src, uint32_t dst) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(dst), "v"(src) : "memory", "m0");
 }
+// the same from a base that all lanes share plus a lane's 32-bit offset
+__device__ __forceinline__ void to_lds_16(const void *base, uint32_t off, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(dst), "v"(off), "s"(base) : "memory", "m0");
+}
 template <int VM> __device__ __forceinline__ void wait_and_meet() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(VM) : "memory");
 }
@@ -234,6 +238,23 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
   constexpr int TABLE_REGS = WK * T::HN * 2 * T::BN / T::THREADS;
   u32x4 breg[ZL ? 1 : T::BI];
   float zreg[ZL ? 1 : TABLE_REGS];
+  // this lane's packed rows and channels in a stage, as offsets from its first row; in the last stage rows past K are
+  // replaced by the last (any code: the activations are zero there)
+  int brow[T::BI], bcol[T::BI];
+  uint32_t boff[T::BI], bend[T::BI];
+#pragma unroll
+  for (int j = 0; j < T::BI; ++j) {
+    const int at = (wave * T::BI + j) % (T::BP / 1024) * (64 / CH) + lane / CH, g = reader(at);
+    brow[j] = T::BN == 128 ? at ^ (g >> 1) : at;
+    bcol[j] = 16 * ((lane % CH) ^ (T::BN == 128 ? 4 * (g & 1) : 4 * g));
+    const int64_t n = n0 + bcol[j] < N ? n0 + bcol[j] : 0, left = a.R - (int64_t)(t.stages - 1) * T::BROWS;
+    boff[j] = (uint32_t)(brow[j] * N + n);
+    bend[j] = (uint32_t)((brow[j] < left ? brow[j] : left - 1) * N + n);
+  }
+  // and its channels in a row of the tables: zeros, then scales, 1 KB each at 256 channels, half a load each at 128
+  const int tl = T::BN == 128 ? lane & 31 : lane;
+  const int64_t tn = n0 + (ZB == 4 ? 4 * tl : 8 * (tl % (T::BN / 8)));
+  const uint32_t toff = (uint32_t)((tn < N ? tn : 0) * ZB);
 
   auto issue = [&](int s, int slot, int table) __attribute__((always_inline)) {
     const uint32_t base = lds0 + slot * T::DATA, tbase = lds0 + T::STAGES * T::DATA + table * T::TABLE;
@@ -244,16 +265,13 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
     }
 #pragma unroll
     for (int j = 0; j < T::BI; ++j) {
-      const int i = wave * T::BI + j, p = i / (T::BP / 1024);
-      const int at = i % (T::BP / 1024) * (64 / CH) + lane / CH, g = reader(at);
-      int64_t r = (int64_t)stage_of(p, s) * T::BROWS + (T::BN == 128 ? at ^ (g >> 1) : at);
-      r = r < a.R ? r : a.R - 1;                       // (past K: any code, the activations are zero)
-      int64_t n = n0 + 16 * ((lane % CH) ^ (T::BN == 128 ? 4 * (g & 1) : 4 * g));
+      const int i = wave * T::BI + j, st = stage_of(i / (T::BP / 1024), s);
       if constexpr (ZL) {
-        n = n < N ? n : 0;
-        to_lds_16(packed + r * N + n, base + T::A + i * 1024);
+        to_lds_16(packed + (int64_t)st * T::BROWS * N, st + 1 < t.stages ? boff[j] : bend[j], base + T::A + i * 1024);
       } else {
-        breg[j] = load_end16(packed + r * N, n, N);
+        int64_t r = (int64_t)st * T::BROWS + brow[j];
+        r = r < a.R ? r : a.R - 1;
+        breg[j] = load_end16(packed + r * N, n0 + bcol[j], N);
       }
     }
 #pragma unroll
@@ -263,13 +281,10 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
         const int q = it / T::MB, h = q % T::HN, st = stage_of(q / T::HN, s);
         to_lds_4(srow[j] + (HALF ? 2 * st + h : st), tbase + T::Z + it * 256);
       } else if constexpr (ZL != 0) {
-        // zeros, then scales: 1 KB each at 256 channels, half a load each at 128
         const int i = it - T::SI, q = i / (T::BN / 128);
-        const int which = T::BN == 128 ? lane >> 5 : i & 1, l = T::BN == 128 ? lane & 31 : lane;
-        int64_t n = ZB == 4 ? n0 + 4 * l : n0 + 8 * (l % (T::BN / 8));
-        n = n < N ? n : 0;
-        to_lds_16((which ? scale : zero) + (table_row(stage_of(q / T::HN, s), q % T::HN) * N + n) * ZB,
-                  tbase + i * 1024);
+        const int64_t row = table_row(stage_of(q / T::HN, s), q % T::HN) * N * ZB;
+        if (T::BN == 128) to_lds_16((lane >> 5 ? scale : zero) + row + toff, tbase + i * 1024);
+        else to_lds_16((i & 1 ? scale : zero) + row, toff, tbase + i * 1024);
       }
     }
     if constexpr (!ZL) {
@@ -346,25 +361,36 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
     u32x4 x[2][RB][T::PARTS];
     uint32_t r[2][C::ROWS];
   };
-  auto fetch = [&](Step &f, int slot, int ks) __attribute__((always_inline)) {
-    const char *base = lds + slot * T::DATA;
+  // where this lane reads: rows (by k-step and product), codes (by product); the two k-steps of a stage are read at
+  // different times, so each has its own addresses, moved on with the ring
+  int xat[2][2], rat[2][2];
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
-      const int g = 2 * v + hi;                         // 8 features g of the 32; (16 features per product)
-      const int chunk = (wn * 4 + ((l32 & 15) >> 2)) ^ (T::BN == 128 ? 4 * (g & 1) : 4 * g);
+      const int g = 2 * v + hi, chunk = (wn * 4 + ((l32 & 15) >> 2)) ^ (T::BN == 128 ? 4 * (g & 1) : 4 * g);
+      xat[ks][v] = part * T::AP + (wm * 16 * RBW + l32) * 128 + (((4 * ks + g) ^ (l32 & 7)) * 16);
+      rat[ks][v] = T::A + part * T::BP + C::ROWS * g * T::BN + chunk * 16 + (l32 & 3) * 4;
+    }
+  auto fetch = [&](Step &f, int ks) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < C::ROWS; ++i) {
-        const int row = (BITS == 4 ? 16 : 32) * ks + C::ROWS * g + (T::BN == 128 ? i ^ (g >> 1) : i);
-        f.r[v][i] =
-            *reinterpret_cast<const uint32_t *>(base + T::A + part * T::BP + row * T::BN + chunk * 16 + (l32 & 3) * 4);
-      }
+    for (int v = 0; v < 2; ++v) {
+#pragma unroll
+      for (int i = 0; i < C::ROWS; ++i)                 // (g >> 1 is v: at 128 channels odd and even rows change places)
+        f.r[v][i] = *reinterpret_cast<const uint32_t *>(
+            lds + rat[ks][v] + ((BITS == 4 ? 16 : 32) * ks + (T::BN == 128 ? i ^ v : i)) * T::BN);
 #pragma unroll
       for (int i = 0; i < RB; ++i)
 #pragma unroll
         for (int p = 0; p < T::PARTS; ++p)
-          f.x[v][i][p] = *reinterpret_cast<const u32x4 *>(base + part * T::AP + p * T::BM * 128 +
-                                                          (wm * 16 * RBW + 32 * i + l32) * 128 +
-                                                          (((4 * ks + g) ^ (l32 & 7)) * 16));
+          f.x[v][i][p] = *reinterpret_cast<const u32x4 *>(lds + xat[ks][v] + p * T::BM * 128 + 32 * i * 128);
+    }
+  };
+  auto move_on = [&](int ks, int by) __attribute__((always_inline)) {
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      xat[ks][v] += by;
+      rat[ks][v] += by;
     }
   };
   auto multiply = [&](Step &f, bool fresh) __attribute__((always_inline)) {
@@ -396,25 +422,28 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
   }
   wait_and_meet<ZL ? (NS - 1) * T::LOADS : 0>();
   Step f0, f1;
-  fetch(f0, 0, 0);
+  fetch(f0, 0);
   int slot = 0, table = 0, fresh_table = NS;
   auto stage = [&](int s, bool fresh, bool last) __attribute__((always_inline)) {
     const bool live = WK == 1 || part * span + s < t.stages;
-    if (EARLY) fetch(f1, slot, 1);
+    const int by = slot + 1 == NS ? -(NS - 1) * T::DATA : T::DATA;
+    move_on(0, by);
+    if (EARLY) fetch(f1, 1);
     if (live) {
       multiply(f0, HALF || fresh);
       if constexpr (HALF) close(table, 0);
     }
-    if (!EARLY) fetch(f1, slot, 1);
+    if (!EARLY) fetch(f1, 1);
+    move_on(1, by);
     wait_and_meet<ZL ? (NS - 2) * T::LOADS : 0>();
     issue(s + NS, slot, fresh_table);
     const int next = slot + 1 == NS ? 0 : slot + 1;
-    if (EARLY) fetch(f0, next, 0);
+    if (EARLY) fetch(f0, 0);
     if (live) {
       multiply(f1, HALF);
       if (HALF || last || part * span + s + 1 == t.stages) close(table, HALF ? 1 : 0);
     }
-    if (!EARLY) fetch(f0, next, 0);
+    if (!EARLY) fetch(f0, 0);
     land(slot, fresh_table);
     slot = next;
     table = table == NS ? 0 : table + 1;
