@@ -8,10 +8,13 @@
 // deep: the activations of the tile's rows, the packed codes (they stay packed in LDS), the group's scales and zeros
 // and the rows' sums.  One barrier per stage: wavefronts wait for their own loads of stage s, meet, and issue the loads
 // of a later stage into the buffer that everybody has finished with.  Each wavefront owns 64 (or 32) x 64 outputs: its
-// four operands of codes are built in registers and used for four (two) row blocks.  fp32 sums of a group are scaled
+// operands of codes are built in registers and used for two (one) blocks of 32 rows.  fp32 sums of a group are scaled
 // into a second set of accumulators, so codes stay exact 16-bit operands whatever the scales are.
+// The zero point's term is one product more per group: sum and -(o + z) are fp32 numbers in three bf16 parts each, whose
+// six largest products (the rest is below 2^-24 of the term) are six of the sixteen features of a 32 x 32 product.  It
+// takes the place of an instruction for every sum, which the vector units have less time for than the matrix cores.
 // A first kernel writes the activations once more, in the order of the operands (fp32: as three bf16 parts), padded to
-// whole stages, and the sums of every row over the part of its group up to the end of each stage.
+// whole stages, and the sums of every row over the part of its group up to the end of each stage, as such an operand.
 #pragma once
 #include "expert_common.h"
 
@@ -43,7 +46,7 @@ template <int VM> __device__ __forceinline__ void wait_and_meet() {
 struct Staged {
   int64_t Kp;              // K padded to whole stages
   int64_t row_bytes;       // of the staged activations: parts * Kp * 2
-  int64_t per_row;         // sums of a row: one per stage, or per k-step where groups are odd multiples of 32
+  int64_t per_row;         // sums of a row, 16 bytes each: one per stage, or per k-step where groups are odd multiples of 32
   size_t sums_at, bytes;
 };
 static inline Staged staged_layout(int64_t x_rows, int64_t K, int x_dtype, bool half) {
@@ -52,15 +55,38 @@ static inline Staged staged_layout(int64_t x_rows, int64_t K, int x_dtype, bool 
   l.row_bytes = (x_dtype == GPTQ_HIP_F32 ? 3 : 1) * l.Kp * 2;
   l.per_row = l.Kp / (half ? 32 : 64);
   l.sums_at = (size_t)round_up64(x_rows * l.row_bytes, 256);
-  l.bytes = l.sums_at + (size_t)round_up64(x_rows * l.per_row * 4, 256);
+  l.bytes = l.sums_at + (size_t)(x_rows * l.per_row) * 16;
   return l;
+}
+
+// v in three bf16 parts
+__device__ __forceinline__ void three_parts(float v, uint32_t *part) {
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    part[i] = __builtin_bit_cast(uint32_t, v);
+    v -= __builtin_bit_cast(float, part[i] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ uint32_t upper_halves(uint32_t a, uint32_t b) {
+  return __builtin_amdgcn_perm(b, a, 0x07060302u);
+}
+// features 0 .. 7 of the zero point's product: parts 1 2 3 1 2 1 of the sum against 1 1 1 2 2 3 of the factor
+__device__ __forceinline__ u32x4 sum_operand(float v) {
+  uint32_t p[3];
+  three_parts(v, p);
+  return u32x4{upper_halves(p[0], p[1]), upper_halves(p[2], p[0]), upper_halves(p[1], p[0]), 0u};
+}
+__device__ __forceinline__ u32x4 factor_operand(float v) {
+  uint32_t p[3];
+  three_parts(v, p);
+  return u32x4{upper_halves(p[0], p[0]), upper_halves(p[0], p[1]), upper_halves(p[1], p[2]), 0u};
 }
 
 // One workgroup per row of x.
 template <int XT, bool DEALT>
 __global__ __launch_bounds__(256) void stage_rows_kernel(const void *__restrict__ x, int64_t K, int64_t Kp,
                                                          int64_t per_row, int64_t row_bytes, int half, int group,
-                                                         char *__restrict__ rows, float *__restrict__ sums) {
+                                                         char *__restrict__ rows, u32x4 *__restrict__ sums) {
   extern __shared__ float seg[];                      // sums of the row's stages (or k-steps)
   constexpr int SZ = XT == GPTQ_HIP_F32 ? 4 : 2, WORDS = SZ / 2;
   const int64_t row = blockIdx.x;
@@ -116,7 +142,7 @@ __global__ __launch_bounds__(256) void stage_rows_kernel(const void *__restrict_
   }
   __syncthreads();
   if (half) {
-    for (int64_t i = threadIdx.x; i < per_row; i += 256) sums[row * per_row + i] = seg[i];
+    for (int64_t i = threadIdx.x; i < per_row; i += 256) sums[row * per_row + i] = sum_operand(seg[i]);
   } else {
     // running sums inside each group: what its last stage holds is the group's
     const int per = group / 64;
@@ -124,7 +150,7 @@ __global__ __launch_bounds__(256) void stage_rows_kernel(const void *__restrict_
       float s = 0.f;
       for (int64_t i = i0; i < i0 + per && i < per_row; ++i) {
         s += seg[i];
-        sums[row * per_row + i] = s;
+        sums[row * per_row + i] = sum_operand(s);
       }
     }
   }
@@ -133,7 +159,7 @@ __global__ __launch_bounds__(256) void stage_rows_kernel(const void *__restrict_
 struct TileArgs {
   ExpertArgs a;
   const char *rows;           // staged activations
-  const float *sums;
+  const u32x4 *sums;
   int64_t row_bytes, Kp, per_row;
   int stages;                 // Kp / 64
   int close;                  // stages of a group (or of a piece of the sum)
@@ -149,7 +175,7 @@ template <int XT, int BITS, int ZL, bool HALF, int RBW, int WM, int WN, int WK> 
   static constexpr int BROWS = BITS == 4 ? 32 : 64;       // packed rows of a part's stage
   static constexpr int HN = HALF ? 2 : 1, MB = (BM + 63) / 64;
   // one part's rows, codes, zeros and scales (of a group), sums; then all parts'
-  static constexpr int AP = PARTS * BM * 128, BP = BROWS * BN, ZP = 2 * BN * 4, SP = MB * 256;
+  static constexpr int AP = PARTS * BM * 128, BP = BROWS * BN, ZP = 2 * BN * 4, SP = MB * 1024;
   static constexpr int A = WK * AP, B = WK * BP, Z = WK * HN * ZP, S = WK * HN * SP;
   // a stage's rows and codes, and its tables, in rings of their own: rows and codes are in registers half a stage before
   // the tables are needed, so their place is free one stage earlier
@@ -218,7 +244,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
   for (int j = 0; j < T::AI; ++j)
     arow[j] = t.rows + row_base(8 * ((wave * T::AI + j) % (T::BM / 8)) + (lane >> 3)) * t.row_bytes +
               ((lane & 7) ^ (lane >> 3)) * 16;
-  const float *srow[T::MI];
+  const u32x4 *srow[T::MI];
 #pragma unroll
   for (int j = 0; j < T::MI; ++j) {
     const int it = (wave + T::WAVES * j) % T::ITEMS;
@@ -279,7 +305,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
       const int it = (wave + T::WAVES * j) % T::ITEMS;   // (more wavefronts than items: the same bytes twice)
       if (it < T::SI) {
         const int q = it / T::MB, h = q % T::HN, st = stage_of(q / T::HN, s);
-        to_lds_4(srow[j] + (HALF ? 2 * st + h : st), tbase + T::Z + it * 256);
+        to_lds_16(srow[j] + (HALF ? 2 * st + h : st), tbase + T::Z + it * 1024);
       } else if constexpr (ZL != 0) {
         const int i = it - T::SI, q = i / (T::BN / 128);
         const int64_t row = table_row(stage_of(q / T::HN, s), q % T::HN) * N * ZB;
@@ -325,37 +351,47 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
 #pragma unroll
       for (int r = 0; r < 16; ++r) out[i][c][r] = acc[i][c][r] = 0.f;
 
-  auto close = [&](int table, int h) __attribute__((always_inline)) {
-    const char *zp = lds + T::STAGES * T::DATA + table * T::TABLE + (part * T::HN + h) * T::ZP;
-    const char *sums = lds + T::STAGES * T::DATA + table * T::TABLE + T::Z + (part * T::HN + h) * T::SP;
-    float z[2], s[2];
+  auto table_pair = [&](const char *p, float *v) __attribute__((always_inline)) {       // of this lane's two channels
     const int col = wn * 64 + mycol;
     if constexpr (ZB == 4) {
-      const float2 zv = *reinterpret_cast<const float2 *>(zp + col * 4);
-      const float2 sv = *reinterpret_cast<const float2 *>(zp + T::BN * 4 + col * 4);
-      z[0] = zv.x; z[1] = zv.y; s[0] = sv.x; s[1] = sv.y;
+      const float2 w = *reinterpret_cast<const float2 *>(p + col * 4);
+      v[0] = w.x;
+      v[1] = w.y;
     } else {
+      const uint32_t w = *reinterpret_cast<const uint32_t *>(p + col * 2);
       const bool bf = a.zs_dtype == GPTQ_HIP_BF16;
-      const uint32_t zw = *reinterpret_cast<const uint32_t *>(zp + col * 2);
-      const uint32_t sw = *reinterpret_cast<const uint32_t *>(zp + T::BN * 4 + col * 2);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const uint32_t zh = (zw >> (16 * c)) & 0xFFFFu, sh = (sw >> (16 * c)) & 0xFFFFu;
-        z[c] = bf ? __builtin_bit_cast(float, zh << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)zh);
-        s[c] = bf ? __builtin_bit_cast(float, sh << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)sh);
+        const uint32_t h = (w >> (16 * c)) & 0xFFFFu;
+        v[c] = bf ? __builtin_bit_cast(float, h << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)h);
       }
     }
+  };
+  // the zero point's term of a group (features 8 .. 15 of that product are zero on the codes' side)
+  auto correct = [&](int table, int h) __attribute__((always_inline)) {
+    const char *base = lds + T::STAGES * T::DATA + table * T::TABLE;
+    float z[2];
+    table_pair(base + (part * T::HN + h) * T::ZP, z);
+    u32x4 f[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) f[c] = factor_operand(hi ? 0.f : -(z[c] + C::OFFSET));
+#pragma unroll
+    for (int i = 0; i < RB; ++i) {
+      const u32x4 sum = *reinterpret_cast<const u32x4 *>(base + T::Z + (part * T::HN + h) * T::SP +
+                                                         (wm * 16 * RBW + 32 * i + l32) * 16);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) acc[i][c] = Op<GPTQ_HIP_BF16>::mma32(sum, f[c], acc[i][c]);
+    }
+  };
+  auto close = [&](int table, int h) __attribute__((always_inline)) {
+    float s[2];
+    table_pair(lds + T::STAGES * T::DATA + table * T::TABLE + (part * T::HN + h) * T::ZP + T::BN * 4, s);
 #pragma unroll
     for (int i = 0; i < RB; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f32x4 sum = *reinterpret_cast<const f32x4 *>(sums + (wm * 16 * RBW + 32 * i + 8 * j + 4 * hi) * 4);
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            out[i][c][4 * j + r] = fmaf(s[c], fmaf(-(z[c] + C::OFFSET), sum[r], acc[i][c][4 * j + r]), out[i][c][4 * j + r]);
-      }
+        for (int r = 0; r < 16; ++r) out[i][c][r] = fmaf(s[c], acc[i][c][r], out[i][c][r]);
   };
   struct Step {                                         // operands of 32 features: rows, and codes as they are
     u32x4 x[2][RB][T::PARTS];
@@ -429,10 +465,15 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
     const int by = slot + 1 == NS ? -(NS - 1) * T::DATA : T::DATA;
     move_on(0, by);
     if (EARLY) fetch(f1, 1);
+    const bool ends = !HALF && live && (last || part * span + s + 1 == t.stages);
     if (live) {
       multiply(f0, HALF || fresh);
-      if constexpr (HALF) close(table, 0);
+      if constexpr (HALF) {
+        correct(table, 0);
+        close(table, 0);
+      }
     }
+    if (ends) correct(table, 0);
     if (!EARLY) fetch(f1, 1);
     move_on(1, by);
     wait_and_meet<ZL ? (NS - 2) * T::LOADS : 0>();
@@ -441,8 +482,12 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
     if (EARLY) fetch(f0, 0);
     if (live) {
       multiply(f1, HALF);
-      if (HALF || last || part * span + s + 1 == t.stages) close(table, HALF ? 1 : 0);
+      if constexpr (HALF) {
+        correct(table, 1);
+        close(table, 1);
+      }
     }
+    if (ends) close(table, 0);
     if (!EARLY) fetch(f0, 0);
     land(slot, fresh_table);
     slot = next;
@@ -542,7 +587,7 @@ template <int XT> static int tile_launch(hipStream_t s, const ExpertArgs &a, int
   const Staged l = staged_layout(a.T, K, a.x_dtype, half);
   const int group = a.group ? (int)a.group : TILE_LONG;
   char *rows = (char *)ws;
-  float *sums = (float *)((char *)ws + l.sums_at);
+  u32x4 *sums = (u32x4 *)((char *)ws + l.sums_at);
   if (a.bits == 4 && Codes<XT, 4>::DEALT)
     stage_rows_kernel<XT, true><<<(unsigned)a.T, 256, l.per_row * 4, s>>>(a.x, K, l.Kp, l.per_row, l.row_bytes, half,
                                                                           group, rows, sums);
