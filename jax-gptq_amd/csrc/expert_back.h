@@ -27,10 +27,10 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(const U *__restrict__ x, 
 static __global__ __launch_bounds__(256) void widen_tables_kernel(const char *__restrict__ zero,
                                                            const char *__restrict__ scale, int dtype, int64_t n,
                                                            float *__restrict__ out) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  out[i] = table_value(zero, dtype, i);
-  out[n + i] = table_value(scale, dtype, i);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    out[i] = table_value(zero, dtype, i);
+    out[n + i] = table_value(scale, dtype, i);
+  }
 }
 
 struct BackLayout {
@@ -356,8 +356,9 @@ template <int XT> static int back_launch(hipStream_t s, const ExpertArgs &a, voi
   }
   if (l.widen) {
     float *f = (float *)((char *)ws + l.tables_at);
-    widen_tables_kernel<<<(unsigned)ceil_div64(l.tables, 256), 256, 0, s>>>((const char *)a.zero, (const char *)a.scale,
-                                                                            a.zs_dtype, l.tables, f);
+    const int64_t blocks = ceil_div64(l.tables, 256);
+    widen_tables_kernel<<<(unsigned)(blocks < 65536 ? blocks : 65536), 256, 0, s>>>(
+        (const char *)a.zero, (const char *)a.scale, a.zs_dtype, l.tables, f);
     GPTQ_CHECK_LAUNCH();
     t.zero = f;
     t.scale = f + l.tables;

@@ -179,9 +179,9 @@ __device__ __forceinline__ Item find_item(const int *__restrict__ offsets, int E
   const int lane = threadIdx.x & 63;
   auto tiles_of = [&](int e, int &lo, int &hi) -> int {
     lo = hi = 0;
-    if (e <= E) {
-      lo = offsets[e];
-      hi = e < E ? offsets[e + 1] : P;
+    if (e <= E) {                       // (whatever the offsets say, no row outside 0 .. P - 1)
+      lo = min(max(offsets[e], 0), P);
+      hi = e < E ? min(max(offsets[e + 1], lo), P) : P;
     }
     return (hi - lo + H - 1) / H;
   };

@@ -50,7 +50,9 @@ template <int XT, int BITS, int ZT, int KS, int CW, bool DMA> struct Strip {
   };
 
   // the rows' features of a unit on their way to LDS; the loads of the unit's weights come behind them
+  // (What this wavefront read from there has arrived: with the wait the loads cannot overtake it.)
   static __device__ __forceinline__ void send_rows(const Ctx &c, int unit, uint32_t lds) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
     for (int i = 0; i < PIECE / 1024; ++i) to_lds_16(c.row[i] + (int64_t)unit * SPAN * SZ, lds + i * 1024);
   }

@@ -127,13 +127,13 @@ def stack_experts(matrices):
     for m in matrices:
         if m.contraction_axis != 0 or m.int_weight.dim() != 2:
             raise ValueError("experts are 2-D matrices packed along axis 0")
-        if (tuple(m.int_weight.shape), m.bits, m.group_size, m.zero.dtype, tuple(m.zero.shape)) != \
-                (tuple(first.int_weight.shape), first.bits, first.group_size, first.zero.dtype,
+        if (tuple(m.int_weight.shape), m.bits, m.group_size, m.zero.dtype, m.scale.dtype, tuple(m.zero.shape)) != \
+                (tuple(first.int_weight.shape), first.bits, first.group_size, first.zero.dtype, first.scale.dtype,
                  tuple(first.zero.shape)):
             raise ValueError("all experts must have the same shape, code width, groups and parameter type")
     return QuantizedExperts(torch.stack([_dev(m.int_weight, torch.uint8) for m in matrices]),
                             torch.stack([_dev(m.zero) for m in matrices]),
-                            torch.stack([_dev(m.scale).to(first.zero.dtype) for m in matrices]),
+                            torch.stack([_dev(m.scale) for m in matrices]),
                             bits=first.bits, group_size=first.group_size)
 
 
@@ -348,8 +348,8 @@ def quantized_expert_matmul(x, experts, plan, sorted_rows=False, transpose_b=Fal
     packed = _on_device(experts.int_weight, x, "int_weight")
     zero = _float_tensor(_on_device(experts.zero, x, "zero"))
     scale = _on_device(experts.scale, x, "scale")
-    if scale.dtype != zero.dtype:
-        scale = scale.to(zero.dtype)
+    if scale.dtype != zero.dtype:           # the kernels read both in one type: fp32 holds either
+        zero, scale = zero.float(), scale.float()
     if x.requires_grad:
         return _ExpertMatmulFn.apply(x, experts, packed, zero, scale, plan, bool(sorted_rows), bool(transpose_b))
     return _expert_matmul_raw(x, packed, zero, scale, experts.bits, experts.group_size, plan, bool(sorted_rows),

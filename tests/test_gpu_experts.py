@@ -332,6 +332,99 @@ def test_product_and_gradient(X, shape, dt):
     within(dx, ref, tol + half_step(ref, x.dtype))
 
 
+# More of what decides how a product is computed: many experts (more than a wavefront counts at once), rows per expert
+# on either side of each change, both code widths, groups of 32, channels that are no multiple of 16.
+MORE_SHAPES = [
+    (700, 8, 128, 128, 272, 4, 64, 0.02),     # 128 experts, 43 rows each
+    (300, 8, 128, 96, 272, 8, 32, 0.02),      # 18 rows each
+    (1100, 1, 1024, 64, 33, 8, 0, 0),         # hardly any columns
+    (40, 4, 256, 64, 144, 4, 32, 0.1),        # 160 rows over 256 experts
+    (500, 1, 1023, 128, 200, 4, 64, 0.3),
+    (60, 1, 2, 384, 136, 4, 128, 0),          # 30 rows each
+    (90, 1, 3, 320, 256, 8, 32, 0.1),
+    (33, 2, 2, 640, 400, 4, 32, 0),
+    (70, 2, 2, 448, 512, 4, 64, 0),           # 70 rows each, K in seven stages
+    (90, 2, 2, 512, 255, 8, 0, 0),
+    (30, 4, 64, 256, 1040, 4, 256, 0),        # about two rows each, strips that share their last channels
+    (17, 1, 1, 8192, 128, 4, 0, 0),           # a long sum without groups
+    (200, 1, 1, 4160, 64, 8, 0, 0),
+    (260, 2, 64, 64, 1100, 4, 32, 0.05),      # 8 rows each, tiles of 256 channels
+    (64, 1, 1, 64, 16, 4, 32, 0),
+]
+
+
+@pytest.mark.parametrize("dt", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("shape", MORE_SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_product_more_shapes(X, shape, dt):
+    test_product_and_gradient(X, shape, dt)
+
+
+@pytest.mark.parametrize("T", [1, 40, 130, 700])
+def test_product_of_subnormal_rows(X, T):
+    """Rows of which most values are below fp16's smallest normal number, and a scale that brings the results back."""
+    layer = Layer(X, T, 2, 256, 144, 4, 64)
+    layer.scale *= 2.0 ** 14
+    layer.stack = X.QuantizedExperts(layer.packed.cuda(), layer.zero.cuda(), layer.scale.cuda(), 4, 64)
+    ids = ids_of(T, T, 1, 2)
+    order, _, offsets = ref_sort(ids, 2)
+    plan = X.sort_tokens(ids.cuda(), 2)
+    x = (torch.randn(T, 256) * 2e-5).half()
+    check_product(X.quantized_expert_matmul(x.cuda(), layer.stack, plan), x[torch.tensor(order)], layer, offsets)
+    g = (torch.randn(T, 144) * 2e-5).half()
+    y = X.quantized_expert_matmul(g.cuda(), layer.stack, plan, sorted_rows=True, transpose_b=True)
+    check_product(y, g, layer, offsets, transpose=True)
+
+
+def test_tables_of_two_types(X):
+    layer = Layer(X, 3, 2, 128, 64, 4, 64)
+    plan = X.sort_tokens(ids_of(1, 9, 1, 2).cuda(), 2)
+    x = torch.randn(9, 128).half().cuda()
+    mixed = X.QuantizedExperts(layer.packed.cuda(), layer.zero.half().cuda(), layer.scale.cuda(), 4, 64)
+    want = X.quantized_expert_matmul(x, layer.stack, plan)        # the zeros are whole numbers: the same in fp16
+    assert torch.equal(X.quantized_expert_matmul(x, mixed, plan), want)
+    again = X.stack_experts(list(mixed))
+    assert again.scale.dtype == torch.float32 and torch.equal(X.quantized_expert_matmul(x, again, plan), want)
+
+
+@pytest.mark.parametrize("T", [2, 200])
+def test_product_offsets_past_32_bits(X, T):
+    """A stack of more than 2^32 bytes whose last expert lies behind that, and an expert wider than most."""
+    E, R, N = 10, 512, 1 << 20
+    K = 2 * R
+    packed = torch.zeros(E, R, N, dtype=torch.uint8, device="cuda")
+    packed[-1] = torch.randint(0, 256, (R, N), dtype=torch.uint8, device="cuda")
+    assert packed.numel() > 1 << 32
+    zero, scale = torch.full((E, N), 8.0, device="cuda"), torch.full((E, N), 0.01, device="cuda")
+    stack = X.QuantizedExperts(packed, zero, scale, 4)
+    ids = torch.full((T, 1), E - 1)
+    ids[0] = 0
+    plan = X.sort_tokens(ids.cuda(), E)
+    x = torch.randn(T, K).half()
+    y = X.quantized_expert_matmul(x.cuda(), stack, plan)
+    at = torch.cat([torch.arange(40), torch.arange(N - 40, N), torch.randint(0, N, (40,))])
+    codes = codes_of(packed[-1:, :, at.cuda()].cpu(), 4)[0].double()
+    w, big = (codes - 8) * 0.01, (codes + 136) * 0.01
+    xd = x.double()
+    ref, norm = xd @ w, (xd.square() @ big.square()).sqrt()
+    ref[0], norm[0] = xd[0].sum() * -0.08, xd[0].norm() * 1.36
+    order = torch.tensor(ref_sort(ids, E)[0])
+    # (0.01 in fp32 is off by up to 2^-24 of itself, on top of the sum)
+    tol = half_step(ref, torch.float16) + (K + 1) * 2.0 ** -24 * norm
+    within(y[:, at.cuda()], ref[order], tol[order])
+    # and back, where only the columns above hold a gradient
+    g = torch.zeros(T, N, dtype=torch.float16)
+    at = at.unique()
+    g[:, at] = torch.randn(T, at.numel()).half()
+    codes = codes_of(packed[-1:, :, at.cuda()].cpu(), 4)[0].double()
+    gd = g[:, at].double()
+    got = X.quantized_expert_matmul(g.cuda(), stack, plan, sorted_rows=True, transpose_b=True)
+    ref, norm = gd @ ((codes - 8) * 0.01).t(), (gd.square() @ ((codes + 136) * 0.01).square().t()).sqrt()
+    ref[0], norm[0] = gd[0].sum() * -0.08, gd[0].norm() * 1.36
+    part = (gd.square() @ ((codes - 8) * 0.01).square().t()).sqrt()
+    part[0] = gd[0].norm() * 0.08
+    within(got, ref, half_step(ref, torch.float16) + (N * 2.0 ** -24 + 2.0 ** -24) * norm + 8 * 2.0 ** -17 * part)
+
+
 @pytest.mark.parametrize("dt", ["fp16", "bf16", "fp32"])
 @pytest.mark.parametrize("T,k,E,K,N,bits,group", [(6, 2, 4, 256, 192, 4, 64), (50, 2, 2, 128, 384, 8, 0),
                                                   (260, 1, 2, 384, 256, 4, 128), (5, 2, 3, 36, 21, 4, 12)])
@@ -555,6 +648,50 @@ def test_block_in_a_graph_on_another_stream(X, T, dt):
             other = _block(X, x, up, gate, down, ids, w)
         torch.cuda.current_stream().wait_stream(side)
         assert torch.equal(other, want)
+
+
+def test_two_streams_at_once(X):
+    """Calls on two streams, neither waiting for the other, each with its own workspaces."""
+    E, k, K, H, T = 4, 2, 512, 768, 300
+    layers = [(Layer(X, i, E, K, H, 4, 64), Layer(X, i + 5, E, K, H, 4, 64), Layer(X, i + 9, E, H, K, 4, 64))
+              for i in range(2)]
+    xs = [torch.randn(T, K).half().cuda() for _ in range(2)]
+    ids = [ids_of(i, T, k, E).cuda() for i in range(2)]
+    w = torch.rand(T, k).cuda()
+    want = [_block(X, xs[i], *layers[i], ids[i], w) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(6):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(_block(X, xs[i], *layers[i], ids[i], w))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for y in got[i]:
+            assert torch.equal(y, want[i])
+
+
+def test_two_graphs_replayed_in_turn(X):
+    E, k, K, H = 4, 2, 256, 384
+    up, gate, down = Layer(X, 1, E, K, H, 4, 64), Layer(X, 2, E, K, H, 4, 64), Layer(X, 3, E, H, K, 4, 64)
+    graphs = []
+    for T in (3, 260):
+        x, w, ids = torch.randn(T, K).half().cuda(), torch.rand(T, k).cuda(), ids_of(T, T, k, E).cuda()
+        _block(X, x, up, gate, down, ids, w)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = _block(X, x, up, gate, down, ids, w)
+        graphs.append((graph, x, w, ids, out))
+    for _ in range(3):
+        for _, x, _, _, _ in graphs:
+            x.copy_(torch.randn(x.shape))
+        for graph, *_ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, x, w, ids, out in graphs:
+            assert torch.equal(out, _block(X, x, up, gate, down, ids, w))
 
 
 def test_gradient_in_a_graph(X):
