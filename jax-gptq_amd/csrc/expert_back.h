@@ -33,12 +33,22 @@ static __global__ __launch_bounds__(256) void widen_tables_kernel(const char *__
   }
 }
 
+constexpr int BACK_BM = 128, BACK_BN = 256;
+// workgroups that run at a time
+static inline int back_slots(int x_dtype) { return x_dtype == GPTQ_HIP_F32 ? 256 : 512; }
+#ifndef BMOST
+#define BMOST 4
+#define BMIN 8
+#endif
+constexpr int BACK_MOST = BMOST, BACK_MIN_STAGES = BMIN;
+
 struct BackLayout {
+  int slots, most;              // parts of the contraction: see Split
   bool pad, widen;
   int64_t Np, tables;           // row pitch in elements; table elements of all experts
-  size_t tables_at, bytes;
+  size_t tables_at, parts_at, bytes;
 };
-static inline BackLayout back_layout(int64_t x_rows, int64_t R, int64_t N, int bits, int64_t group,
+static inline BackLayout back_layout(int64_t x_rows, int64_t P, int64_t R, int64_t N, int bits, int64_t group,
                                      int E, int x_dtype, int zs_dtype) {
   BackLayout l;
   const int64_t K = bits == 4 ? 2 * R : R, size = x_dtype == GPTQ_HIP_F32 ? 4 : 2;
@@ -47,7 +57,12 @@ static inline BackLayout back_layout(int64_t x_rows, int64_t R, int64_t N, int b
   l.widen = zs_dtype != GPTQ_HIP_F32;
   l.tables = (int64_t)E * (group ? K / group : 1) * N;
   l.tables_at = l.pad ? (size_t)round_up64(x_rows * l.Np * size, 256) : 0;
-  l.bytes = l.tables_at + (l.widen ? (size_t)round_up64(2 * l.tables * 4, 256) : 0);
+  l.parts_at = l.tables_at + (l.widen ? (size_t)round_up64(2 * l.tables * 4, 256) : 0);
+  l.slots = back_slots(x_dtype);
+  const int64_t stages = l.Np * size / 128;
+  l.most = (int)(stages / BACK_MIN_STAGES < BACK_MOST ? stages / BACK_MIN_STAGES : BACK_MOST);
+  if (l.most < 1) l.most = 1;
+  l.bytes = l.parts_at + (size_t)unit_bound(P, E, BACK_BM, ceil_div64(K, BACK_BN), l.slots, l.most) * BACK_BM * BACK_BN * 4;
   return l;
 }
 
@@ -56,12 +71,13 @@ struct BackArgs {
   const char *x;                // rows of whole stages
   const float *zero, *scale;
   int64_t row_bytes;
-  int stages;
+  int stages, slots, most;
+  float *parts;                 // sums of parts
 };
 
 // NG: groups a wavefront's 128 features lie in
 template <int XT, int BITS, bool ALIGNED, int NG> struct BackShape {
-  static constexpr int WAVES = 4, THREADS = 256, BM = 128, BN = 256;
+  static constexpr int WAVES = 4, THREADS = 256, BM = BACK_BM, BN = BACK_BN;
   static constexpr int BK = XT == GPTQ_HIP_F32 ? 32 : 64;           // channels of a stage: 128 bytes of a row
   static constexpr int STEPS = BK / 32;
   static constexpr int PARTS = XT == GPTQ_HIP_F32 ? 3 : 2;
@@ -90,10 +106,12 @@ __global__ __launch_bounds__(256, XT == GPTQ_HIP_F32 ? 1 : 2) void back_kernel(B
   const int64_t N = a.C, K = BITS == 4 ? 2 * a.R : a.R;
   const bool f32 = a.out_dtype == GPTQ_HIP_F32;
 
-  const Item tile = find_item<4>(a.offsets, a.E, (int)a.P, T::BM, (uint32_t)((K + T::BN - 1) / T::BN));
+  const Unit unit = find_unit<4>(a.offsets, a.E, (int)a.P, T::BM, (uint32_t)((K + T::BN - 1) / T::BN), t.slots, t.most);
+  const Item &tile = unit.item;
   if (tile.rows <= 0) return;
   const int64_t k0 = (int64_t)tile.col * T::BN;
   if (tile.expert == a.E) {                            // rows of nowhere
+    if (unit.part > 0) return;
     for (int i = threadIdx.x; i < tile.rows * T::BN; i += T::THREADS) {
       const int64_t k = k0 + i % T::BN;
       if (k < K) store_out<XT>(a.out, f32, (int64_t)(tile.row0 + i / T::BN) * K + k, 0.f);
@@ -282,15 +300,17 @@ __global__ __launch_bounds__(256, XT == GPTQ_HIP_F32 ? 1 : 2) void back_kernel(B
   };
 
   constexpr int AHEAD = T::STAGES - 1;
+  const int first = (int)((int64_t)t.stages * unit.part / unit.parts);
+  const int past = (int)((int64_t)t.stages * (unit.part + 1) / unit.parts);
 #pragma unroll
   for (int s = 0; s < AHEAD; ++s) {
-    issue(s < t.stages ? s : t.stages - 1, s);
+    issue(first + s < past ? first + s : past - 1, s);
     land(s);
   }
   int slot = 0, into = AHEAD;
-  for (int s = 0; s < t.stages; ++s) {
+  for (int s = first; s < past; ++s) {
     wait_and_meet<ALIGNED ? (AHEAD - 1) * T::LOADS : 0>();
-    issue(s + AHEAD < t.stages ? s + AHEAD : t.stages - 1, into);
+    issue(s + AHEAD < past ? s + AHEAD : past - 1, into);
     const char *base = lds + slot * T::STAGE;
 #pragma unroll
     for (int h = 0; h < 2 * T::STEPS; ++h) step(base, h / 2, h % 2);
@@ -309,7 +329,7 @@ __global__ __launch_bounds__(256, XT == GPTQ_HIP_F32 ? 1 : 2) void back_kernel(B
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const int in = 8 * (r / 4) + 4 * hi + r % 4, m = wm * 64 + 32 * i + in;
+      const int in = 8 * (r / 4) + 4 * hi + r % 4;
 #pragma unroll
       for (int b = 0; b < 4 / CB; ++b) {
         float d;
@@ -319,23 +339,91 @@ __global__ __launch_bounds__(256, XT == GPTQ_HIP_F32 ? 1 : 2) void back_kernel(B
         } else {
           d = __shfl(sub[b * NG * CB / 4][i], in);
         }
+#pragma unroll
+        for (int c = 0; c < CB; ++c) acc[i][b * CB + c][r] -= d;
+      }
+    }
+  if (unit.parts > 1) {
+    f32x4 *to = reinterpret_cast<f32x4 *>(t.parts) + (int64_t)unit.slot * (T::BM * T::BN / 4) + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          to[((i * 4 + c) * 4 + j) * 256] =
+              f32x4{acc[i][c][4 * j], acc[i][c][4 * j + 1], acc[i][c][4 * j + 2], acc[i][c][4 * j + 3]};
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+#pragma unroll
+      for (int b = 0; b < 4 / CB; ++b) {
+        const int m = wm * 64 + 32 * i + 8 * (r / 4) + 4 * hi + r % 4;
         const int64_t k = k0 + wn * 128 + CB * (32 * b + l32);
         if (m >= tile.rows || k >= K) continue;
         const int64_t at = (int64_t)(tile.row0 + m) * K + k;
-        if constexpr (CB == 2) store2<XT>(a.out, f32, at, acc[i][2 * b][r] - d, acc[i][2 * b + 1][r] - d);
-        else store_out<XT>(a.out, f32, at, acc[i][b][r] - d);
+        if constexpr (CB == 2) store2<XT>(a.out, f32, at, acc[i][2 * b][r], acc[i][2 * b + 1][r]);
+        else store_out<XT>(a.out, f32, at, acc[i][b][r]);
+      }
+}
+
+// The tiles that were cut, added up part by part: blockIdx.y takes a block of 32 rows of each wavefront's, and
+// one of its pairs of columns' blocks.
+template <int XT, int BITS> __global__ __launch_bounds__(256) void back_join_kernel(BackArgs t) {
+  constexpr int CB = BITS == 4 ? 2 : 1;
+  const ExpertArgs &a = t.a;
+  const int64_t K = BITS == 4 ? 2 * a.R : a.R;
+  const uint32_t cols = (uint32_t)((K + BACK_BN - 1) / BACK_BN);
+  Tiles tiles(a.offsets, a.E, (int)a.P, BACK_BM);
+  const Split s = split_items(tiles.total * cols, t.slots, t.most);
+  if (s.parts < 2 || blockIdx.x >= s.rem) return;
+  const Item tile = tiles.at<4>(s.full + blockIdx.x, cols);
+  const int i = blockIdx.y >> 1, c0 = 2 * (blockIdx.y & 1);
+  const int lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5, wave = threadIdx.x >> 6;
+  const int m0 = (wave >> 1) * 64 + 32 * i + 4 * hi;
+  if (tile.rows <= 0 || tile.expert == a.E) return;
+  const bool f32 = a.out_dtype == GPTQ_HIP_F32;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    f32x4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    for (int p = 0; p < s.parts; ++p) {
+      const f32x4 *from = reinterpret_cast<const f32x4 *>(t.parts) +
+                          ((int64_t)p * s.rem + blockIdx.x) * (BACK_BM * BACK_BN / 4) + threadIdx.x;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) v[c] += from[((i * 4 + c0 + c) * 4 + j) * 256];
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int m = m0 + 8 * j + r;
+      if (m >= tile.rows) continue;
+#pragma unroll
+      for (int b = 0; b < 2 / CB; ++b) {
+        const int64_t k = (int64_t)tile.col * BACK_BN + (wave & 1) * 128 + CB * (32 * (c0 / CB + b) + l32);
+        if (k >= K) continue;
+        const int64_t at = (int64_t)(tile.row0 + m) * K + k;
+        if constexpr (CB == 2) store2<XT>(a.out, f32, at, v[0][r], v[1][r]);
+        else store_out<XT>(a.out, f32, at, v[b][r]);
       }
     }
+  }
 }
 
 template <int XT, int BITS, bool ALIGNED, int NG> static int back_one(hipStream_t s, const BackArgs &t) {
   using T = BackShape<XT, BITS, ALIGNED, NG>;
   const int64_t K = BITS == 4 ? 2 * t.a.R : t.a.R;
-  const unsigned blocks = item_grid(t.a.P, t.a.E, T::BM, ceil_div64(K, T::BN), T::THREADS);
+  const int64_t cols = ceil_div64(K, T::BN), parts = unit_bound(t.a.P, t.a.E, T::BM, cols, t.slots, t.most);
+  const unsigned blocks = item_grid(t.a.P, t.a.E, T::BM, cols, T::THREADS, parts);
   if (!blocks) return GPTQ_HIP_EINVAL;
   if (!gptq_raise_lds_limit((const void *)back_kernel<XT, BITS, ALIGNED, NG>, T::LDS)) return GPTQ_HIP_ELAUNCH;
   back_kernel<XT, BITS, ALIGNED, NG><<<blocks, T::THREADS, T::LDS, s>>>(t);
   GPTQ_CHECK_LAUNCH();
+  if (parts) {
+    back_join_kernel<XT, BITS><<<dim3((unsigned)(parts / 2), 4), 256, 0, s>>>(t);
+    GPTQ_CHECK_LAUNCH();
+  }
   return GPTQ_HIP_OK;
 }
 template <int XT, int BITS, bool ALIGNED> static int back_groups(hipStream_t s, const BackArgs &t) {
@@ -344,10 +432,10 @@ template <int XT, int BITS, bool ALIGNED> static int back_groups(hipStream_t s, 
 }
 
 template <int XT> static int back_launch(hipStream_t s, const ExpertArgs &a, void *ws) {
-  const BackLayout l = back_layout(a.T, a.R, a.C, a.bits, a.group, a.E, a.x_dtype, a.zs_dtype);
+  const BackLayout l = back_layout(a.T, a.P, a.R, a.C, a.bits, a.group, a.E, a.x_dtype, a.zs_dtype);
   constexpr int SZ = XT == GPTQ_HIP_F32 ? 4 : 2;
   BackArgs t = {a, (const char *)a.x, (const float *)a.zero, (const float *)a.scale, l.Np * SZ,
-                (int)(l.Np * SZ / 128)};
+                (int)(l.Np * SZ / 128), l.slots, l.most, (float *)((char *)ws + l.parts_at)};
   if (l.pad) {
     typedef typename std::conditional<SZ == 4, uint32_t, uint16_t>::type U;
     pad_rows_kernel<U><<<(unsigned)a.T, 256, 0, s>>>((const U *)a.x, a.C, l.Np, (U *)ws);

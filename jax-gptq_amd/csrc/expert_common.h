@@ -168,70 +168,124 @@ __device__ __forceinline__ void parts3(const u32x4 &lo4, const u32x4 &hi4, u32x4
 
 // Which rows and columns a workgroup owns.  Tiles of H rows are counted expert by expert (the rows of nowhere as one
 // more) and each comes with `cols` columns; PANEL columns at a time (0: all), all tiles of them, make the list of items.
-// Workgroups go round the eight XCDs; each XCD takes a run of the list, so what runs on it at a time shares rows and
-// weights (and lines that two neighbouring strips begin in) in its L2.  The counts come from a scan over the experts, 64
-// at a time; every wavefront does it for itself.
+// The counts come from a scan over the experts, 64 at a time; every wavefront does it for itself.
 struct Item {
   int expert, row0, rows, col;        // rows == 0: nothing to do
 };
-template <int PANEL>
-__device__ __forceinline__ Item find_item(const int *__restrict__ offsets, int E, int P, int H, uint32_t cols) {
-  const int lane = threadIdx.x & 63;
-  auto tiles_of = [&](int e, int &lo, int &hi) -> int {
-    lo = hi = 0;
+struct Tiles {
+  const int *__restrict__ offsets;
+  int E, P, H, lo, hi, n, scan;
+  uint32_t total;
+
+  __device__ __forceinline__ int count(int e, int &l, int &h) const {
+    l = h = 0;
     if (e <= E) {                       // (whatever the offsets say, no row outside 0 .. P - 1)
-      lo = min(max(offsets[e], 0), P);
-      hi = e < E ? min(max(offsets[e + 1], lo), P) : P;
+      l = min(max(offsets[e], 0), P);
+      h = e < E ? min(max(offsets[e + 1], l), P) : P;
     }
-    return (hi - lo + H - 1) / H;
-  };
-  auto scan_of = [&](int n) -> int {
+    return (h - l + H - 1) / H;
+  }
+  __device__ __forceinline__ void load(int e0) {
+    const int lane = threadIdx.x & 63;
+    n = scan = count(e0 + lane, lo, hi);
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-      const int up = __shfl_up(n, d);
-      if (lane >= d) n += up;
+      const int up = __shfl_up(scan, d);
+      if (lane >= d) scan += up;
     }
-    return n;
-  };
-  int lo, hi, n = tiles_of(lane, lo, hi), scan = scan_of(n), total = __shfl(scan, 63);
-  if (E >= 64) {
-    int more = 0, l, h;
-    for (int e = 64 + lane; e <= E; e += 64) more += tiles_of(e, l, h);
-#pragma unroll
-    for (int d = 32; d; d >>= 1) more += __shfl_xor(more, d);
-    total += more;
   }
-  const uint32_t tiles = (uint32_t)__builtin_amdgcn_readfirstlane(total), items = tiles * cols, run = (items + 7) / 8;
+  __device__ __forceinline__ Tiles(const int *offsets_, int E_, int P_, int H_)
+      : offsets(offsets_), E(E_), P(P_), H(H_) {
+    load(0);
+    int all = __shfl(scan, 63);
+    if (E >= 64) {
+      int more = 0, l, h;
+      for (int e = 64 + (threadIdx.x & 63); e <= E; e += 64) more += count(e, l, h);
+#pragma unroll
+      for (int d = 32; d; d >>= 1) more += __shfl_xor(more, d);
+      all += more;
+    }
+    total = (uint32_t)__builtin_amdgcn_readfirstlane(all);
+  }
+  template <int PANEL> __device__ __forceinline__ Item at(uint32_t item, uint32_t cols) {
+    const uint32_t panel = PANEL ? item / (total * PANEL) : 0u, rest = item - panel * total * PANEL;
+    const uint32_t left = cols - PANEL * panel, width = PANEL && left > (uint32_t)PANEL ? (uint32_t)PANEL : left;
+    const int tile = (int)(rest / width), col = (int)(PANEL * panel + rest % width);
+    int before = 0;
+    for (int e0 = 0;; e0 += 64) {
+      if (e0 > 0) load(e0);
+      const uint64_t past = __ballot(before + scan > tile);
+      if (past) {
+        const int who = __ffsll((unsigned long long)past) - 1;
+        const int first = before + __shfl(scan - n, who);
+        const int l = __shfl(lo, who), h = __shfl(hi, who), row0 = l + (tile - first) * H;
+        const int rows = h - row0 < H ? h - row0 : H;
+        return {__builtin_amdgcn_readfirstlane(e0 + who), __builtin_amdgcn_readfirstlane(row0),
+                __builtin_amdgcn_readfirstlane(rows), col};
+      }
+      before += __shfl(scan, 63);
+      if (e0 + 64 > E) return {0, 0, 0, 0};
+    }
+  }
+};
+// Workgroups go round the eight XCDs; each XCD takes a run of the list, so what runs on it at a time shares rows and
+// weights (and lines that two neighbouring strips begin in) in its L2.
+template <int PANEL>
+__device__ __forceinline__ Item find_item(const int *__restrict__ offsets, int E, int P, int H, uint32_t cols) {
+  Tiles tiles(offsets, E, P, H);
+  const uint32_t items = tiles.total * cols, run = (items + 7) / 8;
   const uint32_t pos = blockIdx.x >> 3, item = (blockIdx.x & 7) * run + pos;
   if (pos >= run || item >= items) return {0, 0, 0, 0};
-  const uint32_t panel = PANEL ? item / (tiles * PANEL) : 0u, rest = item - panel * tiles * PANEL;
-  const uint32_t left = cols - PANEL * panel, width = PANEL && left > (uint32_t)PANEL ? (uint32_t)PANEL : left;
-  const int tile = (int)(rest / width), col = (int)(PANEL * panel + rest % width);
-  int before = 0;
-  for (int e0 = 0;; e0 += 64) {
-    if (e0 > 0) {
-      n = tiles_of(e0 + lane, lo, hi);
-      scan = scan_of(n);
-    }
-    const uint64_t past = __ballot(before + scan > tile);
-    if (past) {
-      const int who = __ffsll((unsigned long long)past) - 1;
-      const int first = before + __shfl(scan - n, who);
-      const int l = __shfl(lo, who), h = __shfl(hi, who), row0 = l + (tile - first) * H;
-      const int rows = h - row0 < H ? h - row0 : H;
-      return {__builtin_amdgcn_readfirstlane(e0 + who), __builtin_amdgcn_readfirstlane(row0),
-              __builtin_amdgcn_readfirstlane(rows), col};
-    }
-    before += __shfl(scan, 63);
-    if (e0 + 64 > E) return {0, 0, 0, 0};
+  return tiles.at<PANEL>(item, cols);
+}
+// The same where the items of the last, incomplete round are cut into parts: `slots` workgroups run at a time, so what
+// is left over after whole rounds of them leaves the chip nearly idle, and as many parts of the contraction as fit fill
+// it.  A second kernel adds the parts up, in order.
+struct Split {
+  uint32_t full, rem;                 // items in whole rounds, and after them
+  int parts;                          // of each of those
+};
+__device__ __host__ __forceinline__ Split split_items(uint32_t items, uint32_t slots, int most) {
+  Split s;
+  s.full = items / slots * slots;
+  s.rem = items - s.full;
+  s.parts = s.rem ? (int)(slots / s.rem) : 1;
+  if (s.parts > most) s.parts = most;
+  return s;
+}
+struct Unit {
+  Item item;
+  int part, parts, slot;              // slot: of the parts' sums
+};
+template <int PANEL>
+__device__ __forceinline__ Unit find_unit(const int *__restrict__ offsets, int E, int P, int H, uint32_t cols,
+                                          uint32_t slots, int most) {
+  Tiles tiles(offsets, E, P, H);
+  const uint32_t items = tiles.total * cols;
+  const Split s = split_items(items, slots, most);
+  const uint32_t whole = s.parts == 1 ? items : s.full;          // items that stay in one piece, a run for each XCD
+  const uint32_t run = (whole + 7) / 8;
+  if (blockIdx.x < 8 * run) {
+    const uint32_t item = (blockIdx.x & 7) * run + (blockIdx.x >> 3);
+    if (item >= whole) return {{0, 0, 0, 0}, 0, 1, 0};
+    return {tiles.at<PANEL>(item, cols), 0, 1, 0};
   }
+  if (s.parts == 1) return {{0, 0, 0, 0}, 0, 1, 0};
+  const uint32_t u = blockIdx.x - s.full;
+  if (u >= s.rem * (uint32_t)s.parts) return {{0, 0, 0, 0}, 0, 1, 0};
+  return {tiles.at<PANEL>(s.full + u % s.rem, cols), (int)(u / s.rem), s.parts, (int)u};
 }
 // tiles there can be
 static inline int64_t tile_bound(int64_t P, int E, int H) { return P / H + (P < E + 1 ? P : E + 1); }
-// workgroups of `threads` for all items there can be; 0: too many for a launch
-static inline unsigned item_grid(int64_t P, int E, int H, int64_t cols, int threads) {
-  const int64_t blocks = round_up64(tile_bound(P, E, H) * cols, 8);
+// workgroups of `threads` for all items there can be, and `parts` more; 0: too many for a launch
+static inline unsigned item_grid(int64_t P, int E, int H, int64_t cols, int threads, int64_t parts = 0) {
+  const int64_t blocks = round_up64(tile_bound(P, E, H) * cols, 8) + parts;
   return blocks * threads >= (int64_t)1 << 32 ? 0u : (unsigned)blocks;
+}
+// parts of items there can be, of which each keeps its sums (in at most `slots` places)
+static inline int64_t unit_bound(int64_t P, int E, int H, int64_t cols, int64_t slots, int most) {
+  const int64_t items = tile_bound(P, E, H) * cols;
+  return most < 2 ? 0 : (items * most < slots ? items * most : slots);
 }
 
 // the row of x that row p reads

@@ -187,7 +187,7 @@ size_t gptq_hip_expert_qmatmul_workspace_bytes(int64_t x_rows, int64_t rows, int
   if (c.kind == Choice::TILE)
     return xqmm::staged_layout(x_rows, bits == 4 ? 2 * R : R, x_dtype, xqmm::tile_half(group_size)).bytes;
   if (c.kind == Choice::BACK)
-    return xqmm::back_layout(x_rows, R, C, bits, group_size, n_experts, x_dtype, zs_dtype).bytes;
+    return xqmm::back_layout(x_rows, rows, R, C, bits, group_size, n_experts, x_dtype, zs_dtype).bytes;
   return 0;
 }
 
