@@ -33,17 +33,26 @@ static __global__ __launch_bounds__(256) void widen_tables_kernel(const char *__
   }
 }
 
-constexpr int BACK_BM = 128, BACK_BN = 256;
-// workgroups that run at a time
-static inline int back_slots(int x_dtype) { return x_dtype == GPTQ_HIP_F32 ? 256 : 512; }
-#ifndef BMOST
-#define BMOST 4
-#define BMIN 8
-#endif
-constexpr int BACK_MOST = BMOST, BACK_MIN_STAGES = BMIN;
+constexpr int BACK_BN = 256;
+// A contraction is cut into at most four parts of at least eight stages (six or eight parts, or of four stages, are no
+// faster: what the tiles gain their sums' way through memory costs).
+constexpr int BACK_MOST = 4, BACK_MIN_STAGES = 8;
+
+// Rows of a tile, by the rows of an expert on average.  The instructions that make the operands of codes are shared by
+// its rows, so a tall tile is the faster the fuller it is.  Measured with 32 / 64 / 128 rows, us a call:
+//   8 experts 4096 x 4096, fp16:   8 rows each 53 75 88,  60: 76 80 86,  125: 145 108 128,  200: 148 141 144,
+//                                  375: 317 235 232,  512: 384 300 274
+//   64 experts 2048 x 1424, bf16:  10 rows each 59 90 120,  31: 81 92 122,  64: 128 125 128,  256: 374 342 364
+//   8 experts 4096 x 4096, fp32:   8 rows each 66 77 131,  40: 115 77 130,  162: 224 251 235,  512: 565 525 525
+enum BackRows { BACK_32, BACK_64, BACK_128 };
+static inline BackRows back_rows(int64_t P, int E) {
+  const int64_t rows = P / E;
+  return rows <= 32 ? BACK_32 : (rows <= 256 ? BACK_64 : BACK_128);
+}
 
 struct BackLayout {
-  int slots, most;              // parts of the contraction: see Split
+  BackRows rows;
+  int slots, most;              // workgroups that run at a time; parts of the contraction: see Split
   bool pad, widen;
   int64_t Np, tables;           // row pitch in elements; table elements of all experts
   size_t tables_at, parts_at, bytes;
@@ -58,11 +67,13 @@ static inline BackLayout back_layout(int64_t x_rows, int64_t P, int64_t R, int64
   l.tables = (int64_t)E * (group ? K / group : 1) * N;
   l.tables_at = l.pad ? (size_t)round_up64(x_rows * l.Np * size, 256) : 0;
   l.parts_at = l.tables_at + (l.widen ? (size_t)round_up64(2 * l.tables * 4, 256) : 0);
-  l.slots = back_slots(x_dtype);
+  l.rows = back_rows(P, E);
+  l.slots = (x_dtype == GPTQ_HIP_F32 ? 512 : 1024) / (l.rows == BACK_128 ? 2 : 1);
   const int64_t stages = l.Np * size / 128;
   l.most = (int)(stages / BACK_MIN_STAGES < BACK_MOST ? stages / BACK_MIN_STAGES : BACK_MOST);
   if (l.most < 1) l.most = 1;
-  l.bytes = l.parts_at + (size_t)unit_bound(P, E, BACK_BM, ceil_div64(K, BACK_BN), l.slots, l.most) * BACK_BM * BACK_BN * 4;
+  const int BM = l.rows == BACK_128 ? 128 : (l.rows == BACK_64 ? 64 : 32);
+  l.bytes = l.parts_at + (size_t)unit_bound(P, E, BM, ceil_div64(K, BACK_BN), l.slots, l.most) * BM * BACK_BN * 4;
   return l;
 }
 
@@ -75,9 +86,9 @@ struct BackArgs {
   float *parts;                 // sums of parts
 };
 
-// NG: groups a wavefront's 128 features lie in
-template <int XT, int BITS, bool ALIGNED, int NG> struct BackShape {
-  static constexpr int WAVES = 4, THREADS = 256, BM = BACK_BM, BN = BACK_BN;
+// NG: groups a wavefront's 128 features lie in; the tile's rows are WM times RB blocks of 32, a wavefront has RB of them
+template <int XT, int BITS, bool ALIGNED, int NG, int WM, int RB> struct BackShape {
+  static constexpr int WAVES = 2 * WM, THREADS = 64 * WAVES, BM = 32 * RB * WM, BN = BACK_BN;
   static constexpr int BK = XT == GPTQ_HIP_F32 ? 32 : 64;           // channels of a stage: 128 bytes of a row
   static constexpr int STEPS = BK / 32;
   static constexpr int PARTS = XT == GPTQ_HIP_F32 ? 3 : 2;
@@ -85,15 +96,15 @@ template <int XT, int BITS, bool ALIGNED, int NG> struct BackShape {
   static constexpr int TROWS = 2 * NG;                              // table rows of the tile
   static constexpr int A = BM * 128, B = ROWS * BK, Z = TROWS * 256;
   static constexpr int STAGE = A + B + 2 * Z;
-  static constexpr int STAGES = 3 * STAGE <= 80 * 1024 ? 3 : 2;     // two workgroups share a CU
+  static constexpr int STAGES = 3 * STAGE <= 40 * 1024 * WM ? 3 : 2;     // wavefronts of eight such tiles' rows share a CU
   static constexpr int LDS = STAGES * STAGE;
   static constexpr int AI = A / 1024 / WAVES, BI = B / 1024 / WAVES, ZI = 2 * TROWS / WAVES;
   static constexpr int LOADS = AI + BI + ZI;
 };
 
-template <int XT, int BITS, bool ALIGNED, int NG>
-__global__ __launch_bounds__(256, XT == GPTQ_HIP_F32 ? 1 : 2) void back_kernel(BackArgs t) {
-  using T = BackShape<XT, BITS, ALIGNED, NG>;
+template <int XT, int BITS, bool ALIGNED, int NG, int WM, int RB>
+__global__ __launch_bounds__(128 * WM, XT == GPTQ_HIP_F32 ? 1 : 2) void back_kernel(BackArgs t) {
+  using T = BackShape<XT, BITS, ALIGNED, NG, WM, RB>;
   using O = Op<GPTQ_HIP_BF16>;
   typedef __attribute__((address_space(3))) char lds_char;
   constexpr bool CONVERT = XT == GPTQ_HIP_F32 || BITS == 8;         // codes as c itself, else as 128 + c
@@ -189,10 +200,10 @@ __global__ __launch_bounds__(256, XT == GPTQ_HIP_F32 ? 1 : 2) void back_kernel(B
   // 32 x 32 products over 16 channels: row (column) l32, 8 channels a lane; sums lie with column l32, rows
   // 8 (r / 4) + 4 hi + r % 4.  A lane's packed row gives it two columns at 4 bits (low and high codes), one at 8.
   constexpr int CB = BITS == 4 ? 2 : 1;
-  f32x16 acc[2][4];                                     // [row block][column block]
-  float sub[NG][2];
+  f32x16 acc[RB][4];                                     // [row block][column block]
+  float sub[NG][RB];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < RB; ++i) {
 #pragma unroll
     for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -215,10 +226,10 @@ __global__ __launch_bounds__(256, XT == GPTQ_HIP_F32 ? 1 : 2) void back_kernel(B
 #pragma unroll
         for (int i = 0; i < 4; ++i) { z[4 * v + i] = zv[i] + OFFSET; s[4 * v + i] = sv[i]; }
       }
-      u32x4 x[2][T::PARTS];
+      u32x4 x[RB][T::PARTS];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const char *row = base + (wm * 64 + 32 * i + l32) * 128;
+      for (int i = 0; i < RB; ++i) {
+        const char *row = base + (wm * 32 * RB + 32 * i + l32) * 128;
         uint32_t part[T::PARTS][8];
 #pragma unroll
         for (int e4 = 0; e4 < 2; ++e4) {                // 4 channels at a time (fp32), or of 8 (16 bits)
@@ -290,7 +301,7 @@ __global__ __launch_bounds__(256, XT == GPTQ_HIP_F32 ? 1 : 2) void back_kernel(B
 #pragma unroll
         for (int c = 0; c < CB; ++c)
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
+          for (int i = 0; i < RB; ++i)
 #pragma unroll
             for (int p = 0; p < T::PARTS; ++p) acc[i][b * CB + c] = O::mma32(x[i][p], op[c], acc[i][b * CB + c]);
       }
@@ -324,9 +335,9 @@ __global__ __launch_bounds__(256, XT == GPTQ_HIP_F32 ? 1 : 2) void back_kernel(B
 #pragma unroll
   for (int g = 0; g < NG; ++g)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) sub[g][i] += __shfl_xor(sub[g][i], 32);
+    for (int i = 0; i < RB; ++i) sub[g][i] += __shfl_xor(sub[g][i], 32);
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < RB; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int in = 8 * (r / 4) + 4 * hi + r % 4;
@@ -346,22 +357,22 @@ __global__ __launch_bounds__(256, XT == GPTQ_HIP_F32 ? 1 : 2) void back_kernel(B
   if (unit.parts > 1) {
     f32x4 *to = reinterpret_cast<f32x4 *>(t.parts) + (int64_t)unit.slot * (T::BM * T::BN / 4) + threadIdx.x;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < RB; ++i)
 #pragma unroll
       for (int c = 0; c < 4; ++c)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          to[((i * 4 + c) * 4 + j) * 256] =
+          to[((i * 4 + c) * 4 + j) * T::THREADS] =
               f32x4{acc[i][c][4 * j], acc[i][c][4 * j + 1], acc[i][c][4 * j + 2], acc[i][c][4 * j + 3]};
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < RB; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r)
 #pragma unroll
       for (int b = 0; b < 4 / CB; ++b) {
-        const int m = wm * 64 + 32 * i + 8 * (r / 4) + 4 * hi + r % 4;
+        const int m = wm * 32 * RB + 32 * i + 8 * (r / 4) + 4 * hi + r % 4;
         const int64_t k = k0 + wn * 128 + CB * (32 * b + l32);
         if (m >= tile.rows || k >= K) continue;
         const int64_t at = (int64_t)(tile.row0 + m) * K + k;
@@ -372,18 +383,18 @@ __global__ __launch_bounds__(256, XT == GPTQ_HIP_F32 ? 1 : 2) void back_kernel(B
 
 // The tiles that were cut, added up part by part: blockIdx.y takes a block of 32 rows of each wavefront's, and
 // one of its pairs of columns' blocks.
-template <int XT, int BITS> __global__ __launch_bounds__(256) void back_join_kernel(BackArgs t) {
-  constexpr int CB = BITS == 4 ? 2 : 1;
+template <int XT, int BITS, int WM, int RB> __global__ __launch_bounds__(128 * WM) void back_join_kernel(BackArgs t) {
+  constexpr int CB = BITS == 4 ? 2 : 1, BM = 32 * RB * WM;
   const ExpertArgs &a = t.a;
   const int64_t K = BITS == 4 ? 2 * a.R : a.R;
   const uint32_t cols = (uint32_t)((K + BACK_BN - 1) / BACK_BN);
-  Tiles tiles(a.offsets, a.E, (int)a.P, BACK_BM);
+  Tiles tiles(a.offsets, a.E, (int)a.P, BM);
   const Split s = split_items(tiles.total * cols, t.slots, t.most);
   if (s.parts < 2 || blockIdx.x >= s.rem) return;
   const Item tile = tiles.at<4>(s.full + blockIdx.x, cols);
   const int i = blockIdx.y >> 1, c0 = 2 * (blockIdx.y & 1);
   const int lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5, wave = threadIdx.x >> 6;
-  const int m0 = (wave >> 1) * 64 + 32 * i + 4 * hi;
+  const int m0 = (wave >> 1) * 32 * RB + 32 * i + 4 * hi;
   if (tile.rows <= 0 || tile.expert == a.E) return;
   const bool f32 = a.out_dtype == GPTQ_HIP_F32;
 #pragma unroll
@@ -391,9 +402,9 @@ template <int XT, int BITS> __global__ __launch_bounds__(256) void back_join_ker
     f32x4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
     for (int p = 0; p < s.parts; ++p) {
       const f32x4 *from = reinterpret_cast<const f32x4 *>(t.parts) +
-                          ((int64_t)p * s.rem + blockIdx.x) * (BACK_BM * BACK_BN / 4) + threadIdx.x;
+                          ((int64_t)p * s.rem + blockIdx.x) * (BM * BACK_BN / 4) + threadIdx.x;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) v[c] += from[((i * 4 + c0 + c) * 4 + j) * 256];
+      for (int c = 0; c < 2; ++c) v[c] += from[((i * 4 + c0 + c) * 4 + j) * 128 * WM];
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -411,24 +422,29 @@ template <int XT, int BITS> __global__ __launch_bounds__(256) void back_join_ker
   }
 }
 
-template <int XT, int BITS, bool ALIGNED, int NG> static int back_one(hipStream_t s, const BackArgs &t) {
-  using T = BackShape<XT, BITS, ALIGNED, NG>;
+template <int XT, int BITS, bool ALIGNED, int NG, int WM, int RB> static int back_one(hipStream_t s, const BackArgs &t) {
+  using T = BackShape<XT, BITS, ALIGNED, NG, WM, RB>;
   const int64_t K = BITS == 4 ? 2 * t.a.R : t.a.R;
   const int64_t cols = ceil_div64(K, T::BN), parts = unit_bound(t.a.P, t.a.E, T::BM, cols, t.slots, t.most);
   const unsigned blocks = item_grid(t.a.P, t.a.E, T::BM, cols, T::THREADS, parts);
   if (!blocks) return GPTQ_HIP_EINVAL;
-  if (!gptq_raise_lds_limit((const void *)back_kernel<XT, BITS, ALIGNED, NG>, T::LDS)) return GPTQ_HIP_ELAUNCH;
-  back_kernel<XT, BITS, ALIGNED, NG><<<blocks, T::THREADS, T::LDS, s>>>(t);
+  if (!gptq_raise_lds_limit((const void *)back_kernel<XT, BITS, ALIGNED, NG, WM, RB>, T::LDS)) return GPTQ_HIP_ELAUNCH;
+  back_kernel<XT, BITS, ALIGNED, NG, WM, RB><<<blocks, T::THREADS, T::LDS, s>>>(t);
   GPTQ_CHECK_LAUNCH();
   if (parts) {
-    back_join_kernel<XT, BITS><<<dim3((unsigned)(parts / 2), 4), 256, 0, s>>>(t);
+    back_join_kernel<XT, BITS, WM, RB><<<dim3((unsigned)(parts / 2), 2 * RB), T::THREADS, 0, s>>>(t);
     GPTQ_CHECK_LAUNCH();
   }
   return GPTQ_HIP_OK;
 }
-template <int XT, int BITS, bool ALIGNED> static int back_groups(hipStream_t s, const BackArgs &t) {
-  if (t.a.group % 128 == 0) return back_one<XT, BITS, ALIGNED, 1>(s, t);
-  return t.a.group % 64 == 0 ? back_one<XT, BITS, ALIGNED, 2>(s, t) : back_one<XT, BITS, ALIGNED, 4>(s, t);
+template <int XT, int BITS, bool ALIGNED, int WM, int RB> static int back_groups(hipStream_t s, const BackArgs &t) {
+  if (t.a.group % 128 == 0) return back_one<XT, BITS, ALIGNED, 1, WM, RB>(s, t);
+  return t.a.group % 64 == 0 ? back_one<XT, BITS, ALIGNED, 2, WM, RB>(s, t)
+                             : back_one<XT, BITS, ALIGNED, 4, WM, RB>(s, t);
+}
+template <int XT, int BITS, bool ALIGNED> static int back_shape(hipStream_t s, const BackArgs &t, BackRows rows) {
+  if (rows == BACK_32) return back_groups<XT, BITS, ALIGNED, 1, 1>(s, t);
+  return rows == BACK_64 ? back_groups<XT, BITS, ALIGNED, 1, 2>(s, t) : back_groups<XT, BITS, ALIGNED, 2, 2>(s, t);
 }
 
 template <int XT> static int back_launch(hipStream_t s, const ExpertArgs &a, void *ws) {
@@ -452,8 +468,8 @@ template <int XT> static int back_launch(hipStream_t s, const ExpertArgs &a, voi
     t.scale = f + l.tables;
   }
   if (a.C % 16 == 0 && (uintptr_t)a.packed % 16 == 0)
-    return a.bits == 4 ? back_groups<XT, 4, true>(s, t) : back_groups<XT, 8, true>(s, t);
-  return a.bits == 4 ? back_groups<XT, 4, false>(s, t) : back_groups<XT, 8, false>(s, t);
+    return a.bits == 4 ? back_shape<XT, 4, true>(s, t, l.rows) : back_shape<XT, 8, true>(s, t, l.rows);
+  return a.bits == 4 ? back_shape<XT, 4, false>(s, t, l.rows) : back_shape<XT, 8, false>(s, t, l.rows);
 }
 
 }  // namespace xqmm

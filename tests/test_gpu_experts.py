@@ -350,6 +350,12 @@ MORE_SHAPES = [
     (200, 1, 1, 4160, 64, 8, 0, 0),
     (260, 2, 64, 64, 1100, 4, 32, 0.05),      # 8 rows each, tiles of 256 channels
     (64, 1, 1, 64, 16, 4, 32, 0),
+    (300, 2, 4, 576, 2064, 4, 64, 0.1),       # contractions that are cut, also where rows go nowhere
+    (90, 1, 2, 288, 4096, 8, 32, 0.1),
+    (20, 2, 4, 260, 1100, 4, 0, 0),
+    (600, 2, 2, 512, 1040, 4, 128, 0.05),
+    (1200, 2, 600, 128, 1024, 4, 0, 0),       # more tiles than run at a time: the last ones are cut
+    (620, 1, 1, 512, 1040, 8, 64, 0),
 ]
 
 
