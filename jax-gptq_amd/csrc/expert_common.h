@@ -255,7 +255,7 @@ __device__ __host__ __forceinline__ Split split_items(uint32_t items, uint32_t s
 }
 struct Unit {
   Item item;
-  int part, parts, slot;              // slot: of the parts' sums
+  int part, parts, slot;              // slot: of the part's sums
 };
 template <int PANEL>
 __device__ __forceinline__ Unit find_unit(const int *__restrict__ offsets, int E, int P, int H, uint32_t cols,

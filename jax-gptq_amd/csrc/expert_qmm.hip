@@ -185,7 +185,7 @@ size_t gptq_hip_expert_qmatmul_workspace_bytes(int64_t x_rows, int64_t rows, int
   if (n_experts < 1 || rows <= 0 || x_rows <= 0 || R <= 0 || C <= 0 || group_size < 0) return 0;
   const Choice c = choose(rows, n_experts, C, group_size, x_dtype, transpose_b);
   if (c.kind == Choice::TILE)
-    return xqmm::staged_layout(x_rows, bits == 4 ? 2 * R : R, x_dtype, xqmm::tile_half(group_size)).bytes;
+    return xqmm::staged_layout(x_rows, rows, bits == 4 ? 2 * R : R, C, group_size, n_experts, x_dtype, c.shape).bytes;
   if (c.kind == Choice::BACK)
     return xqmm::back_layout(x_rows, rows, R, C, bits, group_size, n_experts, x_dtype, zs_dtype).bytes;
   return 0;

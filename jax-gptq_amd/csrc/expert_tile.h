@@ -17,6 +17,10 @@
 // whole stages, and the sums of every row over the part of its group up to the end of each stage, as such an operand.
 #pragma once
 #include "expert_common.h"
+#include <math.h>
+#ifndef PAYS
+#define PAYS 0.3
+#endif
 
 namespace xqmm {
 
@@ -42,20 +46,42 @@ template <int VM> __device__ __forceinline__ void wait_and_meet() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(VM) : "memory");
 }
 
+// parts of a contraction at most, stages of one at least, workgroups that run at a time at most
+constexpr int TILE_MOST = 4, TILE_MIN_STAGES = 8, TILE_SLOTS = 512;
+static inline int tile_rows(int shape) { return shape == TILE_32x128_K2 || shape == TILE_32x256 ? 32 : 64; }
+static inline int tile_cols(int shape) { return shape == TILE_32x128_K2 ? 128 : 256; }
+// groups that are no multiple of a stage are closed after every k-step
+static inline bool tile_half(int64_t group) { return group % 64 != 0; }
+// stages of a group, or of a piece of a sum without groups
+static inline int tile_close(int64_t group) { return tile_half(group) ? 1 : (int)(group ? group : TILE_LONG) / 64; }
+
 // layout of the workspace
 struct Staged {
   int64_t Kp;              // K padded to whole stages
   int64_t row_bytes;       // of the staged activations: parts * Kp * 2
   int64_t per_row;         // sums of a row, 16 bytes each: one per stage, or per k-step where groups are odd multiples of 32
-  size_t sums_at, bytes;
+  int most;                // parts of the contraction: see Split
+  size_t sums_at, parts_at, bytes;
 };
-static inline Staged staged_layout(int64_t x_rows, int64_t K, int x_dtype, bool half) {
+static inline Staged staged_layout(int64_t x_rows, int64_t P, int64_t K, int64_t N, int64_t group, int E, int x_dtype,
+                                   int shape) {
+  const bool half = tile_half(group);
   Staged l;
   l.Kp = round_up64(K, TILE_BK);
   l.row_bytes = (x_dtype == GPTQ_HIP_F32 ? 3 : 1) * l.Kp * 2;
   l.per_row = l.Kp / (half ? 32 : 64);
   l.sums_at = (size_t)round_up64(x_rows * l.row_bytes, 256);
-  l.bytes = l.sums_at + (size_t)(x_rows * l.per_row) * 16;
+  l.parts_at = (size_t)round_up64(l.sums_at + (x_rows * l.per_row) * 16, 256);
+  const int64_t stages = l.Kp / TILE_BK, groups = ceil_div64(stages, tile_close(group));
+  const int64_t most = groups < stages / TILE_MIN_STAGES ? groups : stages / TILE_MIN_STAGES;
+  const int BM = tile_rows(shape), BN = tile_cols(shape);
+  // Whether to cut at all is settled here, by the tiles that P rows come to when their experts are drawn at random: the
+  // second kernel costs 2 to 4 us also where it finds nothing to add up.
+  const double busy = E * (1.0 - exp(-(double)P / E)), items = ((double)P / BM + busy / 2) * ceil_div64(N, BN);
+  const int slots = shape == TILE_64x256_K2 || x_dtype == GPTQ_HIP_F32 ? TILE_SLOTS / 2 : TILE_SLOTS;
+  const bool pays = items - slots * floor(items / slots) <= PAYS * slots;
+  l.most = (int)(most < 1 || !pays ? 1 : (most < TILE_MOST ? most : TILE_MOST));
+  l.bytes = l.parts_at + (size_t)unit_bound(P, E, BM, ceil_div64(N, BN), TILE_SLOTS, l.most) * BM * BN * 4;
   return l;
 }
 
@@ -163,7 +189,8 @@ struct TileArgs {
   int64_t row_bytes, Kp, per_row;
   int stages;                 // Kp / 64
   int close;                  // stages of a group (or of a piece of the sum)
-  int grouped;
+  int grouped, most;
+  float *parts;               // sums of parts
 };
 
 // ZL: how tables lie in LDS: 4 or 2 bytes an element as they are in memory, 0: operands that start or end anywhere,
@@ -185,6 +212,7 @@ template <int XT, int BITS, int ZL, bool HALF, int RBW, int WM, int WN, int WK> 
   static constexpr int ROOM = (WAVES == 4 && 2 * STAGE + TABLE <= 80 * 1024 ? 80 * 1024 : 160 * 1024) - TABLE;
   static constexpr int STAGES = 4 * STAGE <= ROOM ? 4 : (3 * STAGE <= ROOM ? 3 : 2);
   static constexpr int LDS = STAGES * STAGE + TABLE;
+  static constexpr int SLOTS = WAVES == 4 && LDS <= 80 * 1024 ? TILE_SLOTS : TILE_SLOTS / 2;   // that run at a time
   // loads of a wavefront per stage
   static constexpr int AI = A / 1024 / WAVES, BI = B / 1024 / WAVES;
   static constexpr int SI = WK * HN * MB, TI = WK * HN * (BN / 128), ITEMS = SI + TI;
@@ -208,10 +236,12 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
   const int64_t N = a.C;
   const bool f32 = a.out_dtype == GPTQ_HIP_F32;
 
-  const Item tile = find_item<4>(a.offsets, a.E, (int)a.P, T::BM, (uint32_t)((N + T::BN - 1) / T::BN));
+  const Unit unit = find_unit<4>(a.offsets, a.E, (int)a.P, T::BM, (uint32_t)((N + T::BN - 1) / T::BN), T::SLOTS, t.most);
+  const Item &tile = unit.item;
   if (tile.rows <= 0) return;
   const int64_t n0 = (int64_t)tile.col * T::BN;
   if (tile.expert == a.E) {                            // rows of nowhere
+    if (unit.part > 0) return;
     for (int i = threadIdx.x; i < tile.rows * T::BN; i += T::THREADS) {
       const int64_t n = n0 + i % T::BN;
       if (n < N) store_out<XT>(a.out, f32, (int64_t)(tile.row0 + i / T::BN) * N + n, 0.f);
@@ -226,11 +256,14 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
   const int zsize = a.zs_dtype == GPTQ_HIP_F32 ? 4 : 2;
   const char *zero = (const char *)a.zero + (int64_t)tile.expert * tables * N * zsize;
   const char *scale = (const char *)a.scale + (int64_t)tile.expert * tables * N * zsize;
-  // part p takes stages p * span .. of K; the cut lies between groups
-  const int span = WK == 1 ? t.stages : ((t.stages + WK - 1) / WK + t.close - 1) / t.close * t.close;
+  // the workgroup's stages of K, and set p's: p * span .. of them; cuts lie between groups
+  const int groups = (t.stages + t.close - 1) / t.close;
+  const int begin = groups * unit.part / unit.parts * t.close;
+  const int end = min(groups * (unit.part + 1) / unit.parts * t.close, t.stages);
+  const int span = WK == 1 ? end - begin : ((end - begin + WK - 1) / WK + t.close - 1) / t.close * t.close;
   auto stage_of = [&](int p, int s) -> int {           // (past the end: the last once more, not multiplied)
-    const int st = p * span + s;
-    return st < t.stages ? st : t.stages - 1;
+    const int st = begin + p * span + s;
+    return st < end ? st : end - 1;
   };
 
   // sources of this lane's loads.  The 16-byte chunks of a row of activations lie turned by the row's number, those of
@@ -461,11 +494,11 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
   fetch(f0, 0);
   int slot = 0, table = 0, fresh_table = NS;
   auto stage = [&](int s, bool fresh, bool last) __attribute__((always_inline)) {
-    const bool live = WK == 1 || part * span + s < t.stages;
+    const bool live = WK == 1 || begin + part * span + s < end;
     const int by = slot + 1 == NS ? -(NS - 1) * T::DATA : T::DATA;
     move_on(0, by);
     if (EARLY) fetch(f1, 1);
-    const bool ends = !HALF && live && (last || part * span + s + 1 == t.stages);
+    const bool ends = !HALF && live && (last || begin + part * span + s + 1 == end);
     if (live) {
       multiply(f0, HALF || fresh);
       if constexpr (HALF) {
@@ -534,6 +567,18 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
           }
   }
 
+  if (unit.parts > 1) {
+    f32x4 *to = reinterpret_cast<f32x4 *>(t.parts) + (int64_t)unit.slot * (T::BM * T::BN / 4) + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < RB; ++i)
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          to[((i * 2 + c) * 4 + j) * (T::SET * 64)] =
+              f32x4{out[i][c][4 * j], out[i][c][4 * j + 1], out[i][c][4 * j + 2], out[i][c][4 * j + 3]};
+    return;
+  }
   const int64_t n = n0 + wn * 64 + mycol;
 #pragma unroll
   for (int i = 0; i < RB; ++i)
@@ -547,15 +592,56 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
     }
 }
 
+// The tiles that were cut, added up part by part; blockIdx.y takes a block of 32 rows of each wavefront's.
+template <int XT, int RBW, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void tile_join_kernel(TileArgs t, uint32_t slots) {
+  constexpr int BM = 16 * RBW * WM, BN = 64 * WN;
+  const ExpertArgs &a = t.a;
+  const uint32_t cols = (uint32_t)((a.C + BN - 1) / BN);
+  Tiles tiles(a.offsets, a.E, (int)a.P, BM);
+  const Split s = split_items(tiles.total * cols, slots, t.most);
+  if (s.parts < 2 || blockIdx.x >= s.rem) return;
+  const Item tile = tiles.at<4>(s.full + blockIdx.x, cols);
+  if (tile.rows <= 0 || tile.expert == a.E) return;
+  const int lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5, wave = threadIdx.x >> 6, i = blockIdx.y;
+  const int m0 = wave / WN * 16 * RBW + 32 * i + 4 * hi;
+  const int64_t n = (int64_t)tile.col * BN + wave % WN * 64 + 4 * (l32 & 15) + 2 * (l32 >> 4);
+  const bool f32 = a.out_dtype == GPTQ_HIP_F32;
+  if (n >= a.C) return;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    f32x4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    for (int p = 0; p < s.parts; ++p) {
+      const f32x4 *from = reinterpret_cast<const f32x4 *>(t.parts) +
+                          ((int64_t)p * s.rem + blockIdx.x) * (BM * BN / 4) + threadIdx.x;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) v[c] += from[((i * 2 + c) * 4 + j) * (64 * WM * WN)];
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int m = m0 + 8 * j + r;
+      if (m >= tile.rows) continue;
+      const int64_t at = (int64_t)(tile.row0 + m) * a.C + n;
+      if (n + 1 < a.C) store2<XT>(a.out, f32, at, v[0][r], v[1][r]);
+      else store_out<XT>(a.out, f32, at, v[0][r]);
+    }
+  }
+}
+
 template <int XT, int BITS, int ZL, bool HALF, int RBW, int WM, int WN, int WK>
 static int tile_one(hipStream_t s, const TileArgs &t) {
   using T = TileShape<XT, BITS, ZL, HALF, RBW, WM, WN, WK>;
   const void *kernel = (const void *)tile_kernel<XT, BITS, ZL, HALF, RBW, WM, WN, WK>;
-  const unsigned blocks = item_grid(t.a.P, t.a.E, T::BM, ceil_div64(t.a.C, T::BN), T::THREADS);
+  const int64_t cols = ceil_div64(t.a.C, T::BN), parts = unit_bound(t.a.P, t.a.E, T::BM, cols, T::SLOTS, t.most);
+  const unsigned blocks = item_grid(t.a.P, t.a.E, T::BM, cols, T::THREADS, parts);
   if (!blocks) return GPTQ_HIP_EINVAL;
   if (!gptq_raise_lds_limit(kernel, T::LDS)) return GPTQ_HIP_ELAUNCH;
   tile_kernel<XT, BITS, ZL, HALF, RBW, WM, WN, WK><<<blocks, T::THREADS, T::LDS, s>>>(t);
   GPTQ_CHECK_LAUNCH();
+  if (parts) {
+    tile_join_kernel<XT, RBW, WM, WN><<<dim3((unsigned)(parts / 2), RBW / 2), 64 * T::SET, 0, s>>>(t, T::SLOTS);
+    GPTQ_CHECK_LAUNCH();
+  }
   return GPTQ_HIP_OK;
 }
 template <int XT, int BITS, int RBW, int WM, int WN, int WK>
@@ -578,13 +664,10 @@ template <int XT, int BITS> static int tile_shape(hipStream_t s, const TileArgs 
   return tile_tables<XT, BITS, 4, 1, 4, 1>(s, t, half, zl);
 }
 
-// groups that are no multiple of a stage are closed after every k-step
-static inline bool tile_half(int64_t group) { return group % 64 != 0; }
-
 template <int XT> static int tile_launch(hipStream_t s, const ExpertArgs &a, int shape, void *ws) {
   const int64_t K = a.bits == 4 ? 2 * a.R : a.R;
   const bool half = tile_half(a.group);
-  const Staged l = staged_layout(a.T, K, a.x_dtype, half);
+  const Staged l = staged_layout(a.T, a.P, K, a.C, a.group, a.E, a.x_dtype, shape);
   const int group = a.group ? (int)a.group : TILE_LONG;
   char *rows = (char *)ws;
   u32x4 *sums = (u32x4 *)((char *)ws + l.sums_at);
@@ -595,8 +678,8 @@ template <int XT> static int tile_launch(hipStream_t s, const ExpertArgs &a, int
     stage_rows_kernel<XT, false><<<(unsigned)a.T, 256, l.per_row * 4, s>>>(a.x, K, l.Kp, l.per_row, l.row_bytes, half,
                                                                            group, rows, sums);
   GPTQ_CHECK_LAUNCH();
-  const TileArgs t = {a, rows, sums, l.row_bytes, l.Kp, l.per_row, (int)(l.Kp / TILE_BK), half ? 1 : group / 64,
-                      a.group != 0};
+  const TileArgs t = {a, rows, sums, l.row_bytes, l.Kp, l.per_row, (int)(l.Kp / TILE_BK), tile_close(a.group),
+                      a.group != 0, l.most, (float *)((char *)ws + l.parts_at)};
   const bool aligned = a.C % 16 == 0 && (uintptr_t)a.packed % 16 == 0 && (uintptr_t)a.zero % 16 == 0 &&
                        (uintptr_t)a.scale % 16 == 0;
   const int zl = !aligned ? 0 : (a.zs_dtype == GPTQ_HIP_F32 ? 4 : 2);
