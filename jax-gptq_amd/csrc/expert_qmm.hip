@@ -144,17 +144,20 @@ struct Choice {
 //   64 experts 2048 x 1424:  4 rows 37 43 43 52 61,  16: 52 52 44 55 64,   48: 145 79 70 62 73,     128: - 170 143 117 137
 //   8 experts 11008 x 4096:  4 rows 45 76 125 152 112,  24: 87 97 126 153 117,  48: 133 107 130 155 119,
 //                            96: - 184 164 158 132,  128: - 228 259 201 225
+// fp32 rows are three operands, for which 64 rows are too many (32 x 128 in halves of K / 32 x 256 / 64 x 256):
+//   8 experts 4096 x 4096:  30 rows 80 86 302,  80: 123 121 306,  162: 208 190 387,  512: 583 500 1012
 static Choice choose(int64_t P, int E, int64_t C, int64_t group, int x_dtype, int transpose) {
   if ((group && group % 32) || C < 16) return {Choice::SIMPLE, 0};
   if (transpose) return {Choice::BACK, 0};
   const int64_t rows = P / E;
   if ((P < E ? P : E) * ceil_div64(C, 256) >= 256) {
     if (rows <= 8 && C >= 128) return {Choice::STRIP, 0};
-    return {Choice::TILE, rows <= 24 ? TILE_32x256 : TILE_64x256};
+    return {Choice::TILE, rows <= 24 || x_dtype == GPTQ_HIP_F32 ? TILE_32x256 : TILE_64x256};
   }
   if (rows <= 24 && C >= 128) return {Choice::STRIP, 0};
+  if (x_dtype == GPTQ_HIP_F32) return {Choice::TILE, rows <= 80 ? TILE_32x128_K2 : TILE_32x256};
   if (rows <= 48) return {Choice::TILE, TILE_32x128_K2};
-  return {Choice::TILE, rows <= 96 && x_dtype != GPTQ_HIP_F32 ? TILE_64x256_K2 : TILE_64x256};
+  return {Choice::TILE, rows <= 96 ? TILE_64x256_K2 : TILE_64x256};
 }
 
 // GPTQ_HIP_OK, or why the product is refused

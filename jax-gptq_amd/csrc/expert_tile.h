@@ -18,9 +18,6 @@
 #pragma once
 #include "expert_common.h"
 #include <math.h>
-#ifndef PAYS
-#define PAYS 0.3
-#endif
 
 namespace xqmm {
 
@@ -78,8 +75,8 @@ static inline Staged staged_layout(int64_t x_rows, int64_t P, int64_t K, int64_t
   // Whether to cut at all is settled here, by the tiles that P rows come to when their experts are drawn at random: the
   // second kernel costs 2 to 4 us also where it finds nothing to add up.
   const double busy = E * (1.0 - exp(-(double)P / E)), items = ((double)P / BM + busy / 2) * ceil_div64(N, BN);
-  const int slots = shape == TILE_64x256_K2 || x_dtype == GPTQ_HIP_F32 ? TILE_SLOTS / 2 : TILE_SLOTS;
-  const bool pays = items - slots * floor(items / slots) <= PAYS * slots;
+  const int slots = shape == TILE_64x256_K2 ? TILE_SLOTS / 2 : TILE_SLOTS;
+  const bool pays = items - slots * floor(items / slots) <= 0.3 * slots;
   l.most = (int)(most < 1 || !pays ? 1 : (most < TILE_MOST ? most : TILE_MOST));
   l.bytes = l.parts_at + (size_t)unit_bound(P, E, BM, ceil_div64(N, BN), TILE_SLOTS, l.most) * BM * BN * 4;
   return l;
@@ -658,10 +655,12 @@ static int tile_tables(hipStream_t s, const TileArgs &t, bool half, int zl) {
 template <int XT, int BITS> static int tile_shape(hipStream_t s, const TileArgs &t, int shape, bool half, int zl) {
   if (shape == TILE_32x128_K2) return tile_tables<XT, BITS, 2, 1, 2, 2>(s, t, half, zl);
   if (shape == TILE_32x256) return tile_tables<XT, BITS, 2, 1, 4, 1>(s, t, half, zl);
-  if constexpr (XT != GPTQ_HIP_F32) {                   // (three parts of 64 rows and both halves do not fit LDS)
+  if constexpr (XT == GPTQ_HIP_F32) {                   // (three operands of 64 rows fill the registers and LDS)
+    return GPTQ_HIP_EINVAL;
+  } else {
     if (shape == TILE_64x256_K2) return tile_tables<XT, BITS, 4, 1, 4, 2>(s, t, half, zl);
+    return tile_tables<XT, BITS, 4, 1, 4, 1>(s, t, half, zl);
   }
-  return tile_tables<XT, BITS, 4, 1, 4, 1>(s, t, half, zl);
 }
 
 template <int XT> static int tile_launch(hipStream_t s, const ExpertArgs &a, int shape, void *ws) {
