@@ -20,7 +20,7 @@ int expert_strip_f16(hipStream_t s, const ExpertArgs &a);
 int expert_strip_bf16(hipStream_t s, const ExpertArgs &a);
 int expert_strip_f32(hipStream_t s, const ExpertArgs &a);
 // the same by tiles (expert_tile.h) of these rows x channels; K2: K in two halves, side by side
-enum { TILE_32x128_K2, TILE_32x256, TILE_64x256, TILE_64x256_K2 };
+enum { TILE_32x256, TILE_64x256, TILE_64x256_K2 };
 int expert_tile_f16(hipStream_t s, const ExpertArgs &a, int shape, void *ws);
 int expert_tile_bf16(hipStream_t s, const ExpertArgs &a, int shape, void *ws);
 int expert_tile_f32(hipStream_t s, const ExpertArgs &a, int shape, void *ws);

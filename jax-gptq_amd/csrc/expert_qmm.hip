@@ -137,27 +137,24 @@ struct Choice {
   int shape;                // TILE_*
 };
 // By the rows of an expert, on average, and by whether tiles of 256 channels, one row of them per expert, fill the 256
-// CUs.  Each kernel costs the same for 1 row as for all that its tile holds, so a wider tile pays once the rows fill
-// half of it or so; where columns are few, strips of 128 channels and halves of K bring more workgroups.  Measured, us a
-// call (strip / 32 x 128 in halves of K / 32 x 256 / 64 x 256 / 64 x 256 in halves of K):
-//   8 experts 4096 x 11008:  4 rows 55 66 67 83 93,  16: 76 73 68 84 94,  48: 161 113 108 92 105,  128: - 237 206 172 197
-//   64 experts 2048 x 1424:  4 rows 37 43 43 52 61,  16: 52 52 44 55 64,   48: 145 79 70 62 73,     128: - 170 143 117 137
-//   8 experts 11008 x 4096:  4 rows 45 76 125 152 112,  24: 87 97 126 153 117,  48: 133 107 130 155 119,
-//                            96: - 184 164 158 132,  128: - 228 259 201 225
-// fp32 rows are three operands, for which 64 rows are too many (32 x 128 in halves of K / 32 x 256 / 64 x 256):
-//   8 experts 4096 x 4096:  30 rows 80 86 302,  80: 123 121 306,  162: 208 190 387,  512: 583 500 1012
+// CUs (`wide`).  Each kernel costs nearly the same for 1 row as for all that its tile holds, so a taller tile pays once the
+// rows fill half of it or so; where there are few columns of tiles, strips last longer, and two halves of K in a workgroup
+// beat parts in two.  Measured, us a call (strip / 32 x 256 / 64 x 256 / 64 x 256 in halves of K):
+//   8 experts 4096 x 11008 (wide):  8 rows each 40 61 76 86,  15: 47 61 77 -,  20: 70 62 76 -,  37: - 90 78 91,
+//                                   80: - 127 129 138,  162: - 222 179 209
+//   64 experts 2048 x 1424 (wide):  5 rows each 27 41 50 58,  15: 36 40 49 -,  31: - 54 52 62,  64: - 75 74 91
+//   8 experts 11008 x 4096:  8 rows each 41 58 73 71,  15: 48 58 74 -,  25: 72 69 76 75,  37: - 93 79 111,  50: - 117 80 113,
+//                            80: - 153 134 124,  125: - 179 194 167,  162: - 234 203 225
+// fp32 rows are three operands, for which 64 rows are too many (strip / 32 x 256 / 64 x 256):
+//   8 experts 4096 x 4096:  8 rows each 32 51 285,  20: 57 51 301,  40: 81 77 306,  162: - 187 387,  512: - 483 1012
 static Choice choose(int64_t P, int E, int64_t C, int64_t group, int x_dtype, int transpose) {
   if ((group && group % 32) || C < 16) return {Choice::SIMPLE, 0};
   if (transpose) return {Choice::BACK, 0};
   const int64_t rows = P / E;
-  if ((P < E ? P : E) * ceil_div64(C, 256) >= 256) {
-    if (rows <= 8 && C >= 128) return {Choice::STRIP, 0};
-    return {Choice::TILE, rows <= 24 || x_dtype == GPTQ_HIP_F32 ? TILE_32x256 : TILE_64x256};
-  }
-  if (rows <= 24 && C >= 128) return {Choice::STRIP, 0};
-  if (x_dtype == GPTQ_HIP_F32) return {Choice::TILE, rows <= 80 ? TILE_32x128_K2 : TILE_32x256};
-  if (rows <= 48) return {Choice::TILE, TILE_32x128_K2};
-  return {Choice::TILE, rows <= 96 ? TILE_64x256_K2 : TILE_64x256};
+  const bool wide = (P < E ? P : E) * ceil_div64(C, 256) >= 256, fp32 = x_dtype == GPTQ_HIP_F32;
+  if (C >= 128 && rows <= (wide || fp32 ? 15 : 24)) return {Choice::STRIP, 0};
+  if (fp32 || rows <= (wide ? 31 : 24)) return {Choice::TILE, TILE_32x256};
+  return {Choice::TILE, !wide && rows > 56 && rows <= 128 ? TILE_64x256_K2 : TILE_64x256};
 }
 
 // GPTQ_HIP_OK, or why the product is refused

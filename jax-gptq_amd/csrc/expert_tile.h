@@ -1,5 +1,6 @@
-// Many rows per expert: a workgroup computes a tile of one expert's outputs, K in stages of 64: 128 or 64 rows x 256
-// channels, or 64 or 32 rows x 128 channels with K in two halves, which fill the chip where the tiles are few.
+// Many rows per expert: a workgroup computes a tile of one expert's outputs, 32 or 64 rows x 256 channels, K in stages
+// of 64.  Where the tiles are few, K is cut: in two halves side by side in a workgroup of twice the wavefronts, or in
+// parts of their own, which a second kernel adds up.
 //
 //   y[p, n] = sum_G s[G, n] (sum_{k in G} x[p, k] (o + c[k, n]) - (o + z[G, n]) sum_{k in G} x[p, k])
 //
@@ -45,8 +46,8 @@ template <int VM> __device__ __forceinline__ void wait_and_meet() {
 
 // parts of a contraction at most, stages of one at least, workgroups that run at a time at most
 constexpr int TILE_MOST = 4, TILE_MIN_STAGES = 8, TILE_SLOTS = 512;
-static inline int tile_rows(int shape) { return shape == TILE_32x128_K2 || shape == TILE_32x256 ? 32 : 64; }
-static inline int tile_cols(int shape) { return shape == TILE_32x128_K2 ? 128 : 256; }
+constexpr int TILE_BN = 256;
+static inline int tile_rows(int shape) { return shape == TILE_32x256 ? 32 : 64; }
 // groups that are no multiple of a stage are closed after every k-step
 static inline bool tile_half(int64_t group) { return group % 64 != 0; }
 // stages of a group, or of a piece of a sum without groups
@@ -71,12 +72,12 @@ static inline Staged staged_layout(int64_t x_rows, int64_t P, int64_t K, int64_t
   l.parts_at = (size_t)round_up64(l.sums_at + (x_rows * l.per_row) * 16, 256);
   const int64_t stages = l.Kp / TILE_BK, groups = ceil_div64(stages, tile_close(group));
   const int64_t most = groups < stages / TILE_MIN_STAGES ? groups : stages / TILE_MIN_STAGES;
-  const int BM = tile_rows(shape), BN = tile_cols(shape);
+  const int BM = tile_rows(shape), BN = TILE_BN;
   // Whether to cut at all is settled here, by the tiles that P rows come to when their experts are drawn at random: the
   // second kernel costs 2 to 4 us also where it finds nothing to add up.
   const double busy = E * (1.0 - exp(-(double)P / E)), items = ((double)P / BM + busy / 2) * ceil_div64(N, BN);
   const int slots = shape == TILE_64x256_K2 ? TILE_SLOTS / 2 : TILE_SLOTS;
-  const bool pays = items - slots * floor(items / slots) <= 0.3 * slots;
+  const bool pays = items - slots * floor(items / slots) <= 0.5 * slots;
   l.most = (int)(most < 1 || !pays ? 1 : (most < TILE_MOST ? most : TILE_MOST));
   l.bytes = l.parts_at + (size_t)unit_bound(P, E, BM, ceil_div64(N, BN), TILE_SLOTS, l.most) * BM * BN * 4;
   return l;
@@ -192,14 +193,14 @@ struct TileArgs {
 
 // ZL: how tables lie in LDS: 4 or 2 bytes an element as they are in memory, 0: operands that start or end anywhere,
 // whose codes and tables pass through registers (tables converted to fp32).
-// A wavefront owns 16 RBW rows x 64 channels; WM x WN wavefronts cover the tile, WK such sets take a part of K each.
-template <int XT, int BITS, int ZL, bool HALF, int RBW, int WM, int WN, int WK> struct TileShape {
-  static constexpr int SET = WM * WN, WAVES = SET * WK, THREADS = 64 * WAVES, BM = 16 * RBW * WM, BN = 64 * WN;
+// A wavefront owns 16 RBW rows x 64 channels; four cover the tile, WK such sets take a part of K each.
+template <int XT, int BITS, int ZL, bool HALF, int RBW, int WK> struct TileShape {
+  static constexpr int SET = 4, WAVES = SET * WK, THREADS = 64 * WAVES, BM = 16 * RBW, BN = TILE_BN;
   static constexpr int PARTS = Op<XT>::PARTS;
   static constexpr int BROWS = BITS == 4 ? 32 : 64;       // packed rows of a part's stage
-  static constexpr int HN = HALF ? 2 : 1, MB = (BM + 63) / 64;
+  static constexpr int HN = HALF ? 2 : 1;
   // one part's rows, codes, zeros and scales (of a group), sums; then all parts'
-  static constexpr int AP = PARTS * BM * 128, BP = BROWS * BN, ZP = 2 * BN * 4, SP = MB * 1024;
+  static constexpr int AP = PARTS * BM * 128, BP = BROWS * BN, ZP = 2 * BN * 4, SP = 1024;
   static constexpr int A = WK * AP, B = WK * BP, Z = WK * HN * ZP, S = WK * HN * SP;
   // a stage's rows and codes, and its tables, in rings of their own: rows and codes are in registers half a stage before
   // the tables are needed, so their place is free one stage earlier
@@ -212,16 +213,16 @@ template <int XT, int BITS, int ZL, bool HALF, int RBW, int WM, int WN, int WK> 
   static constexpr int SLOTS = WAVES == 4 && LDS <= 80 * 1024 ? TILE_SLOTS : TILE_SLOTS / 2;   // that run at a time
   // loads of a wavefront per stage
   static constexpr int AI = A / 1024 / WAVES, BI = B / 1024 / WAVES;
-  static constexpr int SI = WK * HN * MB, TI = WK * HN * (BN / 128), ITEMS = SI + TI;
+  static constexpr int SI = WK * HN, TI = WK * HN * (BN / 128), ITEMS = SI + TI;
   static constexpr int MI = (ITEMS + WAVES - 1) / WAVES;
   static constexpr int LOADS = AI + BI + MI;
   static_assert(A % (1024 * WAVES) == 0 && B % (1024 * WAVES) == 0 && LDS <= 160 * 1024, "whole loads");
   static_assert(RBW % 2 == 0 && (WK == 1 || (WK - 1) * SET * RBW * 4 * 1024 <= LDS), "partial tiles fit");
 };
 
-template <int XT, int BITS, int ZL, bool HALF, int RBW, int WM, int WN, int WK>
-__global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) {
-  using T = TileShape<XT, BITS, ZL, HALF, RBW, WM, WN, WK>;
+template <int XT, int BITS, int ZL, bool HALF, int RBW, int WK>
+__global__ __launch_bounds__(256 * WK, 2) void tile_kernel(TileArgs t) {
+  using T = TileShape<XT, BITS, ZL, HALF, RBW, WK>;
   using C = Codes<XT, BITS>;
   using O = Op<XT>;
   typedef __attribute__((address_space(3))) char lds_char;
@@ -229,7 +230,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
   const ExpertArgs &a = t.a;
   const int lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int part = wave / T::SET, wm = wave / WN % WM, wn = wave % WN;
+  const int part = wave / T::SET, wn = wave % T::SET;
   const int64_t N = a.C;
   const bool f32 = a.out_dtype == GPTQ_HIP_F32;
 
@@ -279,7 +280,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
   for (int j = 0; j < T::MI; ++j) {
     const int it = (wave + T::WAVES * j) % T::ITEMS;
     srow[j] = t.sums;
-    if (it < T::SI) srow[j] = t.sums + row_base(64 * (it % T::MB) + lane) * t.per_row;
+    if (it < T::SI) srow[j] = t.sums + row_base(lane) * t.per_row;
   }
   auto table_row = [&](int st, int h) -> int64_t {
     if (!t.grouped) return 0;
@@ -301,15 +302,14 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
 #pragma unroll
   for (int j = 0; j < T::BI; ++j) {
     const int at = (wave * T::BI + j) % (T::BP / 1024) * (64 / CH) + lane / CH, g = reader(at);
-    brow[j] = T::BN == 128 ? at ^ (g >> 1) : at;
-    bcol[j] = 16 * ((lane % CH) ^ (T::BN == 128 ? 4 * (g & 1) : 4 * g));
+    brow[j] = at;
+    bcol[j] = 16 * ((lane % CH) ^ (4 * g));
     const int64_t n = n0 + bcol[j] < N ? n0 + bcol[j] : 0, left = a.R - (int64_t)(t.stages - 1) * T::BROWS;
     boff[j] = (uint32_t)(brow[j] * N + n);
     bend[j] = (uint32_t)((brow[j] < left ? brow[j] : left - 1) * N + n);
   }
-  // and its channels in a row of the tables: zeros, then scales, 1 KB each at 256 channels, half a load each at 128
-  const int tl = T::BN == 128 ? lane & 31 : lane;
-  const int64_t tn = n0 + (ZB == 4 ? 4 * tl : 8 * (tl % (T::BN / 8)));
+  // and its channels in a row of the tables: zeros, then scales, 1 KB each
+  const int64_t tn = n0 + (ZB == 4 ? 4 * lane : 8 * (lane % (T::BN / 8)));
   const uint32_t toff = (uint32_t)((tn < N ? tn : 0) * ZB);
 
   auto issue = [&](int s, int slot, int table) __attribute__((always_inline)) {
@@ -334,13 +334,12 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
     for (int j = 0; j < T::MI; ++j) {
       const int it = (wave + T::WAVES * j) % T::ITEMS;   // (more wavefronts than items: the same bytes twice)
       if (it < T::SI) {
-        const int q = it / T::MB, h = q % T::HN, st = stage_of(q / T::HN, s);
+        const int h = it % T::HN, st = stage_of(it / T::HN, s);
         to_lds_16(srow[j] + (HALF ? 2 * st + h : st), tbase + T::Z + it * 1024);
       } else if constexpr (ZL != 0) {
         const int i = it - T::SI, q = i / (T::BN / 128);
         const int64_t row = table_row(stage_of(q / T::HN, s), q % T::HN) * N * ZB;
-        if (T::BN == 128) to_lds_16((lane >> 5 ? scale : zero) + row + toff, tbase + i * 1024);
-        else to_lds_16((i & 1 ? scale : zero) + row, toff, tbase + i * 1024);
+        to_lds_16((i & 1 ? scale : zero) + row, toff, tbase + i * 1024);
       }
     }
     if constexpr (!ZL) {
@@ -408,7 +407,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
 #pragma unroll
     for (int i = 0; i < RB; ++i) {
       const u32x4 sum = *reinterpret_cast<const u32x4 *>(base + T::Z + (part * T::HN + h) * T::SP +
-                                                         (wm * 16 * RBW + 32 * i + l32) * 16);
+                                                         (32 * i + l32) * 16);
 #pragma unroll
       for (int c = 0; c < 2; ++c) acc[i][c] = Op<GPTQ_HIP_BF16>::mma32(sum, f[c], acc[i][c]);
     }
@@ -434,17 +433,17 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
   for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
-      const int g = 2 * v + hi, chunk = (wn * 4 + ((l32 & 15) >> 2)) ^ (T::BN == 128 ? 4 * (g & 1) : 4 * g);
-      xat[ks][v] = part * T::AP + (wm * 16 * RBW + l32) * 128 + (((4 * ks + g) ^ (l32 & 7)) * 16);
+      const int g = 2 * v + hi, chunk = (wn * 4 + ((l32 & 15) >> 2)) ^ (4 * g);
+      xat[ks][v] = part * T::AP + (l32) * 128 + (((4 * ks + g) ^ (l32 & 7)) * 16);
       rat[ks][v] = T::A + part * T::BP + C::ROWS * g * T::BN + chunk * 16 + (l32 & 3) * 4;
     }
   auto fetch = [&](Step &f, int ks) __attribute__((always_inline)) {
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
 #pragma unroll
-      for (int i = 0; i < C::ROWS; ++i)                 // (g >> 1 is v: at 128 channels odd and even rows change places)
-        f.r[v][i] = *reinterpret_cast<const uint32_t *>(
-            lds + rat[ks][v] + ((BITS == 4 ? 16 : 32) * ks + (T::BN == 128 ? i ^ v : i)) * T::BN);
+      for (int i = 0; i < C::ROWS; ++i)
+        f.r[v][i] =
+            *reinterpret_cast<const uint32_t *>(lds + rat[ks][v] + ((BITS == 4 ? 16 : 32) * ks + i) * T::BN);
 #pragma unroll
       for (int i = 0; i < RB; ++i)
 #pragma unroll
@@ -581,7 +580,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
   for (int i = 0; i < RB; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const int m = wm * 16 * RBW + 32 * i + 8 * (r / 4) + 4 * hi + r % 4;
+      const int m = 32 * i + 8 * (r / 4) + 4 * hi + r % 4;
       if (m >= tile.rows || n >= N) continue;
       const int64_t at = (int64_t)(tile.row0 + m) * N + n;
       if (n + 1 < N) store2<XT>(a.out, f32, at, out[i][0][r], out[i][1][r]);
@@ -590,9 +589,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void tile_kernel(TileArgs t) 
 }
 
 // The tiles that were cut, added up part by part; blockIdx.y takes a block of 32 rows of each wavefront's.
-template <int XT, int RBW, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void tile_join_kernel(TileArgs t, uint32_t slots) {
-  constexpr int BM = 16 * RBW * WM, BN = 64 * WN;
+template <int XT, int RBW> __global__ __launch_bounds__(256) void tile_join_kernel(TileArgs t, uint32_t slots) {
+  constexpr int BM = 16 * RBW, BN = TILE_BN;
   const ExpertArgs &a = t.a;
   const uint32_t cols = (uint32_t)((a.C + BN - 1) / BN);
   Tiles tiles(a.offsets, a.E, (int)a.P, BM);
@@ -601,8 +599,8 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_join_kernel(TileArgs t, uin
   const Item tile = tiles.at<4>(s.full + blockIdx.x, cols);
   if (tile.rows <= 0 || tile.expert == a.E) return;
   const int lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5, wave = threadIdx.x >> 6, i = blockIdx.y;
-  const int m0 = wave / WN * 16 * RBW + 32 * i + 4 * hi;
-  const int64_t n = (int64_t)tile.col * BN + wave % WN * 64 + 4 * (l32 & 15) + 2 * (l32 >> 4);
+  const int m0 = 32 * i + 4 * hi;
+  const int64_t n = (int64_t)tile.col * BN + wave * 64 + 4 * (l32 & 15) + 2 * (l32 >> 4);
   const bool f32 = a.out_dtype == GPTQ_HIP_F32;
   if (n >= a.C) return;
 #pragma unroll
@@ -612,7 +610,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_join_kernel(TileArgs t, uin
       const f32x4 *from = reinterpret_cast<const f32x4 *>(t.parts) +
                           ((int64_t)p * s.rem + blockIdx.x) * (BM * BN / 4) + threadIdx.x;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) v[c] += from[((i * 2 + c) * 4 + j) * (64 * WM * WN)];
+      for (int c = 0; c < 2; ++c) v[c] += from[((i * 2 + c) * 4 + j) * 256];
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -625,41 +623,40 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_join_kernel(TileArgs t, uin
   }
 }
 
-template <int XT, int BITS, int ZL, bool HALF, int RBW, int WM, int WN, int WK>
+template <int XT, int BITS, int ZL, bool HALF, int RBW, int WK>
 static int tile_one(hipStream_t s, const TileArgs &t) {
-  using T = TileShape<XT, BITS, ZL, HALF, RBW, WM, WN, WK>;
-  const void *kernel = (const void *)tile_kernel<XT, BITS, ZL, HALF, RBW, WM, WN, WK>;
+  using T = TileShape<XT, BITS, ZL, HALF, RBW, WK>;
+  const void *kernel = (const void *)tile_kernel<XT, BITS, ZL, HALF, RBW, WK>;
   const int64_t cols = ceil_div64(t.a.C, T::BN), parts = unit_bound(t.a.P, t.a.E, T::BM, cols, T::SLOTS, t.most);
   const unsigned blocks = item_grid(t.a.P, t.a.E, T::BM, cols, T::THREADS, parts);
   if (!blocks) return GPTQ_HIP_EINVAL;
   if (!gptq_raise_lds_limit(kernel, T::LDS)) return GPTQ_HIP_ELAUNCH;
-  tile_kernel<XT, BITS, ZL, HALF, RBW, WM, WN, WK><<<blocks, T::THREADS, T::LDS, s>>>(t);
+  tile_kernel<XT, BITS, ZL, HALF, RBW, WK><<<blocks, T::THREADS, T::LDS, s>>>(t);
   GPTQ_CHECK_LAUNCH();
   if (parts) {
-    tile_join_kernel<XT, RBW, WM, WN><<<dim3((unsigned)(parts / 2), RBW / 2), 64 * T::SET, 0, s>>>(t, T::SLOTS);
+    tile_join_kernel<XT, RBW><<<dim3((unsigned)(parts / 2), RBW / 2), 256, 0, s>>>(t, T::SLOTS);
     GPTQ_CHECK_LAUNCH();
   }
   return GPTQ_HIP_OK;
 }
-template <int XT, int BITS, int RBW, int WM, int WN, int WK>
+template <int XT, int BITS, int RBW, int WK>
 static int tile_tables(hipStream_t s, const TileArgs &t, bool half, int zl) {
   if (half) {
-    if (zl == 4) return tile_one<XT, BITS, 4, true, RBW, WM, WN, WK>(s, t);
-    if (zl == 2) return tile_one<XT, BITS, 2, true, RBW, WM, WN, WK>(s, t);
-    return tile_one<XT, BITS, 0, true, RBW, WM, WN, WK>(s, t);
+    if (zl == 4) return tile_one<XT, BITS, 4, true, RBW, WK>(s, t);
+    if (zl == 2) return tile_one<XT, BITS, 2, true, RBW, WK>(s, t);
+    return tile_one<XT, BITS, 0, true, RBW, WK>(s, t);
   }
-  if (zl == 4) return tile_one<XT, BITS, 4, false, RBW, WM, WN, WK>(s, t);
-  if (zl == 2) return tile_one<XT, BITS, 2, false, RBW, WM, WN, WK>(s, t);
-  return tile_one<XT, BITS, 0, false, RBW, WM, WN, WK>(s, t);
+  if (zl == 4) return tile_one<XT, BITS, 4, false, RBW, WK>(s, t);
+  if (zl == 2) return tile_one<XT, BITS, 2, false, RBW, WK>(s, t);
+  return tile_one<XT, BITS, 0, false, RBW, WK>(s, t);
 }
 template <int XT, int BITS> static int tile_shape(hipStream_t s, const TileArgs &t, int shape, bool half, int zl) {
-  if (shape == TILE_32x128_K2) return tile_tables<XT, BITS, 2, 1, 2, 2>(s, t, half, zl);
-  if (shape == TILE_32x256) return tile_tables<XT, BITS, 2, 1, 4, 1>(s, t, half, zl);
+  if (shape == TILE_32x256) return tile_tables<XT, BITS, 2, 1>(s, t, half, zl);
   if constexpr (XT == GPTQ_HIP_F32) {                   // (three operands of 64 rows fill the registers and LDS)
     return GPTQ_HIP_EINVAL;
   } else {
-    if (shape == TILE_64x256_K2) return tile_tables<XT, BITS, 4, 1, 4, 2>(s, t, half, zl);
-    return tile_tables<XT, BITS, 4, 1, 4, 1>(s, t, half, zl);
+    if (shape == TILE_64x256_K2) return tile_tables<XT, BITS, 4, 2>(s, t, half, zl);
+    return tile_tables<XT, BITS, 4, 1>(s, t, half, zl);
   }
 }
 
