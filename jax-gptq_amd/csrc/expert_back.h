@@ -381,8 +381,8 @@ __global__ __launch_bounds__(128 * WM, XT == GPTQ_HIP_F32 ? 1 : 2) void back_ker
       }
 }
 
-// The tiles that were cut, added up part by part: blockIdx.y takes a block of 32 rows of each wavefront's, and
-// one of its pairs of columns' blocks.
+// The tiles that were cut, added up part by part: blockIdx.y takes a quarter of a block of 32 rows of each wavefront's,
+// and one of its pairs of columns' blocks.
 template <int XT, int BITS, int WM, int RB> __global__ __launch_bounds__(128 * WM) void back_join_kernel(BackArgs t) {
   constexpr int CB = BITS == 4 ? 2 : 1, BM = 32 * RB * WM;
   const ExpertArgs &a = t.a;
@@ -392,32 +392,33 @@ template <int XT, int BITS, int WM, int RB> __global__ __launch_bounds__(128 * W
   const Split s = split_items(tiles.total * cols, t.slots, t.most);
   if (s.parts < 2 || blockIdx.x >= s.rem) return;
   const Item tile = tiles.at<4>(s.full + blockIdx.x, cols);
-  const int i = blockIdx.y >> 1, c0 = 2 * (blockIdx.y & 1);
+  const int i = blockIdx.y >> 3, c0 = blockIdx.y >> 1 & 2, j = blockIdx.y & 3;
   const int lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5, wave = threadIdx.x >> 6;
-  const int m0 = (wave >> 1) * 32 * RB + 32 * i + 4 * hi;
+  const int m0 = (wave >> 1) * 32 * RB + 32 * i + 8 * j + 4 * hi;
   if (tile.rows <= 0 || tile.expert == a.E) return;
   const bool f32 = a.out_dtype == GPTQ_HIP_F32;
+  const f32x4 *from = reinterpret_cast<const f32x4 *>(t.parts) + (int64_t)blockIdx.x * (BM * BACK_BN / 4) + threadIdx.x;
+  f32x4 w[BACK_MOST][2];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    f32x4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-    for (int p = 0; p < s.parts; ++p) {
-      const f32x4 *from = reinterpret_cast<const f32x4 *>(t.parts) +
-                          ((int64_t)p * s.rem + blockIdx.x) * (BM * BACK_BN / 4) + threadIdx.x;
+  for (int p = 0; p < BACK_MOST; ++p)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) v[c] += from[((i * 4 + c0 + c) * 4 + j) * 128 * WM];
-    }
+    for (int c = 0; c < 2; ++c)                        // (parts that there are not: the last once more, left out below)
+      w[p][c] = from[(int64_t)min(p, s.parts - 1) * s.rem * (BM * BACK_BN / 4) + ((i * 4 + c0 + c) * 4 + j) * 128 * WM];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int m = m0 + 8 * j + r;
-      if (m >= tile.rows) continue;
+  for (int p = 1; p < BACK_MOST; ++p)
 #pragma unroll
-      for (int b = 0; b < 2 / CB; ++b) {
-        const int64_t k = (int64_t)tile.col * BACK_BN + (wave & 1) * 128 + CB * (32 * (c0 / CB + b) + l32);
-        if (k >= K) continue;
-        const int64_t at = (int64_t)(tile.row0 + m) * K + k;
-        if constexpr (CB == 2) store2<XT>(a.out, f32, at, v[0][r], v[1][r]);
-        else store_out<XT>(a.out, f32, at, v[b][r]);
-      }
+    for (int c = 0; c < 2; ++c)
+      if (p < s.parts) w[0][c] += w[p][c];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    if (m0 + r >= tile.rows) continue;
+#pragma unroll
+    for (int b = 0; b < 2 / CB; ++b) {
+      const int64_t k = (int64_t)tile.col * BACK_BN + (wave & 1) * 128 + CB * (32 * (c0 / CB + b) + l32);
+      if (k >= K) continue;
+      const int64_t at = (int64_t)(tile.row0 + m0 + r) * K + k;
+      if constexpr (CB == 2) store2<XT>(a.out, f32, at, w[0][0][r], w[0][1][r]);
+      else store_out<XT>(a.out, f32, at, w[0][b][r]);
     }
   }
 }
@@ -432,7 +433,7 @@ template <int XT, int BITS, bool ALIGNED, int NG, int WM, int RB> static int bac
   back_kernel<XT, BITS, ALIGNED, NG, WM, RB><<<blocks, T::THREADS, T::LDS, s>>>(t);
   GPTQ_CHECK_LAUNCH();
   if (parts) {
-    back_join_kernel<XT, BITS, WM, RB><<<dim3((unsigned)(parts / 2), 2 * RB), T::THREADS, 0, s>>>(t);
+    back_join_kernel<XT, BITS, WM, RB><<<dim3((unsigned)(parts / 2), 8 * RB), T::THREADS, 0, s>>>(t);
     GPTQ_CHECK_LAUNCH();
   }
   return GPTQ_HIP_OK;
