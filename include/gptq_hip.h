@@ -350,11 +350,14 @@ int gptq_hip_expert_combine_grad(void *stream, const void *y, const void *g, int
  *   transpose_b = 0: out [rows, C] = x @ W[e];  transpose_b = 1: out [rows, K] = x @ W[e]^T.
  * order null: x holds the rows in sorted order (x_rows == rows); else row p is x[order[p] / top_k] and
  * rows == x_rows * top_k.  Rows of nowhere give zeros and are not read.  Codes enter the products exactly, sums and
- * scales are fp32, the result is rounded once to out_dtype (x_dtype or F32).  A row with an infinity or a NaN may be
- * NaN throughout; other rows are untouched by it.  rows < 2^24, K <= 262140, C <= 2^20.
+ * scales are fp32 (a group's sum of x times codes comes before its scale and has to stay in fp32's range), the result
+ * is rounded once to out_dtype (x_dtype or F32).  A row with an infinity or a NaN may be NaN throughout; other rows are
+ * untouched by it.  rows < 2^24, K <= 262140, C <= 2^20.  Equal calls give equal bits; the order of a row's sums
+ * depends on how many rows every expert has.
  * ws, 16-byte aligned: gptq_hip_expert_qmatmul_workspace_bytes (contents need no preparation; calls that overlap in
- * time need one each).  Plain kernels, an order of magnitude slower, take groups that are no multiple of 32, fewer
- * than 8 channels (transposed: 16) and, transposed, an x that is not 16-byte aligned. */
+ * time need one each).  The first call of a kind on a device raises kernels' limits of LDS: make one before capturing.
+ * Plain kernels, an order of magnitude slower, take groups that are no multiple of 32, fewer than 16 channels and,
+ * transposed, an x that is not 16-byte aligned. */
 size_t gptq_hip_expert_qmatmul_workspace_bytes(int64_t x_rows, int64_t rows, int64_t R, int64_t C, int bits,
                                                int64_t group_size, int n_experts, int x_dtype, int zs_dtype,
                                                int transpose_b);

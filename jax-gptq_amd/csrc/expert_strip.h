@@ -4,9 +4,13 @@
 //
 // Bound by the weights' bytes (every expert that any row picked is read once from HBM as long as its rows fit one
 // tile).  Each of the eight wavefronts takes every eighth unit of 32 KS input features and multiplies all rows of the
-// tile with the whole strip (sixteen wavefronts, for the calls that have few workgroups: a quarter slower): nothing is shared while K runs, so there is no barrier, and a wavefront has the next
-// units' loads (weights, tables, activations) in flight while it multiplies one.  A workgroup covers K by itself, so
-// no partial result leaves it: no workspace, no counter, no second launch.
+// tile with the whole strip (sixteen wavefronts, for the calls that have few workgroups, are a quarter slower): nothing
+// is shared while K runs, so there is no barrier, and a wavefront has the next units' loads (weights, tables,
+// activations) in flight while it multiplies one.  A workgroup covers K by itself, so no partial result leaves it: no
+// workspace, no counter, no second launch.
+// Measured: 1 token of 2 experts on 4096 x 11008, 4 bits, groups of 128, 14.4 us a call for 48 MB of codes and tables
+// (3.3 TB/s, of which the start and end of the launch take 4 to 5 us; a copy runs at 5.2); 12 tokens of 4 of 64 experts
+// on 2048 x 1424, groups of 64, 17.5 us for 63 MB.
 // Codes enter the matrix cores exactly; the group's sum of activations comes from one more product against ones; the
 // scale and the zero point (with the codes' offset) are applied to the fp32 sums group by group.
 // In a k-step of 32 features lane (l16, g) owns features 8 g .. 8 g + 7; it loads CW consecutive bytes of a packed row;

@@ -50,6 +50,8 @@ __global__ __launch_bounds__(1024) void sort_count_kernel(const ID *__restrict__
 // walk takes 64 pairs at a time: the lanes that share a bucket are found with one ballot per bit of the bucket number,
 // a lane's rank is the number of such lanes before it, and the first of them moves the counter on.
 // `counts` (several chunks): the pairs of every bucket in every chunk, from sort_count_kernel.
+// Bound by latency: ids come in, two passes over LDS counters, scattered stores of 4 bytes.  48 pairs: 3.0 us; 262144 pairs
+// of 128 experts: 2.4 us for the counts and 11.6 us for this kernel, whose 64 workgroups each add up all chunks' counts.
 template <typename ID>
 __global__ __launch_bounds__(1024) void sort_kernel(const ID *__restrict__ ids, int64_t P, int64_t chunk, int E,
                                                     const int *__restrict__ counts, int n_chunks,
@@ -142,7 +144,8 @@ template <typename T> struct Vec {
   static __device__ __forceinline__ void store(T *p, const Raw &r) { *reinterpret_cast<Raw *>(p) = r; }
 };
 
-// copies of the tokens' rows: each row is read once and written to its k places
+// copies of the tokens' rows: each row is read once and written to its k places.  Bound by the stores: 8192 rows of 4096
+// bf16 to two places each, 201 MB in 63 us (3.2 TB/s; stores alone run at 2.3 to 2.6 TB/s here).
 template <typename T>
 __global__ __launch_bounds__(256) void gather_kernel(const T *__restrict__ x, int top_k, int64_t K,
                                                      const int *__restrict__ position,
@@ -182,7 +185,8 @@ __global__ __launch_bounds__(256) void gather_kernel(const T *__restrict__ x, in
 template <typename TW>
 __device__ __forceinline__ float weight_at(const TW *w, int64_t i) { return w ? to_f32(w[i]) : 1.f; }
 
-// out[t] = sum_j w[t, j] y[position[t, j]], fp32 in order of j, rounded once; pairs that go nowhere are not read
+// out[t] = sum_j w[t, j] y[position[t, j]], fp32 in order of j, rounded once; pairs that go nowhere are not read.  Bound by
+// the loads: 4096 tokens of 4 rows of 4096 bf16, 168 MB in 38 us (4.4 TB/s).
 template <typename T, typename TO, typename TW>
 __global__ __launch_bounds__(256) void combine_kernel(const T *__restrict__ y, int top_k, int64_t N,
                                                       const int *__restrict__ position,
@@ -231,7 +235,8 @@ __global__ __launch_bounds__(256) void combine_kernel(const T *__restrict__ y, i
   }
 }
 
-// dy[p] = w[t, j] g[t] and dw[t, j] = <g[t], y[p]>, one workgroup per token; zero for pairs that go nowhere
+// dy[p] = w[t, j] g[t] and dw[t, j] = <g[t], y[p]>, one workgroup per token; zero for pairs that go nowhere.  y and dy pass
+// once, g stays in L2: 4096 tokens of 4 rows of 4096 bf16, 302 MB in 60 us (5.0 TB/s, what a copy reaches).
 template <typename T, typename TW>
 __global__ __launch_bounds__(256) void combine_grad_kernel(const T *__restrict__ y, const T *__restrict__ g, int top_k,
                                                            int64_t N, const int *__restrict__ position,
