@@ -282,7 +282,7 @@ def combine_tokens(y, plan, weights=None):
     y = _rows_of(_float_tensor(y), plan.n_rows, plan, "y")
     if weights is not None:
         weights = _on_device(_float_tensor(weights), plan.order, "weights")
-        if weights.numel() != plan.n_rows or (weights.dim() > 1 and weights.shape[-1] != plan.top_k):
+        if weights.numel() != plan.n_rows or (weights.shape[-1] != plan.top_k if weights.dim() > 1 else plan.top_k > 1):
             raise ValueError(f"weights must be [..., {plan.top_k}] with one row per token")
     if y.requires_grad or (weights is not None and weights.requires_grad):
         out = _CombineFn.apply(y, weights, plan)
@@ -362,7 +362,11 @@ def gptq_experts(W, xs, expert_ids, bits=4, **options):
 
     Each expert is solved by :func:`gptq` against the rows that reach it (sorted and gathered by the operators above).
     An expert that no row reaches has no Hessian; it is rounded to its own grid, which is the solve with the identity
-    as its Hessian.  ``options`` are those of :func:`gptq` (``block_size``, ``damping``, ``group_size``, ...)."""
+    as its Hessian.  ``options`` are those of :func:`gptq` (``block_size``, ``damping``, ``group_size``, ...) but ``H``
+    and ``shared``, which are one Hessian for several matrices."""
+    for name in ("H", "shared"):
+        if options.get(name) is not None:
+            raise ValueError(f"{name} is one Hessian for several matrices; every expert has its own")
     if not isinstance(W, torch.Tensor):
         W = _dev(W)
     if W.dim() != 3:

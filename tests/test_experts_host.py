@@ -6,7 +6,8 @@ import pytest
 import torch
 
 from jax_gptq_amd import _native as N
-from jax_gptq_amd.experts import QuantizedExperts, TokenPlan, quantized_expert_matmul, sort_tokens, stack_experts
+from jax_gptq_amd.experts import (QuantizedExperts, TokenPlan, gptq_experts, quantized_expert_matmul, sort_tokens,
+                                  stack_experts)
 from jax_gptq_amd.gptq import QuantizedMatrix
 
 NULL = ctypes.c_void_p(0)
@@ -125,3 +126,12 @@ def test_product_wants_a_stack_that_fits_the_plan():
         quantized_expert_matmul(torch.zeros(2, 32), torch.zeros(4, 32, 8), plan)
     with pytest.raises(ValueError):
         quantized_expert_matmul(torch.zeros(2, 32), QuantizedExperts(*_stack()), plan)
+
+
+def test_solve_refuses_one_hessian_for_all_experts():
+    # H and shared belong to matrices applied to the same activations; every expert has its own
+    W, xs, ids = torch.zeros(2, 128, 16), [torch.zeros(4, 128)], [torch.zeros(4, 1, dtype=torch.int64)]
+    with pytest.raises(ValueError, match="H"):
+        gptq_experts(W, xs, ids, H=torch.eye(128))
+    with pytest.raises(ValueError, match="shared"):
+        gptq_experts(W, xs, ids, shared={})

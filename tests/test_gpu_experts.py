@@ -254,6 +254,8 @@ def test_rows_leading_axes_strides_and_refusals(X):
     for bad in (torch.ones(3, 4), torch.ones(4, 3, 4)):
         with pytest.raises(ValueError):
             X.combine_tokens(y, plan, bad.cuda())
+    with pytest.raises(ValueError):
+        X.combine_tokens(y, plan, torch.ones(24).cuda())
 
 
 def test_combine_reads_no_row_of_nowhere(X):
@@ -379,6 +381,30 @@ def test_product_of_subnormal_rows(X, T):
     g = (torch.randn(T, 144) * 2e-5).half()
     y = X.quantized_expert_matmul(g.cuda(), layer.stack, plan, sorted_rows=True, transpose_b=True)
     check_product(y, g, layer, offsets, transpose=True)
+
+
+@pytest.mark.parametrize("T", [1, 60, 700])
+def test_product_where_nothing_goes_anywhere(X, T):
+    layer = Layer(X, T, 3, 1024, 1040, 4, 64)
+    plan = X.sort_tokens(torch.full((T, 2), -1).cuda(), 3)
+    for dt in ("fp16", "fp32"):
+        x = torch.full((T, 1024), float("nan")).to(TYPES[dt]).cuda().requires_grad_()
+        y = X.quantized_expert_matmul(x, layer.stack, plan)
+        assert (y == 0).all()
+        (dx,) = torch.autograd.grad(y, x, torch.full_like(y, float("nan")))
+        assert (dx == 0).all()
+
+
+@pytest.mark.parametrize("T,bits,group", [(2, 4, 0), (2, 8, 32), (40, 4, 32), (200, 8, 0), (200, 4, 65536)])
+def test_product_of_long_rows(X, T, bits, group):
+    E, K, N = 1, 131072, 144
+    layer = Layer(X, T, E, K, N, bits, group)
+    plan = X.sort_tokens(torch.zeros(T, 1, dtype=torch.int64).cuda(), E)
+    x = torch.randn(T, K).bfloat16()
+    check_product(X.quantized_expert_matmul(x.cuda(), layer.stack, plan), x, layer, [0, T])
+    g = torch.randn(T, N).bfloat16()
+    check_product(X.quantized_expert_matmul(g.cuda(), layer.stack, plan, sorted_rows=True, transpose_b=True), g, layer,
+                  [0, T], transpose=True)
 
 
 def test_tables_of_two_types(X):
