@@ -361,11 +361,13 @@ __global__ __launch_bounds__(128 * WM, XT == GPTQ_HIP_F32 ? 1 : 2) void back_ker
 #pragma unroll
     for (int i = 0; i < RB; ++i)
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int j = 0; j < 4; ++j) {
+        if (wm * 32 * RB + 32 * i + 8 * j >= tile.rows) continue;        // (rows past the last)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int c = 0; c < 4; ++c)
           to[((i * 4 + c) * 4 + j) * T::THREADS] =
               f32x4{acc[i][c][4 * j], acc[i][c][4 * j + 1], acc[i][c][4 * j + 2], acc[i][c][4 * j + 3]};
+      }
     return;
   }
 #pragma unroll
@@ -397,7 +399,7 @@ template <int XT, int BITS, int WM, int RB> __global__ __launch_bounds__(128 * W
   const int i = blockIdx.y >> 3, c0 = blockIdx.y >> 1 & 2, j = blockIdx.y & 3;
   const int lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5, wave = threadIdx.x >> 6;
   const int m0 = (wave >> 1) * 32 * RB + 32 * i + 8 * j + 4 * hi;
-  if (tile.rows <= 0 || tile.expert == a.E) return;
+  if (tile.rows <= m0 - 4 * hi || tile.expert == a.E) return;
   const bool f32 = a.out_dtype == GPTQ_HIP_F32;
   const f32x4 *from = reinterpret_cast<const f32x4 *>(t.parts) + (int64_t)blockIdx.x * (BM * BACK_BN / 4) + threadIdx.x;
   f32x4 w[BACK_MOST][2];

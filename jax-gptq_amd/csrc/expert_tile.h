@@ -606,7 +606,7 @@ template <int XT, int RBW> __global__ __launch_bounds__(256) void tile_join_kern
   const int i = blockIdx.y >> 2, j = blockIdx.y & 3, m0 = 32 * i + 8 * j + 4 * hi;
   const int64_t n = (int64_t)tile.col * BN + wave * 64 + 4 * (l32 & 15) + 2 * (l32 >> 4);
   const bool f32 = a.out_dtype == GPTQ_HIP_F32;
-  if (n >= a.C) return;
+  if (n >= a.C || 32 * i + 8 * j >= tile.rows) return;
   const f32x4 *from = reinterpret_cast<const f32x4 *>(t.parts) + (int64_t)blockIdx.x * (BM * BN / 4) + threadIdx.x;
   f32x4 w[TILE_MOST][2];
 #pragma unroll
