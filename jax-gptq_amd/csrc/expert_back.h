@@ -12,7 +12,7 @@
 // rows are used for four column blocks.  Rows, codes and tables travel to LDS without passing a register, several
 // stages deep, one barrier per stage, as in the untransposed tiles.
 // Measured: 16384 rows of 8 experts, 4096 x 11008, bf16: 2513 to 2570 us, 575 to 588 TFLOP/s of the 598 that two products
-// each leave; 4096 rows on 4096 x 4096, fp16: 275 us (499); 64 rows: 53 us, where 75 MB of weights and tables take 15.
+// each leave; 4096 rows on 4096 x 4096, fp16: 275 us (499); 64 rows: 47 us, where 75 MB of weights and tables take 15.
 #pragma once
 #include "expert_tile.h"
 
@@ -42,10 +42,10 @@ constexpr int BACK_MOST = 4, BACK_MIN_STAGES = 8;
 
 // Rows of a tile, by the rows of an expert on average.  The instructions that make the operands of codes are shared by
 // its rows, so a tall tile is the faster the fuller it is.  Measured with 32 / 64 / 128 rows, us a call:
-//   8 experts 4096 x 4096, fp16:   8 rows each 53 75 88,  60: 76 80 86,  125: 145 108 128,  200: 148 141 144,
-//                                  375: 317 235 232,  512: 384 300 274
-//   64 experts 2048 x 1424, bf16:  10 rows each 59 90 120,  31: 81 92 122,  64: 128 125 128,  256: 374 342 364
-//   8 experts 4096 x 4096, fp32:   8 rows each 66 77 131,  40: 115 77 130,  162: 224 251 235,  512: 565 525 525
+//   8 experts 4096 x 4096, fp16:   8 rows each 47 69 77,  60: 74 76 83,  125: 150 106 131,  200: 160 141 145,
+//                                  375: 318 236 234,  512: 382 301 274
+//   64 experts 2048 x 1424, bf16:  10 rows each 55 81 124,  31: 80 88 125,  64: 126 128 130,  256: 370 342 367
+//   8 experts 4096 x 4096, fp32:   8 rows each 60 70 126,  40: 116 75 125,  162: 223 250 235,  512: 568 518 524
 enum BackRows { BACK_32, BACK_64, BACK_128 };
 static inline BackRows back_rows(int64_t P, int E) {
   const int64_t rows = P / E;
