@@ -245,7 +245,7 @@ struct Split {
   uint32_t full, rem;                 // items in whole rounds, and after them
   int parts;                          // of each of those
 };
-__device__ __host__ __forceinline__ Split split_items(uint32_t items, uint32_t slots, int most) {
+__device__ __forceinline__ Split split_items(uint32_t items, uint32_t slots, int most) {
   Split s;
   s.full = items / slots * slots;
   s.rem = items - s.full;
