@@ -30,13 +30,15 @@ __all__ = ["QuantizedExperts", "TokenPlan", "stack_experts", "gptq_experts", "so
 MAX_EXPERTS = 1024
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream       # (torch.cuda.current_stream builds an object: 2 us a call)
+# A call's share of the host is what a small one takes, and a backward pass runs this on the engine's thread, where
+# every Python step takes twice as long: so no objects for streams and devices (2 us a call) in here.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current = torch._C._cuda_getDevice
 
 
-def _launch(entry, device, what, *args):
-    """Calls a C entry point on ``device``'s current stream; pointers are passed as integers."""
-    index = device.index
-    if index == torch.cuda.current_device():
+def _launch(entry, index, what, *args):
+    """Calls a C entry point on the current stream of GPU ``index``; pointers are passed as integers."""
+    if index == _current():
         code = entry(_raw_stream(index), *args)
     else:
         with torch.cuda.device(index):
@@ -47,7 +49,7 @@ def _launch(entry, device, what, *args):
 
 def _on_device(t, like, what):
     """``t`` contiguous; operands of one call live on one GPU."""
-    if t.device != like.device:
+    if t.get_device() != like.get_device():
         raise ValueError(f"{what} is on {t.device}, expected {like.device}")
     return t if t.is_contiguous() else t.contiguous()
 
@@ -151,11 +153,8 @@ class TokenPlan:
         self.token_shape = tuple(token_shape)
         self.top_k = top_k
         self.n_experts = n_experts
-        self.n_tokens = order.numel() // top_k
-
-    @property
-    def n_rows(self):
-        return self.order.numel()
+        self.n_rows = order.numel()
+        self.n_tokens = self.n_rows // top_k
 
 
 def sort_tokens(expert_ids, n_experts):
@@ -176,44 +175,42 @@ def sort_tokens(expert_ids, n_experts):
     if top_k == 0:
         raise ValueError("at least one choice per token")
     ids = ids.contiguous()
-    P, device = ids.numel(), ids.device
-    lib = N.load()
-    order, position, offsets = torch.empty(2 * P + n_experts + 1, dtype=torch.int32, device=device).split(
-        (P, P, n_experts + 1))
+    P, lib = ids.numel(), N.load()
+    order, position, offsets = ids.new_empty(2 * P + n_experts + 1, dtype=torch.int32).split((P, P, n_experts + 1))
     nbytes = lib.gptq_hip_expert_sort_workspace_bytes(P, n_experts)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    _launch(lib.gptq_hip_expert_sort, device, "expert_sort", ids.data_ptr(), ids.element_size(), P, n_experts,
+    ws = ids.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _launch(lib.gptq_hip_expert_sort, ids.get_device(), "expert_sort", ids.data_ptr(), ids.element_size(), P, n_experts,
             order.data_ptr(), position.data_ptr(), offsets.data_ptr(), ws.data_ptr() if nbytes else None, nbytes)
     return TokenPlan(order, position, offsets, ids.shape[:-1], top_k, n_experts)
 
 
 def _rows_of(x, rows, plan, what):
     """``x`` as ``[rows, width]`` on the plan's GPU."""
-    if x.dim() < 2:
+    dims = x.dim()
+    if dims < 2:
         raise ValueError(f"{what} must have at least 2 dimensions")
     x = _on_device(x, plan.order, what)
-    shape = x.shape
-    width = shape[-1]
+    width = x.size(-1)
     if width == 0 or x.numel() != rows * width:
         raise ValueError(f"{what} has {x.numel() // max(width, 1)} rows of {width}, expected {rows}")
-    return x if len(shape) == 2 else x.reshape(rows, width)
+    return x if dims == 2 else x.reshape(rows, width)
 
 
 def _combine_raw(y, plan, weights, out_dtype):
-    width, device = y.shape[1], y.device
-    out = torch.empty((plan.n_tokens, width), dtype=out_dtype, device=device)
-    _launch(N.load().gptq_hip_expert_combine, device, "expert_combine", y.data_ptr(), _DT[y.dtype], plan.n_tokens,
-            plan.top_k, width, plan.position.data_ptr(), plan.offsets.data_ptr(), plan.n_experts,
-            None if weights is None else weights.data_ptr(), N.F32 if weights is None else _DT[weights.dtype],
+    width, tokens = y.size(1), plan.n_tokens
+    out = y.new_empty((tokens, width), dtype=out_dtype)
+    w, w_dtype = (None, N.F32) if weights is None else (weights.data_ptr(), _DT[weights.dtype])
+    _launch(N.load().gptq_hip_expert_combine, y.get_device(), "expert_combine", y.data_ptr(), _DT[y.dtype], tokens,
+            plan.top_k, width, plan.position.data_ptr(), plan.offsets.data_ptr(), plan.n_experts, w, w_dtype,
             out.data_ptr(), _DT[out_dtype])
     return out
 
 
 def _gather_raw(x, plan):
-    width, device = x.shape[1], x.device
-    out = torch.empty((plan.n_rows, width), dtype=x.dtype, device=device)
-    _launch(N.load().gptq_hip_expert_gather, device, "expert_gather", x.data_ptr(), _DT[x.dtype], plan.n_tokens,
-            plan.top_k, width, plan.position.data_ptr(), plan.offsets.data_ptr(), plan.n_experts, out.data_ptr())
+    width, tokens, top_k = x.size(1), plan.n_tokens, plan.top_k
+    out = x.new_empty((tokens * top_k, width))
+    _launch(N.load().gptq_hip_expert_gather, x.get_device(), "expert_gather", x.data_ptr(), _DT[x.dtype], tokens,
+            top_k, width, plan.position.data_ptr(), plan.offsets.data_ptr(), plan.n_experts, out.data_ptr())
     return out
 
 
@@ -227,9 +224,10 @@ class _GatherFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g):
+        plan = ctx.plan
         if torch.is_grad_enabled():
-            return combine_tokens(g, ctx.plan).reshape(ctx.plan.n_tokens, -1), None
-        return _combine_raw(g.contiguous(), ctx.plan, None, g.dtype), None
+            return combine_tokens(g, plan).reshape(plan.n_tokens, -1), None
+        return _combine_raw(g if g.is_contiguous() else g.contiguous(), plan, None, g.dtype), None
 
 
 def gather_tokens(x, plan):
@@ -252,10 +250,11 @@ class _CombineFn(torch.autograd.Function):
         plan = ctx.plan
         if torch.is_grad_enabled():
             return _combine_grad_graph(y, weights, g, plan) + (None,)
-        g = g.contiguous()
+        if not g.is_contiguous():
+            g = g.contiguous()
         dy = torch.empty_like(y) if ctx.needs_input_grad[0] else None
         dw = torch.empty_like(weights) if ctx.needs_input_grad[1] else None
-        _launch(N.load().gptq_hip_expert_combine_grad, y.device, "expert_combine_grad", y.data_ptr(), g.data_ptr(),
+        _launch(N.load().gptq_hip_expert_combine_grad, y.get_device(), "expert_combine_grad", y.data_ptr(), g.data_ptr(),
                 _DT[y.dtype], plan.n_tokens, plan.top_k, y.shape[1], plan.position.data_ptr(),
                 plan.offsets.data_ptr(), plan.n_experts, None if weights is None else weights.data_ptr(),
                 N.F32 if weights is None else _DT[weights.dtype], None if dy is None else dy.data_ptr(),
@@ -288,20 +287,20 @@ def combine_tokens(y, plan, weights=None):
         out = _CombineFn.apply(y, weights, plan)
     else:
         out = _combine_raw(y, plan, weights, y.dtype)
-    return out if len(plan.token_shape) == 1 else out.reshape(plan.token_shape + (y.shape[1],))
+    return out if len(plan.token_shape) == 1 else out.reshape(plan.token_shape + (y.size(1),))
 
 
 def _expert_matmul_raw(x, packed, zero, scale, bits, group, plan, sorted_rows, transpose_b, out_dtype):
-    lib, device = N.load(), x.device
+    lib = N.load()
     E, R, C = packed.shape
-    x_rows, x_dtype, n_rows = x.shape[0], _DT[x.dtype], plan.n_rows
-    out = torch.empty((n_rows, R * (8 // bits) if transpose_b else C), dtype=out_dtype, device=device)
+    x_rows, x_dtype, n_rows = x.size(0), _DT[x.dtype], plan.n_rows
+    out = x.new_empty((n_rows, R * (8 // bits) if transpose_b else C), dtype=out_dtype)
     if transpose_b and x.data_ptr() % 16:
         x = x.clone()           # (the transposed kernels load 16 bytes at a time)
     nbytes = lib.gptq_hip_expert_qmatmul_workspace_bytes(x_rows, n_rows, R, C, bits, group, E, x_dtype, _DT[zero.dtype],
                                                          transpose_b)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    _launch(lib.gptq_hip_expert_qmatmul, device, "expert_qmatmul", x.data_ptr(), x_dtype, x_rows,
+    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _launch(lib.gptq_hip_expert_qmatmul, x.get_device(), "expert_qmatmul", x.data_ptr(), x_dtype, x_rows,
             None if sorted_rows else plan.order.data_ptr(), plan.top_k, n_rows, plan.offsets.data_ptr(), E,
             packed.data_ptr(), R, C, zero.data_ptr(), scale.data_ptr(), _DT[zero.dtype], group, bits, transpose_b,
             out.data_ptr(), _DT[out_dtype], ws.data_ptr() if nbytes else None, nbytes)
