@@ -157,18 +157,22 @@ static Choice choose(int64_t P, int E, int64_t C, int64_t group, int x_dtype, in
   return {Choice::TILE, !wide && rows > 56 && rows <= 128 ? TILE_64x256_K2 : TILE_64x256};
 }
 
+// the sizes that the product takes
+static bool sizes_fit(int64_t x_rows, int64_t rows, int64_t R, int64_t C, int bits, int64_t group, int E) {
+  if ((bits != 4 && bits != 8) || E < 1 || E > 1024 || R < 1 || C < 1 || x_rows < 0 || rows < 0) return false;
+  const int64_t lim = (int64_t)1 << 30;
+  // (the plain kernels have one workgroup of 256 threads per row and four output columns in a grid dimension)
+  if (rows >= (int64_t)1 << 24 || R > lim || C > (int64_t)1 << 20 || x_rows > lim) return false;
+  const int64_t K = bits == 4 ? 2 * R : R;
+  return K <= 262140 && group >= 0 && !(group && (K % group || (bits == 4 && group % 2)));
+}
+
 // GPTQ_HIP_OK, or why the product is refused
 static int check_args(const ExpertArgs &a) {
   if (a.bits != 4 && a.bits != 8) return GPTQ_HIP_EINVAL;
   if (!float_type(a.x_dtype) || !float_type(a.out_dtype) || !float_type(a.zs_dtype)) return GPTQ_HIP_EDTYPE;
   if (a.out_dtype != a.x_dtype && a.out_dtype != GPTQ_HIP_F32) return GPTQ_HIP_EDTYPE;
-  const int64_t lim = (int64_t)1 << 30;
-  if (a.E < 1 || a.E > 1024 || a.top_k < 1 || a.T < 0 || a.P < 0 || a.R < 1 || a.C < 1) return GPTQ_HIP_EINVAL;
-  // (the plain kernels have one workgroup of 256 threads per row and four output columns in a grid dimension)
-  if (a.P >= (int64_t)1 << 24 || a.R > lim || a.C > (int64_t)1 << 20 || a.T > lim) return GPTQ_HIP_EINVAL;
-  const int64_t K = a.bits == 4 ? 2 * a.R : a.R;
-  if (K > 262140) return GPTQ_HIP_EINVAL;
-  if (a.group < 0 || (a.group && (K % a.group || (a.bits == 4 && a.group % 2)))) return GPTQ_HIP_EINVAL;
+  if (!sizes_fit(a.T, a.P, a.R, a.C, a.bits, a.group, a.E) || a.top_k < 1) return GPTQ_HIP_EINVAL;
   if (a.order ? a.P != a.T * a.top_k : a.P != a.T) return GPTQ_HIP_EINVAL;
   if (a.P == 0) return GPTQ_HIP_OK;
   if (!a.x || !a.offsets || !a.packed || !a.zero || !a.scale || !a.out) return GPTQ_HIP_EINVAL;
@@ -182,7 +186,8 @@ extern "C" {
 size_t gptq_hip_expert_qmatmul_workspace_bytes(int64_t x_rows, int64_t rows, int64_t R, int64_t C, int bits,
                                                int64_t group_size, int n_experts, int x_dtype, int zs_dtype,
                                                int transpose_b) {
-  if (n_experts < 1 || rows <= 0 || x_rows <= 0 || R <= 0 || C <= 0 || group_size < 0) return 0;
+  if (!sizes_fit(x_rows, rows, R, C, bits, group_size, n_experts) || rows == 0 || x_rows == 0) return 0;
+  if (!float_type(x_dtype) || !float_type(zs_dtype)) return 0;
   const Choice c = choose(rows, n_experts, C, group_size, x_dtype, transpose_b);
   if (c.kind == Choice::TILE)
     return xqmm::staged_layout(x_rows, rows, bits == 4 ? 2 * R : R, C, group_size, n_experts, x_dtype, c.shape).bytes;

@@ -361,7 +361,7 @@ static int sort_launch(hipStream_t s, const void *ids, int64_t P, int E, int *or
 extern "C" {
 
 size_t gptq_hip_expert_sort_workspace_bytes(int64_t pairs, int n_experts) {
-  if (pairs <= 0 || n_experts < 1 || n_experts > MAX_EXPERTS) return 0;
+  if (pairs <= 0 || pairs > (int64_t)1 << 30 || n_experts < 1 || n_experts > MAX_EXPERTS) return 0;
   const int64_t chunk = sort_chunk(pairs);
   return pairs <= chunk ? 0 : (size_t)ceil_div64(pairs, chunk) * (n_experts + 1) * 4;
 }

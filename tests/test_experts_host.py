@@ -135,3 +135,14 @@ def test_solve_refuses_one_hessian_for_all_experts():
         gptq_experts(W, xs, ids, H=torch.eye(128))
     with pytest.raises(ValueError, match="shared"):
         gptq_experts(W, xs, ids, shared={})
+
+
+def test_workspace_query_of_what_the_product_refuses(lib):
+    def need(x_rows=600, rows=1200, R=512, C=1024, bits=4, group=64, experts=4, dt=N.F16, zdt=N.F32, tr=0):
+        return lib.gptq_hip_expert_qmatmul_workspace_bytes(x_rows, rows, R, C, bits, group, experts, dt, zdt, tr)
+    assert need() > 0 and need(tr=1) > 0
+    for bad in (dict(group=1 << 32), dict(group=-64), dict(group=1 << 40, R=1 << 50), dict(group=96), dict(bits=3),
+                dict(rows=1 << 24), dict(x_rows=1 << 40), dict(R=1 << 40), dict(C=1 << 40), dict(experts=0),
+                dict(experts=1 << 20), dict(rows=0), dict(x_rows=-1), dict(dt=9), dict(zdt=N.F64)):
+        for tr in (0, 1):
+            assert need(**bad, tr=tr) == 0, (bad, tr)
