@@ -355,9 +355,9 @@ int gptq_hip_expert_combine_grad(void *stream, const void *y, const void *g, int
  * untouched by it.  rows < 2^24, K <= 262140, C <= 2^20.  Equal calls give equal bits; the order of a row's sums
  * depends on how many rows every expert has.
  * ws, 16-byte aligned: gptq_hip_expert_qmatmul_workspace_bytes (contents need no preparation; calls that overlap in
- * time need one each; 0 for sizes that the product refuses).  The first call of a kind on a device raises kernels' limits of LDS: make one before capturing.
- * Plain kernels, an order of magnitude slower, take groups that are no multiple of 32, fewer than 16 channels and,
- * transposed, an x that is not 16-byte aligned. */
+ * time need one each; 0 for sizes that the product refuses).  The first call of a kind on a device raises kernels'
+ * limits of LDS: make one before capturing.  Plain kernels, an order of magnitude slower, take groups that are no
+ * multiple of 32, fewer than 16 channels and, transposed, an x that is not 16-byte aligned. */
 size_t gptq_hip_expert_qmatmul_workspace_bytes(int64_t x_rows, int64_t rows, int64_t R, int64_t C, int bits,
                                                int64_t group_size, int n_experts, int x_dtype, int zs_dtype,
                                                int transpose_b);
