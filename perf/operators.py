@@ -25,18 +25,8 @@ _TYPES = {"fp16": torch.float16, "bf16": torch.bfloat16, "fp32": torch.float32}
 _BYTES = {"fp16": 2, "bf16": 2, "fp32": 4}
 
 
-_package = None
-
-
 def _experts():
-    """The package's operators (only where `own` is true), looked up once as a program's import does."""
-    global _package
-    if _package is None:
-        _package = _import_experts()
-    return _package
-
-
-def _import_experts():
+    """The package's operators (only where `own` is true)."""
     path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "jax-gptq_amd")
     if path not in sys.path:
         sys.path.insert(0, path)
