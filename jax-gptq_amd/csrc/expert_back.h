@@ -6,7 +6,8 @@
 // The scale varies along the contraction, so it goes to the activations: a = x s in fp32, cut to 16 bits and split
 // into two bf16 parts (fp32 activations: all 24 bits in three), which meet the exact codes in as many products; the
 // second sum is taken in fp32 over the very values that were multiplied.  The cut is 2^-16 of a term, far below the
-// rounding of a 16-bit result; one part of 8 or 11 bits would not be.
+// rounding of a 16-bit result; one part of 8 or 11 bits would not be.  The second sum is taken from the first every
+// BACK_CLOSE channels.
 // Bound by the matrix cores, two products per 16-bit operand pair, and by the instructions that make the parts: a
 // wavefront owns 32 or 64 rows x 128 features (one group of 128, or two or four smaller ones), so that the parts of its
 // rows are used for four column blocks.  Rows, codes and tables travel to LDS without passing a register, several
@@ -36,6 +37,12 @@ static __global__ __launch_bounds__(256) void widen_tables_kernel(const char *__
 }
 
 constexpr int BACK_BN = 256;
+// Channels after which the second sum is taken from the first.  With gradients of one sign both grow by a hundred times
+// what their difference does, so that over all channels their rounding is what is left of it.  Largest error against the
+// size of the results for a gradient of ones, 11008 channels, fp16 rows, 4 bits: 1.6e-3 without, 2.9e-4 / 1.5e-4 / 5.6e-5
+// every 512 / 256 / 128; fp32 rows 2.8e-4, 1.2e-5 / 6.8e-6 / 5.0e-6.  It costs 16384 bf16 rows on 4096 x 11008 2 to 4 %
+// (2527, then 2574 / 2596 / 2635 us); fp32 rows gain (526, then 474 / 481 / 486 us for 4096 rows on 4096 x 4096).
+constexpr int BACK_CLOSE = 128;
 // A contraction is cut into at most four parts of at least eight stages (six or eight parts, or of four stages, are no
 // faster: what the tiles gain their sums' way through memory costs).
 constexpr int BACK_MOST = 4, BACK_MIN_STAGES = 8;
@@ -312,6 +319,27 @@ __global__ __launch_bounds__(128 * WM, XT == GPTQ_HIP_F32 ? 1 : 2) void back_ker
     }
   };
 
+  // The second sums leave the first: one product each.  A lane's sum lies with row l32, over its half of the channels, in
+  // three bf16 parts against -1.
+  auto close = [&]() __attribute__((always_inline)) {
+    constexpr int RBS = 4 / CB, HALF_BLOCK = NG > RBS;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const uint32_t keep = !HALF_BLOCK || (l32 >> 4) == (g & 1) ? 0xFFFFFFFFu : 0u;
+      const u32x4 minus = {0xBF80BF80u & keep, 0x0000BF80u & keep, 0u, 0u};
+#pragma unroll
+      for (int i = 0; i < RB; ++i) {
+        uint32_t part[3];
+        three_parts(sub[g][i], part);
+        sub[g][i] = 0.f;
+        const u32x4 sum = {upper_halves(part[0], part[1]), upper_halves(part[2], 0u), 0u, 0u};
+#pragma unroll
+        for (int c = HALF_BLOCK ? g / 2 * CB : g * 4 / NG; c < (HALF_BLOCK ? (g / 2 + 1) * CB : (g + 1) * 4 / NG); ++c)
+          acc[i][c] = O::mma32(sum, minus, acc[i][c]);
+      }
+    }
+  };
+
   constexpr int AHEAD = T::STAGES - 1;
   const int first = (int)((int64_t)t.stages * unit.part / unit.parts);
   const int past = (int)((int64_t)t.stages * (unit.part + 1) / unit.parts);
@@ -327,35 +355,13 @@ __global__ __launch_bounds__(128 * WM, XT == GPTQ_HIP_F32 ? 1 : 2) void back_ker
     const char *base = lds + slot * T::STAGE;
 #pragma unroll
     for (int h = 0; h < 2 * T::STEPS; ++h) step(base, h / 2, h % 2);
+    if ((s + 1 - first) % (BACK_CLOSE / T::BK) == 0 || s + 1 == past) close();
     land(into);
     slot = slot + 1 == T::STAGES ? 0 : slot + 1;
     into = into + 1 == T::STAGES ? 0 : into + 1;
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // no load may reach LDS after this workgroup's end
 
-  // the second sum lies with row l32 of each block, half of it in either half of the wavefront
-#pragma unroll
-  for (int g = 0; g < NG; ++g)
-#pragma unroll
-    for (int i = 0; i < RB; ++i) sub[g][i] += __shfl_xor(sub[g][i], 32);
-#pragma unroll
-  for (int i = 0; i < RB; ++i)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int in = 8 * (r / 4) + 4 * hi + r % 4;
-#pragma unroll
-      for (int b = 0; b < 4 / CB; ++b) {
-        float d;
-        if constexpr (NG > 4 / CB) {                    // two groups in a block
-          const float d0 = __shfl(sub[2 * b][i], in), d1 = __shfl(sub[2 * b + 1][i], in);
-          d = l32 < 16 ? d0 : d1;
-        } else {
-          d = __shfl(sub[b * NG * CB / 4][i], in);
-        }
-#pragma unroll
-        for (int c = 0; c < CB; ++c) acc[i][b * CB + c][r] -= d;
-      }
-    }
   if (unit.parts > 1) {
     f32x4 *to = reinterpret_cast<f32x4 *>(t.parts) + (int64_t)unit.slot * (T::BM * T::BN / 4) + threadIdx.x;
 #pragma unroll
