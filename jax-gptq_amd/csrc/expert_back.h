@@ -3,17 +3,19 @@
 //
 //   y[p, k] = sum_n (x[p, n] s[G(k), n]) (o + c[k, n]) - sum_n (x[p, n] s[G(k), n]) (o + z[G(k), n])
 //
-// The scale varies along the contraction, so it goes to the activations: a = x s in fp32, cut to 16 bits and split
-// into two bf16 parts (fp32 activations: all 24 bits in three), which meet the exact codes in as many products; the
-// second sum is taken in fp32 over the very values that were multiplied.  The cut is 2^-16 of a term, far below the
-// rounding of a 16-bit result; one part of 8 or 11 bits would not be.  The second sum is taken from the first every
+// The scale varies along the contraction, so it goes to the activations: a = x s in fp32, as two bf16 parts, each rounded
+// to nearest (fp32 activations: all 24 bits in three), which meet the exact codes in as many products; the second sum is
+// taken in fp32 over the very values that were multiplied.  What two parts leave out is 2^-18 of a term at most, far below
+// the rounding of a 16-bit result; one part of 8 or 11 bits would not be.  The second sum is taken from the first every
 // BACK_CLOSE channels.
 // Bound by the matrix cores, two products per 16-bit operand pair, and by the instructions that make the parts: a
 // wavefront owns 32 or 64 rows x 128 features (one group of 128, or two or four smaller ones), so that the parts of its
 // rows are used for four column blocks.  Rows, codes and tables travel to LDS without passing a register, several
 // stages deep, one barrier per stage, as in the untransposed tiles.
-// Measured: 16384 rows of 8 experts, 4096 x 11008, bf16: 2513 to 2570 us, 575 to 588 TFLOP/s of the 598 that two products
-// each leave; 4096 rows on 4096 x 4096, fp16: 275 us (499); 64 rows: 47 us, where 75 MB of weights and tables take 15.
+// Measured: 16384 rows of 8 experts, 4096 x 11008, bf16: 2720 us, 543 TFLOP/s of the 598 that two products each leave;
+// 4096 rows on 4096 x 4096, fp16: 293 us (469); 64 rows: 46 us, where 75 MB of weights and tables take 15.  Parts that are
+// cut off instead of rounded (2^-15 of a term, always towards zero) took 2645, 295 and 48.5 us; with groups of 32, where
+// the parts are made once per group, 577 instead of 661 us for 2000 rows.
 #pragma once
 #include "expert_tile.h"
 
@@ -94,6 +96,13 @@ struct BackArgs {
   int stages, slots, most;
   float *parts;                 // sums of parts
 };
+
+// {bf16(a), bf16(b)}, rounded to nearest
+__device__ __forceinline__ uint32_t nearest2(float a, float b) {
+  typedef float float2v __attribute__((ext_vector_type(2)));
+  typedef __bf16 bfloat2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2v){a, b}, bfloat2));
+}
 
 // NG: groups a wavefront's 128 features lie in; the tile's rows are WM times RB blocks of 32, a wavefront has RB of them
 template <int XT, int BITS, bool ALIGNED, int NG, int WM, int RB> struct BackShape {
@@ -239,40 +248,47 @@ __global__ __launch_bounds__(128 * WM, XT == GPTQ_HIP_F32 ? 1 : 2) void back_ker
 #pragma unroll
       for (int i = 0; i < RB; ++i) {
         const char *row = base + (wm * 32 * RB + 32 * i + l32) * 128;
-        uint32_t part[T::PARTS][8];
 #pragma unroll
-        for (int e4 = 0; e4 < 2; ++e4) {                // 4 channels at a time (fp32), or of 8 (16 bits)
+        for (int e = 0; e < 8; e += 2) {                // two channels at a time, of 4 (fp32) or 8 in 16 bytes
           u32x4 q;
-          if (XT == GPTQ_HIP_F32) q = *reinterpret_cast<const u32x4 *>(row + ((n / 4 + e4) ^ (l32 & 7)) * 16);
+          if (XT == GPTQ_HIP_F32) q = *reinterpret_cast<const u32x4 *>(row + ((n / 4 + e / 4) ^ (l32 & 7)) * 16);
           else q = *reinterpret_cast<const u32x4 *>(row + ((n / 8) ^ (l32 & 7)) * 16);
+          float p[2];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int e = 4 * e4 + k;
-            const uint32_t word = XT == GPTQ_HIP_F32 ? q[k] : q[e / 2];
-            float p;
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t word = XT == GPTQ_HIP_F32 ? q[(e + k) & 3] : q[e / 2];
             if (XT == GPTQ_HIP_F32) {
-              p = __builtin_bit_cast(float, word) * s[e];
+              p[k] = __builtin_bit_cast(float, word) * s[e + k];
             } else if (XT == GPTQ_HIP_BF16) {
-              p = __builtin_bit_cast(float, (e & 1) ? word & 0xFFFF0000u : word << 16) * s[e];
+              p[k] = __builtin_bit_cast(float, k ? word & 0xFFFF0000u : word << 16) * s[e + k];
             } else {                                    // (conversion and product in one instruction)
-              const uint16_t h = (uint16_t)((e & 1) ? word >> 16 : word);
-              p = fmaf((float)__builtin_bit_cast(_Float16, h), s[e], 0.f);
-            }
-            if (T::PARTS == 2) p = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, p) & 0xFFFFFF00u);
-            sub[g][i] = fmaf(p, z[e], sub[g][i]);
-            part[0][e] = __builtin_bit_cast(uint32_t, p);
-#pragma unroll
-            for (int c = 1; c < T::PARTS; ++c) {
-              p -= __builtin_bit_cast(float, part[c - 1][e] & 0xFFFF0000u);
-              part[c][e] = __builtin_bit_cast(uint32_t, p);
+              const uint16_t h = (uint16_t)(k ? word >> 16 : word);
+              p[k] = fmaf((float)__builtin_bit_cast(_Float16, h), s[e + k], 0.f);
             }
           }
+          if constexpr (T::PARTS == 2) {                // rounded to nearest, both of them; the sum is of their values
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const uint32_t both = nearest2(p[0], p[1]);
+              x[i][c][e / 2] = both;
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const float v = __builtin_bit_cast(float, k ? both & 0xFFFF0000u : both << 16);
+                sub[g][i] = fmaf(v, z[e + k], sub[g][i]);
+                p[k] -= v;
+              }
+            }
+          } else {
+            uint32_t part[2][3];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              sub[g][i] = fmaf(p[k], z[e + k], sub[g][i]);
+              three_parts(p[k], part[k]);
+            }
+#pragma unroll
+            for (int c = 0; c < T::PARTS; ++c) x[i][c][e / 2] = upper_halves(part[0][c], part[1][c]);
+          }
         }
-#pragma unroll
-        for (int c = 0; c < T::PARTS; ++c)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            x[i][c][e] = __builtin_amdgcn_perm(part[c][2 * e + 1], part[c][2 * e], 0x07060302u);
       }
       // blocks of 32 packed rows with columns in this group; a block of 4-bit codes and groups of 32 columns lies in two
       // groups, each takes its half of the lanes

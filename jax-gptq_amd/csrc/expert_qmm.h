@@ -24,7 +24,7 @@ enum { TILE_32x256, TILE_64x256, TILE_64x256_K2 };
 int expert_tile_f16(hipStream_t s, const ExpertArgs &a, int shape, void *ws);
 int expert_tile_bf16(hipStream_t s, const ExpertArgs &a, int shape, void *ws);
 int expert_tile_f32(hipStream_t s, const ExpertArgs &a, int shape, void *ws);
-// the transposed product by tiles of 128 rows x 256 input features (expert_back.h)
+// the transposed product by tiles of 32, 64 or 128 rows x 256 input features (expert_back.h)
 int expert_back_f16(hipStream_t s, const ExpertArgs &a, void *ws);
 int expert_back_bf16(hipStream_t s, const ExpertArgs &a, void *ws);
 int expert_back_f32(hipStream_t s, const ExpertArgs &a, void *ws);

@@ -335,10 +335,12 @@ def quantized_expert_matmul(x, experts, plan, sorted_rows=False, transpose_b=Fal
     ``x`` holds the tokens ``[T, K]`` (``[..., K]``), whose rows the kernels fetch through the plan, or, with
     ``sorted_rows``, the rows in sorted order ``[T * top_k, K]``.  The codes enter the matrix cores exactly (fp32
     activations as three bfloat16 parts), sums and scales are fp32, and the result is rounded once to ``x``'s type
-    (``quantized_matmul`` rounds to fp16 on the way, as the reference does).  A row of ``x`` with an infinity or a NaN
-    may become NaN throughout, other rows do not see it; so may one whose sums of ``x`` times codes over a group, which
-    come before the scale, leave fp32's range.  Equal calls give equal bits; which kernel runs, and with it the order of
-    a row's sums, follows from the number of rows of every expert.  Differentiable with respect to ``x``."""
+    (``quantized_matmul`` rounds to fp16 on the way, as the reference does).  ``transpose_b``, and with it the gradient,
+    applies the scale to ``x``: 16-bit rows times scale enter as two bfloat16 parts, which leave out up to 2^-18 of each
+    term.  A row of ``x`` with an infinity or a NaN may become NaN throughout, other rows do not see it; so may one whose
+    sums of ``x`` times codes over a group, which come before the scale, or, transposed, of ``x`` times scale times codes
+    leave fp32's range.  Equal calls give equal bits; which kernel runs, and with it the order of a row's sums, follows
+    from the number of rows of every expert.  Differentiable with respect to ``x``."""
     if not isinstance(experts, QuantizedExperts):
         raise TypeError("experts must be QuantizedExperts")
     if len(experts) != plan.n_experts:
