@@ -106,3 +106,19 @@ def test_transposed_product_cuts_operands_by_2_to_the_minus_18(X, rows, bits, gr
     err = (wide_product(g.cuda(), layer.stack, plan, 1).cpu().double() - ref).abs()
     tol = 2.0 ** -18 * ref + (2 * N // 16 + 3) * 2.0 ** -24 * size
     assert (err <= tol).all(), float((err / ref).max())
+
+
+# rows: strips, tiles of 32 and 64 rows
+@pytest.mark.parametrize("rows", [4, 28, 100, 200])
+@pytest.mark.parametrize("K,bits,group", [(8192, 4, 8192), (8192, 4, 0), (6144, 4, 1024), (8448, 8, 4224), (4928, 4, 704),
+                                          (65536, 4, 65536), (4096, 4, 128)])
+@pytest.mark.parametrize("dt", ["fp16", "bf16", "fp32"])
+def test_product_of_one_sign(X, rows, K, bits, group, dt):
+    """Rows behind a function that leaves one sign; sums without groups and groups of many hundred features."""
+    layer = Layer(X, K, 1, K, 144, bits, group)
+    x = torch.randn(rows, K).abs()
+    x[:rows // 2] = 1
+    x = x.to(TYPES[dt])
+    y = X.quantized_expert_matmul(x.cuda(), layer.stack, one_expert(X, rows))
+    # pieces of 512 features: up to 96 products, 8 + 8 + 8 additions for the rows' sum, what joins them
+    check_pieces(y, x, layer, 512, 96 + 24 + 8)
