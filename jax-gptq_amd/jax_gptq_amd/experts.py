@@ -196,82 +196,97 @@ def _rows_of(x, rows, plan, what):
     return x if dims == 2 else x.reshape(rows, width)
 
 
-def _combine_raw(y, plan, weights, out_dtype):
-    width, tokens = y.size(1), plan.n_tokens
+def _combine_raw(y, weights, position, offsets, top_k, out_dtype):
+    width, tokens = y.size(1), position.numel() // top_k
     out = y.new_empty((tokens, width), dtype=out_dtype)
     w, w_dtype = (None, N.F32) if weights is None else (weights.data_ptr(), _DT[weights.dtype])
     _launch(N.load().gptq_hip_expert_combine, y.get_device(), "expert_combine", y.data_ptr(), _DT[y.dtype], tokens,
-            plan.top_k, width, plan.position.data_ptr(), plan.offsets.data_ptr(), plan.n_experts, w, w_dtype,
-            out.data_ptr(), _DT[out_dtype])
+            top_k, width, position.data_ptr(), offsets.data_ptr(), offsets.numel() - 1, w, w_dtype, out.data_ptr(),
+            _DT[out_dtype])
     return out
 
 
-def _gather_raw(x, plan):
-    width, tokens, top_k = x.size(1), plan.n_tokens, plan.top_k
+def _gather_raw(x, position, offsets, top_k):
+    tokens, width = x.shape
     out = x.new_empty((tokens * top_k, width))
     _launch(N.load().gptq_hip_expert_gather, x.get_device(), "expert_gather", x.data_ptr(), _DT[x.dtype], tokens,
-            top_k, width, plan.position.data_ptr(), plan.offsets.data_ptr(), plan.n_experts, out.data_ptr())
+            top_k, width, position.data_ptr(), offsets.data_ptr(), offsets.numel() - 1, out.data_ptr())
     return out
 
 
-# The backward passes are launches that record nothing, so where a graph of the gradient itself is asked for (grad mode
-# is on in a backward pass then) they go through the differentiable operators instead.
+# What a backward pass reads is saved by the graph, which refuses tensors that were written to since.  The backward passes
+# are launches that record nothing, so where a graph of the gradient itself is asked for (grad mode is on in a backward
+# pass then) they go through the differentiable operators instead, on the tensors that were saved.
 class _GatherFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, plan):
-        ctx.plan = plan
-        return _gather_raw(x, plan)
+    def forward(ctx, x, position, offsets, top_k):
+        ctx.save_for_backward(position, offsets)
+        ctx.top_k = top_k
+        return _gather_raw(x, position, offsets, top_k)
 
     @staticmethod
     def backward(ctx, g):
-        plan = ctx.plan
+        position, offsets = ctx.saved_tensors
+        if not g.is_contiguous():
+            g = g.contiguous()
         if torch.is_grad_enabled():
-            return combine_tokens(g, plan).reshape(plan.n_tokens, -1), None
-        return _combine_raw(g if g.is_contiguous() else g.contiguous(), plan, None, g.dtype), None
+            return _combine(g, None, position, offsets, None, ctx.top_k), None, None, None
+        return _combine_raw(g, None, position, offsets, ctx.top_k, g.dtype), None, None, None
+
+
+def _gather(x, position, offsets, top_k):
+    if x.requires_grad:
+        return _GatherFn.apply(x, position, offsets, top_k)
+    return _gather_raw(x, position, offsets, top_k)
 
 
 def gather_tokens(x, plan):
     """The tokens' rows in sorted order: ``x`` ``[T, K]`` (or ``[..., K]``) -> ``[T * top_k, K]``; rows of pairs that
     go nowhere are zero.  The gradient adds up a token's copies in fp32 and rounds once."""
     x = _rows_of(_float_tensor(x), plan.n_tokens, plan, "x")
-    return _GatherFn.apply(x, plan) if x.requires_grad else _gather_raw(x, plan)
+    return _gather(x, plan.position, plan.offsets, plan.top_k)
 
 
 class _CombineFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, y, weights, plan):
-        ctx.plan = plan
-        ctx.save_for_backward(y, weights)
-        return _combine_raw(y, plan, weights, y.dtype)
+    def forward(ctx, y, weights, position, offsets, order, top_k):
+        ctx.save_for_backward(y, weights, position, offsets, order)
+        ctx.top_k = top_k
+        return _combine_raw(y, weights, position, offsets, top_k, y.dtype)
 
     @staticmethod
     def backward(ctx, g):
-        y, weights = ctx.saved_tensors
-        plan = ctx.plan
-        if torch.is_grad_enabled():
-            return _combine_grad_graph(y, weights, g, plan) + (None,)
+        y, weights, position, offsets, order = ctx.saved_tensors
         if not g.is_contiguous():
             g = g.contiguous()
+        if torch.is_grad_enabled():
+            return _combine_grad_graph(y, weights, g, position, offsets, order, ctx.top_k) + (None,) * 4
         dy = torch.empty_like(y) if ctx.needs_input_grad[0] else None
         dw = torch.empty_like(weights) if ctx.needs_input_grad[1] else None
         _launch(N.load().gptq_hip_expert_combine_grad, y.get_device(), "expert_combine_grad", y.data_ptr(), g.data_ptr(),
-                _DT[y.dtype], plan.n_tokens, plan.top_k, y.shape[1], plan.position.data_ptr(),
-                plan.offsets.data_ptr(), plan.n_experts, None if weights is None else weights.data_ptr(),
+                _DT[y.dtype], g.shape[0], ctx.top_k, y.shape[1], position.data_ptr(), offsets.data_ptr(),
+                offsets.numel() - 1, None if weights is None else weights.data_ptr(),
                 N.F32 if weights is None else _DT[weights.dtype], None if dy is None else dy.data_ptr(),
                 None if dw is None else dw.data_ptr())
-        return dy, dw, None
+        return dy, dw, None, None, None, None
 
 
-def _combine_grad_graph(y, weights, g, plan):
+def _combine_grad_graph(y, weights, g, position, offsets, order, top_k):
     """The gradients of ``combine_tokens`` as differentiable operations."""
-    rows = gather_tokens(g, plan)
+    rows = _gather(g, position, offsets, top_k)
     if weights is None:
         return rows, None
-    live = (torch.arange(plan.n_rows, device=y.device) < plan.offsets[-1])[:, None]
-    sorted_weights = weights.reshape(-1)[plan.order.long()][:, None].float()
+    live = (torch.arange(position.numel(), device=y.device) < offsets[-1])[:, None]
+    sorted_weights = weights.reshape(-1)[order.long()][:, None].float()
     dy = torch.where(live, rows.float() * sorted_weights, 0.0).to(y.dtype)
     dots = torch.where(live, rows.float() * y.float(), 0.0).sum(dim=1)
-    return dy, dots[plan.position.long()].reshape(weights.shape).to(weights.dtype)
+    return dy, dots[position.long()].reshape(weights.shape).to(weights.dtype)
+
+
+def _combine(y, weights, position, offsets, order, top_k):
+    if y.requires_grad or (weights is not None and weights.requires_grad):
+        return _CombineFn.apply(y, weights, position, offsets, order, top_k)
+    return _combine_raw(y, weights, position, offsets, top_k, y.dtype)
 
 
 def combine_tokens(y, plan, weights=None):
@@ -283,17 +298,14 @@ def combine_tokens(y, plan, weights=None):
         weights = _on_device(_float_tensor(weights), plan.order, "weights")
         if weights.numel() != plan.n_rows or (weights.shape[-1] != plan.top_k if weights.dim() > 1 else plan.top_k > 1):
             raise ValueError(f"weights must be [..., {plan.top_k}] with one row per token")
-    if y.requires_grad or (weights is not None and weights.requires_grad):
-        out = _CombineFn.apply(y, weights, plan)
-    else:
-        out = _combine_raw(y, plan, weights, y.dtype)
+    out = _combine(y, weights, plan.position, plan.offsets, plan.order, plan.top_k)
     return out if len(plan.token_shape) == 1 else out.reshape(plan.token_shape + (y.size(1),))
 
 
-def _expert_matmul_raw(x, packed, zero, scale, bits, group, plan, sorted_rows, transpose_b, out_dtype):
+def _expert_matmul_raw(x, packed, zero, scale, order, offsets, top_k, bits, group, sorted_rows, transpose_b, out_dtype):
     lib = N.load()
     E, R, C = packed.shape
-    x_rows, x_dtype, n_rows = x.size(0), _DT[x.dtype], plan.n_rows
+    x_rows, x_dtype, n_rows = x.size(0), _DT[x.dtype], order.numel()
     out = x.new_empty((n_rows, R * (8 // bits) if transpose_b else C), dtype=out_dtype)
     if transpose_b and x.data_ptr() % 16:
         x = x.clone()           # (the transposed kernels load 16 bytes at a time)
@@ -301,31 +313,44 @@ def _expert_matmul_raw(x, packed, zero, scale, bits, group, plan, sorted_rows, t
                                                          transpose_b)
     ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     _launch(lib.gptq_hip_expert_qmatmul, x.get_device(), "expert_qmatmul", x.data_ptr(), x_dtype, x_rows,
-            None if sorted_rows else plan.order.data_ptr(), plan.top_k, n_rows, plan.offsets.data_ptr(), E,
-            packed.data_ptr(), R, C, zero.data_ptr(), scale.data_ptr(), _DT[zero.dtype], group, bits, transpose_b,
-            out.data_ptr(), _DT[out_dtype], ws.data_ptr() if nbytes else None, nbytes)
+            None if sorted_rows else order.data_ptr(), top_k, n_rows, offsets.data_ptr(), E, packed.data_ptr(), R, C,
+            zero.data_ptr(), scale.data_ptr(), _DT[zero.dtype], group, bits, transpose_b, out.data_ptr(), _DT[out_dtype],
+            ws.data_ptr() if nbytes else None, nbytes)
     return out
 
 
 class _ExpertMatmulFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, experts, packed, zero, scale, plan, sorted_rows, transpose_b):
-        ctx.rest = (experts, packed, zero, scale, plan, sorted_rows, transpose_b)
-        return _expert_matmul_raw(x, packed, zero, scale, experts.bits, experts.group_size, plan, sorted_rows,
-                                  transpose_b, x.dtype)
+    def forward(ctx, x, packed, zero, scale, order, position, offsets, top_k, bits, group, sorted_rows, transpose_b):
+        ctx.save_for_backward(packed, zero, scale, order, position, offsets)
+        ctx.rest = (top_k, bits, group, sorted_rows, transpose_b)
+        return _expert_matmul_raw(x, packed, zero, scale, order, offsets, top_k, bits, group, sorted_rows, transpose_b,
+                                  x.dtype)
 
     @staticmethod
     def backward(ctx, g):
-        experts, packed, zero, scale, plan, sorted_rows, transpose_b = ctx.rest
+        packed, zero, scale, order, position, offsets = ctx.saved_tensors
+        top_k, bits, group, sorted_rows, transpose_b = ctx.rest
+        if not g.is_contiguous():
+            g = g.contiguous()
         if torch.is_grad_enabled():
-            dx = quantized_expert_matmul(g, experts, plan, sorted_rows=True, transpose_b=not transpose_b)
-            return (dx if sorted_rows else combine_tokens(dx, plan).reshape(plan.n_tokens, -1),) + (None,) * 7
+            dx = _expert_matmul(g, packed, zero, scale, order, position, offsets, top_k, bits, group, True,
+                                not transpose_b)
+            return (dx if sorted_rows else _combine(dx, None, position, offsets, order, top_k),) + (None,) * 11
         # a token's copies are added up before the one rounding: their gradients travel in fp32
-        dx = _expert_matmul_raw(g.contiguous(), packed, zero, scale, experts.bits, experts.group_size, plan, True,
-                                not transpose_b, g.dtype if sorted_rows else torch.float32)
+        dx = _expert_matmul_raw(g, packed, zero, scale, order, offsets, top_k, bits, group, True, not transpose_b,
+                                g.dtype if sorted_rows else torch.float32)
         if not sorted_rows:
-            dx = _combine_raw(dx, plan, None, g.dtype)
-        return (dx,) + (None,) * 7
+            dx = _combine_raw(dx, None, position, offsets, top_k, g.dtype)
+        return (dx,) + (None,) * 11
+
+
+def _expert_matmul(x, packed, zero, scale, order, position, offsets, top_k, bits, group, sorted_rows, transpose_b):
+    if x.requires_grad:
+        return _ExpertMatmulFn.apply(x, packed, zero, scale, order, position, offsets, top_k, bits, group, sorted_rows,
+                                     transpose_b)
+    return _expert_matmul_raw(x, packed, zero, scale, order, offsets, top_k, bits, group, sorted_rows, transpose_b,
+                              x.dtype)
 
 
 def quantized_expert_matmul(x, experts, plan, sorted_rows=False, transpose_b=False):
@@ -353,10 +378,8 @@ def quantized_expert_matmul(x, experts, plan, sorted_rows=False, transpose_b=Fal
     scale = _on_device(experts.scale, x, "scale")
     if scale.dtype != zero.dtype:           # the kernels read both in one type: fp32 holds either
         zero, scale = zero.float(), scale.float()
-    if x.requires_grad:
-        return _ExpertMatmulFn.apply(x, experts, packed, zero, scale, plan, bool(sorted_rows), bool(transpose_b))
-    return _expert_matmul_raw(x, packed, zero, scale, experts.bits, experts.group_size, plan, bool(sorted_rows),
-                              bool(transpose_b), x.dtype)
+    return _expert_matmul(x, packed, zero, scale, plan.order, plan.position, plan.offsets, plan.top_k, experts.bits,
+                          experts.group_size, bool(sorted_rows), bool(transpose_b))
 
 
 def gptq_experts(W, xs, expert_ids, bits=4, **options):
