@@ -214,9 +214,9 @@ def _gather_raw(x, position, offsets, top_k):
     return out
 
 
-# What a backward pass reads is saved by the graph, which refuses tensors that were written to since.  The backward passes
-# are launches that record nothing, so where a graph of the gradient itself is asked for (grad mode is on in a backward
-# pass then) they go through the differentiable operators instead, on the tensors that were saved.
+# What a backward pass reads is saved by the graph, which refuses tensors that were written to since.  A backward pass is
+# made of operators that can be differentiated themselves: where a graph of the gradient is asked for (grad mode is on
+# then) they record one, else they are plain launches; the gradient has the same bits either way.
 class _GatherFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, position, offsets, top_k):
@@ -230,7 +230,7 @@ class _GatherFn(torch.autograd.Function):
         if not g.is_contiguous():
             g = g.contiguous()
         if torch.is_grad_enabled():
-            return _combine(g, None, position, offsets, None, ctx.top_k), None, None, None
+            return _combine(g, None, position, offsets, ctx.top_k, g.dtype), None, None, None
         return _combine_raw(g, None, position, offsets, ctx.top_k, g.dtype), None, None, None
 
 
@@ -249,44 +249,61 @@ def gather_tokens(x, plan):
 
 class _CombineFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, y, weights, position, offsets, order, top_k):
-        ctx.save_for_backward(y, weights, position, offsets, order)
+    def forward(ctx, y, weights, position, offsets, top_k, out_dtype):
+        ctx.save_for_backward(y, weights, position, offsets)
         ctx.top_k = top_k
-        return _combine_raw(y, weights, position, offsets, top_k, y.dtype)
+        return _combine_raw(y, weights, position, offsets, top_k, out_dtype)
 
     @staticmethod
     def backward(ctx, g):
-        y, weights, position, offsets, order = ctx.saved_tensors
+        y, weights, position, offsets = ctx.saved_tensors
+        g = g.to(y.dtype)
         if not g.is_contiguous():
             g = g.contiguous()
         if torch.is_grad_enabled():
-            return _combine_grad_graph(y, weights, g, position, offsets, order, ctx.top_k) + (None,) * 4
-        dy = torch.empty_like(y) if ctx.needs_input_grad[0] else None
-        dw = torch.empty_like(weights) if ctx.needs_input_grad[1] else None
-        _launch(N.load().gptq_hip_expert_combine_grad, y.get_device(), "expert_combine_grad", y.data_ptr(), g.data_ptr(),
-                _DT[y.dtype], g.shape[0], ctx.top_k, y.shape[1], position.data_ptr(), offsets.data_ptr(),
-                offsets.numel() - 1, None if weights is None else weights.data_ptr(),
-                N.F32 if weights is None else _DT[weights.dtype], None if dy is None else dy.data_ptr(),
-                None if dw is None else dw.data_ptr())
-        return dy, dw, None, None, None, None
+            if weights is None:
+                return (_gather(g, position, offsets, ctx.top_k),) + (None,) * 5
+            return _CombineGradFn.apply(y, weights, g, position, offsets, ctx.top_k) + (None,) * 4
+        return _combine_grad_raw(y, weights, g, position, offsets, ctx.top_k, *ctx.needs_input_grad[:2]) + (None,) * 4
 
 
-def _combine_grad_graph(y, weights, g, position, offsets, order, top_k):
-    """The gradients of ``combine_tokens`` as differentiable operations."""
-    rows = _gather(g, position, offsets, top_k)
-    if weights is None:
-        return rows, None
-    live = (torch.arange(position.numel(), device=y.device) < offsets[-1])[:, None]
-    sorted_weights = weights.reshape(-1)[order.long()][:, None].float()
-    dy = torch.where(live, rows.float() * sorted_weights, 0.0).to(y.dtype)
-    dots = torch.where(live, rows.float() * y.float(), 0.0).sum(dim=1)
-    return dy, dots[position.long()].reshape(weights.shape).to(weights.dtype)
+def _combine_grad_raw(y, weights, g, position, offsets, top_k, want_y=True, want_weights=True):
+    dy = torch.empty_like(y) if want_y else None
+    dw = torch.empty_like(weights) if want_weights else None
+    _launch(N.load().gptq_hip_expert_combine_grad, y.get_device(), "expert_combine_grad", y.data_ptr(), g.data_ptr(),
+            _DT[y.dtype], g.shape[0], top_k, y.shape[1], position.data_ptr(), offsets.data_ptr(), offsets.numel() - 1,
+            None if weights is None else weights.data_ptr(), N.F32 if weights is None else _DT[weights.dtype],
+            None if dy is None else dy.data_ptr(), None if dw is None else dw.data_ptr())
+    return dy, dw
 
 
-def _combine(y, weights, position, offsets, order, top_k):
+class _CombineGradFn(torch.autograd.Function):
+    """dy[p] = w[t, j] g[t] and dw[t, j] = <g[t], y[p]> for the pair (t, j) of row p, to be differentiated again: with
+    ey, ew in the places of their gradients, y gets ew g and w gets <g, ey>, which is the same operator, and g the sum
+    of w ey + ew y over the pairs of a token."""
+
+    @staticmethod
+    def forward(ctx, y, weights, g, position, offsets, top_k):
+        ctx.save_for_backward(y, weights, g, position, offsets)
+        ctx.top_k = top_k
+        return _combine_grad_raw(y, weights, g, position, offsets, top_k)
+
+    @staticmethod
+    def backward(ctx, ey, ew):
+        y, weights, g, position, offsets = ctx.saved_tensors
+        top_k, ey, ew = ctx.top_k, ey.contiguous(), ew.contiguous()
+        dg = _combine(ey, weights, position, offsets, top_k, g.dtype) + _combine(y, ew, position, offsets, top_k, g.dtype)
+        if torch.is_grad_enabled():
+            dy, dw = _CombineGradFn.apply(ey, ew, g, position, offsets, top_k)
+        else:
+            dy, dw = _combine_grad_raw(ey, ew, g, position, offsets, top_k)
+        return dy, dw, dg, None, None, None
+
+
+def _combine(y, weights, position, offsets, top_k, out_dtype):
     if y.requires_grad or (weights is not None and weights.requires_grad):
-        return _CombineFn.apply(y, weights, position, offsets, order, top_k)
-    return _combine_raw(y, weights, position, offsets, top_k, y.dtype)
+        return _CombineFn.apply(y, weights, position, offsets, top_k, out_dtype)
+    return _combine_raw(y, weights, position, offsets, top_k, out_dtype)
 
 
 def combine_tokens(y, plan, weights=None):
@@ -298,7 +315,7 @@ def combine_tokens(y, plan, weights=None):
         weights = _on_device(_float_tensor(weights), plan.order, "weights")
         if weights.numel() != plan.n_rows or (weights.shape[-1] != plan.top_k if weights.dim() > 1 else plan.top_k > 1):
             raise ValueError(f"weights must be [..., {plan.top_k}] with one row per token")
-    out = _combine(y, weights, plan.position, plan.offsets, plan.order, plan.top_k)
+    out = _combine(y, weights, plan.position, plan.offsets, plan.top_k, y.dtype)
     return out if len(plan.token_shape) == 1 else out.reshape(plan.token_shape + (y.size(1),))
 
 
@@ -321,36 +338,33 @@ def _expert_matmul_raw(x, packed, zero, scale, order, offsets, top_k, bits, grou
 
 class _ExpertMatmulFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, packed, zero, scale, order, position, offsets, top_k, bits, group, sorted_rows, transpose_b):
+    def forward(ctx, x, packed, zero, scale, order, position, offsets, top_k, bits, group, sorted_rows, transpose_b,
+                out_dtype):
         ctx.save_for_backward(packed, zero, scale, order, position, offsets)
-        ctx.rest = (top_k, bits, group, sorted_rows, transpose_b)
+        ctx.rest = (top_k, bits, group, sorted_rows, transpose_b, x.dtype)
         return _expert_matmul_raw(x, packed, zero, scale, order, offsets, top_k, bits, group, sorted_rows, transpose_b,
-                                  x.dtype)
+                                  out_dtype)
 
     @staticmethod
     def backward(ctx, g):
         packed, zero, scale, order, position, offsets = ctx.saved_tensors
-        top_k, bits, group, sorted_rows, transpose_b = ctx.rest
+        top_k, bits, group, sorted_rows, transpose_b, dtype = ctx.rest
         if not g.is_contiguous():
             g = g.contiguous()
-        if torch.is_grad_enabled():
-            dx = _expert_matmul(g, packed, zero, scale, order, position, offsets, top_k, bits, group, True,
-                                not transpose_b)
-            return (dx if sorted_rows else _combine(dx, None, position, offsets, order, top_k),) + (None,) * 11
         # a token's copies are added up before the one rounding: their gradients travel in fp32
-        dx = _expert_matmul_raw(g, packed, zero, scale, order, offsets, top_k, bits, group, True, not transpose_b,
-                                g.dtype if sorted_rows else torch.float32)
-        if not sorted_rows:
-            dx = _combine_raw(dx, None, position, offsets, top_k, g.dtype)
-        return (dx,) + (None,) * 11
+        dx = _expert_matmul(g, packed, zero, scale, order, position, offsets, top_k, bits, group, True, not transpose_b,
+                            g.dtype if sorted_rows else torch.float32)
+        dx = dx.to(dtype) if sorted_rows else _combine(dx, None, position, offsets, top_k, dtype)
+        return (dx,) + (None,) * 12
 
 
-def _expert_matmul(x, packed, zero, scale, order, position, offsets, top_k, bits, group, sorted_rows, transpose_b):
+def _expert_matmul(x, packed, zero, scale, order, position, offsets, top_k, bits, group, sorted_rows, transpose_b,
+                   out_dtype):
     if x.requires_grad:
         return _ExpertMatmulFn.apply(x, packed, zero, scale, order, position, offsets, top_k, bits, group, sorted_rows,
-                                     transpose_b)
+                                     transpose_b, out_dtype)
     return _expert_matmul_raw(x, packed, zero, scale, order, offsets, top_k, bits, group, sorted_rows, transpose_b,
-                              x.dtype)
+                              out_dtype)
 
 
 def quantized_expert_matmul(x, experts, plan, sorted_rows=False, transpose_b=False):
@@ -379,7 +393,7 @@ def quantized_expert_matmul(x, experts, plan, sorted_rows=False, transpose_b=Fal
     if scale.dtype != zero.dtype:           # the kernels read both in one type: fp32 holds either
         zero, scale = zero.float(), scale.float()
     return _expert_matmul(x, packed, zero, scale, plan.order, plan.position, plan.offsets, plan.top_k, experts.bits,
-                          experts.group_size, bool(sorted_rows), bool(transpose_b))
+                          experts.group_size, bool(sorted_rows), bool(transpose_b), x.dtype)
 
 
 def gptq_experts(W, xs, expert_ids, bits=4, **options):
