@@ -12,8 +12,8 @@ picks ``top_k`` for every token.  The pieces, in the order a layer uses them::
 ``W_*`` are :class:`QuantizedExperts`, from :func:`stack_experts` (packed matrices, e.g. of separate ``gptq`` calls)
 or :func:`gptq_experts` (all experts of a layer against the tokens that reach them).  An id outside
 ``0 .. n_experts - 1`` marks a (token, choice) pair that goes nowhere, e.g. padding: its rows stand behind the last
-expert's, are zero, and add nothing.  Differentiable with respect to activations and router weights; the packed
-matrices are frozen, as in ``quantized_matmul``.  Nothing here waits for the GPU, so everything but
+expert's, are zero, and add nothing.  Differentiable with respect to activations and router weights, in reverse mode
+(forward mode raises); the packed matrices are frozen, as in ``quantized_matmul``.  Nothing here waits for the GPU, so everything but
 ``gptq_experts`` can be captured into a HIP graph.  As with any torch operator, capture a backward pass with leaves
 that no eager graph still refers to.
 """
@@ -22,7 +22,7 @@ from __future__ import annotations
 import torch
 
 from . import _native as N
-from .gptq import _DT, QuantizedMatrix, _dev, _float_dev, gptq, pack_matrix
+from .gptq import _DT, QuantizedMatrix, _dev, _differentiated, _float_dev, gptq, pack_matrix
 
 __all__ = ["QuantizedExperts", "TokenPlan", "stack_experts", "gptq_experts", "sort_tokens", "gather_tokens",
            "combine_tokens", "quantized_expert_matmul"]
@@ -235,7 +235,7 @@ class _GatherFn(torch.autograd.Function):
 
 
 def _gather(x, position, offsets, top_k):
-    if x.requires_grad:
+    if _differentiated(x):
         return _GatherFn.apply(x, position, offsets, top_k)
     return _gather_raw(x, position, offsets, top_k)
 
@@ -301,7 +301,7 @@ class _CombineGradFn(torch.autograd.Function):
 
 
 def _combine(y, weights, position, offsets, top_k, out_dtype):
-    if y.requires_grad or (weights is not None and weights.requires_grad):
+    if _differentiated(y) or (weights is not None and _differentiated(weights)):
         return _CombineFn.apply(y, weights, position, offsets, top_k, out_dtype)
     return _combine_raw(y, weights, position, offsets, top_k, out_dtype)
 
@@ -360,7 +360,7 @@ class _ExpertMatmulFn(torch.autograd.Function):
 
 def _expert_matmul(x, packed, zero, scale, order, position, offsets, top_k, bits, group, sorted_rows, transpose_b,
                    out_dtype):
-    if x.requires_grad:
+    if _differentiated(x):
         return _ExpertMatmulFn.apply(x, packed, zero, scale, order, position, offsets, top_k, bits, group, sorted_rows,
                                      transpose_b, out_dtype)
     return _expert_matmul_raw(x, packed, zero, scale, order, offsets, top_k, bits, group, sorted_rows, transpose_b,

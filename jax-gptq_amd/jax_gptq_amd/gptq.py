@@ -61,6 +61,12 @@ def _float_dev(x, keep_fp64=False):
     return t
 
 
+def _differentiated(t):
+    """Whether autograd follows ``t``, in either mode.  A tensor with a tangent (forward mode) does not require a
+    gradient; a launch would lose the tangent without a word, an autograd function without a ``jvp`` raises."""
+    return t.requires_grad or torch.autograd.forward_ad.unpack_dual(t).tangent is not None
+
+
 def _stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 

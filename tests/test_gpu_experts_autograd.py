@@ -179,3 +179,17 @@ def test_second_and_third_derivatives(X, name, dt):
         largest = want.abs().max()
         step = half * largest.clamp_min(torch.finfo(dt).smallest_normal)
         assert (got - want).abs().max() <= 4 * (order_of + 1) * step + 2.0 ** -14 * largest, n
+
+
+# ------------------------------------------------------------------------------------ forward mode
+@pytest.mark.parametrize("name", NAMES)
+def test_forward_mode_is_refused(X, name):
+    """A tangent is not lost without a word."""
+    import torch.autograd.forward_ad as forward
+    f, x, _ = operators(X)[name]
+    plan = X.sort_tokens(ids_of(0, T, TOP_K, E).cuda(), E)
+    want = f(x, plan)
+    with forward.dual_level():
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            f(forward.make_dual(x, torch.ones_like(x)), plan)
+        assert torch.equal(f(x, plan), want)        # without a tangent: as ever
