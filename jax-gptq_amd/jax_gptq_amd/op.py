@@ -3,8 +3,9 @@
 ``quantized_matmul(x, quantized_matrix, transpose_b=False)`` flattens the leading
 dimensions of ``x``, launches the packed-int4 HIP kernel (the counterpart of the
 ``jt.triton_call`` at ``op.py:46-63``) and restores the shape.  Like the reference's
-``custom_vjp`` (``op.py:71-81``) it is differentiable with respect to ``x`` only: the
-backward pass is the same operator with ``transpose_b`` flipped.
+``custom_vjp`` (``op.py:71-81``) it is differentiable with respect to ``x`` only and in
+reverse mode only (forward mode raises): the backward pass is the same operator with
+``transpose_b`` flipped.
 """
 from __future__ import annotations
 
@@ -13,7 +14,7 @@ import ctypes
 import torch
 
 from . import _native as N
-from .gptq import _DT, _float_dev, _dev, _ptr, _stream, _ws
+from .gptq import _DT, _differentiated, _float_dev, _dev, _ptr, _stream, _ws
 
 
 # The matmul workspace starts with split-K arrival counters that must be zero when a call
@@ -101,7 +102,7 @@ def _quantized_matmul(x, quantized_matrix, transpose_b):
     if bits not in (4, 8):
         raise ValueError("quantized_matmul takes 4-bit or 8-bit codes")
     group = int(getattr(quantized_matrix, "group_size", 0) or 0)
-    if x.requires_grad:
+    if _differentiated(x):
         return _QuantizedMatmulFn.apply(x, iw, zero, scale, bool(transpose_b), bits, group)
     return _quantized_matmul_raw(x, iw, zero, scale, bool(transpose_b), bits, group)
 
