@@ -1,4 +1,4 @@
-"""Builds libgptq_hip.so (gfx950 only) next to the Python package.
+"""Builds libgptq_hip.so (gfx950 only) next to the Python package, and the autograd nodes for torch over it.
 
     python jax-gptq_amd/build.py [--force]
 
@@ -29,13 +29,32 @@ def _hipcc():
     return "hipcc"
 
 
+TORCH_SHIM = os.path.join(OUT_DIR, "_torch_experts.so")
+
+
 def needs_build():
-    if not os.path.exists(LIB):
+    if not os.path.exists(LIB) or not os.path.exists(TORCH_SHIM):
         return True
-    t = os.path.getmtime(LIB)
+    t = min(os.path.getmtime(LIB), os.path.getmtime(TORCH_SHIM))
     deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)]
     deps.append(os.path.join(HERE, "..", "include", "gptq_hip.h"))
     return any(os.path.getmtime(d) > t for d in deps)
+
+
+def torch_shim_command():
+    """The host compiler's command for csrc/torch_experts.cc, against the torch that is installed.  It names no symbol of
+    libgptq_hip.so: the package hands it the entry points of the library that it loads."""
+    import sysconfig
+    import torch
+    home = os.path.dirname(torch.__file__)
+    include = [os.path.join(home, "include"), os.path.join(home, "include", "torch", "csrc", "api", "include"),
+               os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_hipcc()))), "include"),
+               sysconfig.get_paths()["include"]]
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+            "-DTORCH_EXTENSION_NAME=_torch_experts", "-DTORCH_API_INCLUDE_EXTENSION_H", "-D__HIP_PLATFORM_AMD__=1",
+            "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+            *[a for d in include for a in ("-isystem", d)], os.path.join(CSRC, "torch_experts.cc"), "-o", TORCH_SHIM,
+            "-L", os.path.join(home, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
 
 
 def build(force=False, verbose=True):
@@ -51,6 +70,8 @@ def build(force=False, verbose=True):
         objs.append(obj)
         cmd = [hipcc, *FLAGS, "-c", os.path.join(CSRC, src), "-o", obj]
         procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
+    procs.append(("torch_experts.cc", subprocess.Popen(torch_shim_command(), stdout=subprocess.PIPE,
+                                                       stderr=subprocess.STDOUT)))
     failed = False
     for src, p in procs:
         out = p.communicate()[0].decode()
@@ -61,11 +82,11 @@ def build(force=False, verbose=True):
         elif verbose and out.strip():
             sys.stderr.write(f"[build] {src}:\n{out}\n")
     if failed:
-        raise RuntimeError("hipcc failed")
+        raise RuntimeError("a compiler failed")
     cmd = [hipcc, "-shared", "--offload-arch=gfx950", "-fPIC", *objs, "-o", LIB]
     subprocess.check_call(cmd)
     if verbose:
-        print(f"[build] wrote {LIB}")
+        print(f"[build] wrote {LIB} and {TORCH_SHIM}")
     return LIB
 
 

@@ -116,6 +116,26 @@ def load():
     return lib
 
 
+_torch = None
+
+
+def load_torch():
+    """The autograd nodes of the experts' operators (csrc/torch_experts.cc) on the library's entry points; built with the
+    library and loaded by the first call of such an operator."""
+    global _torch
+    if _torch is None:
+        lib = load()
+        try:
+            from . import _torch_experts
+        except ImportError as e:
+            raise ImportError("jax_gptq_amd/_torch_experts.so is missing or does not fit this torch: build it with "
+                              "`python jax-gptq_amd/build.py`") from e
+        _torch_experts.bind({name: ctypes.cast(getattr(lib, name), _vp).value for name in SIGNATURES
+                             if name == "gptq_hip_error_string" or name.startswith("gptq_hip_expert_")})
+        _torch = _torch_experts
+    return _torch
+
+
 def check(code, what):
     """Map a status code to the exception type the reference raises in that situation."""
     if code == OK:

@@ -22,29 +22,12 @@ from __future__ import annotations
 import torch
 
 from . import _native as N
-from .gptq import _DT, QuantizedMatrix, _dev, _differentiated, _float_dev, gptq, pack_matrix
+from .gptq import _DT, QuantizedMatrix, _dev, _float_dev, gptq, pack_matrix
 
 __all__ = ["QuantizedExperts", "TokenPlan", "stack_experts", "gptq_experts", "sort_tokens", "gather_tokens",
            "combine_tokens", "quantized_expert_matmul"]
 
 MAX_EXPERTS = 1024
-
-
-# A call's share of the host is what a small one takes, and a backward pass runs this on the engine's thread, where
-# every Python step takes twice as long: so no objects for streams and devices (2 us a call) in here.
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current = torch._C._cuda_getDevice
-
-
-def _launch(entry, index, what, *args):
-    """Calls a C entry point on the current stream of GPU ``index``; pointers are passed as integers."""
-    if index == _current():
-        code = entry(_raw_stream(index), *args)
-    else:
-        with torch.cuda.device(index):
-            code = entry(_raw_stream(index), *args)
-    if code:
-        N.check(code, what)
 
 
 def _on_device(t, like, what):
@@ -175,12 +158,7 @@ def sort_tokens(expert_ids, n_experts):
     if top_k == 0:
         raise ValueError("at least one choice per token")
     ids = ids.contiguous()
-    P, lib = ids.numel(), N.load()
-    order, position, offsets = ids.new_empty(2 * P + n_experts + 1, dtype=torch.int32).split((P, P, n_experts + 1))
-    nbytes = lib.gptq_hip_expert_sort_workspace_bytes(P, n_experts)
-    ws = ids.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    _launch(lib.gptq_hip_expert_sort, ids.get_device(), "expert_sort", ids.data_ptr(), ids.element_size(), P, n_experts,
-            order.data_ptr(), position.data_ptr(), offsets.data_ptr(), ws.data_ptr() if nbytes else None, nbytes)
+    order, position, offsets = N.load_torch().sort(ids, n_experts)
     return TokenPlan(order, position, offsets, ids.shape[:-1], top_k, n_experts)
 
 
@@ -196,114 +174,11 @@ def _rows_of(x, rows, plan, what):
     return x if dims == 2 else x.reshape(rows, width)
 
 
-def _combine_raw(y, weights, position, offsets, top_k, out_dtype):
-    width, tokens = y.size(1), position.numel() // top_k
-    out = y.new_empty((tokens, width), dtype=out_dtype)
-    w, w_dtype = (None, N.F32) if weights is None else (weights.data_ptr(), _DT[weights.dtype])
-    _launch(N.load().gptq_hip_expert_combine, y.get_device(), "expert_combine", y.data_ptr(), _DT[y.dtype], tokens,
-            top_k, width, position.data_ptr(), offsets.data_ptr(), offsets.numel() - 1, w, w_dtype, out.data_ptr(),
-            _DT[out_dtype])
-    return out
-
-
-def _gather_raw(x, position, offsets, top_k):
-    tokens, width = x.shape
-    out = x.new_empty((tokens * top_k, width))
-    _launch(N.load().gptq_hip_expert_gather, x.get_device(), "expert_gather", x.data_ptr(), _DT[x.dtype], tokens,
-            top_k, width, position.data_ptr(), offsets.data_ptr(), offsets.numel() - 1, out.data_ptr())
-    return out
-
-
-# What a backward pass reads is saved by the graph, which refuses tensors that were written to since.  A backward pass is
-# made of operators that can be differentiated themselves: where a graph of the gradient is asked for (grad mode is on
-# then) they record one, else they are plain launches; the gradient has the same bits either way.
-class _GatherFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, position, offsets, top_k):
-        ctx.save_for_backward(position, offsets)
-        ctx.top_k = top_k
-        return _gather_raw(x, position, offsets, top_k)
-
-    @staticmethod
-    def backward(ctx, g):
-        position, offsets = ctx.saved_tensors
-        if not g.is_contiguous():
-            g = g.contiguous()
-        if torch.is_grad_enabled():
-            return _combine(g, None, position, offsets, ctx.top_k, g.dtype), None, None, None
-        return _combine_raw(g, None, position, offsets, ctx.top_k, g.dtype), None, None, None
-
-
-def _gather(x, position, offsets, top_k):
-    if _differentiated(x):
-        return _GatherFn.apply(x, position, offsets, top_k)
-    return _gather_raw(x, position, offsets, top_k)
-
-
 def gather_tokens(x, plan):
     """The tokens' rows in sorted order: ``x`` ``[T, K]`` (or ``[..., K]``) -> ``[T * top_k, K]``; rows of pairs that
     go nowhere are zero.  The gradient adds up a token's copies in fp32 and rounds once."""
     x = _rows_of(_float_tensor(x), plan.n_tokens, plan, "x")
-    return _gather(x, plan.position, plan.offsets, plan.top_k)
-
-
-class _CombineFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, y, weights, position, offsets, top_k, out_dtype):
-        ctx.save_for_backward(y, weights, position, offsets)
-        ctx.top_k = top_k
-        return _combine_raw(y, weights, position, offsets, top_k, out_dtype)
-
-    @staticmethod
-    def backward(ctx, g):
-        y, weights, position, offsets = ctx.saved_tensors
-        g = g.to(y.dtype)
-        if not g.is_contiguous():
-            g = g.contiguous()
-        if torch.is_grad_enabled():
-            if weights is None:
-                return (_gather(g, position, offsets, ctx.top_k),) + (None,) * 5
-            return _CombineGradFn.apply(y, weights, g, position, offsets, ctx.top_k) + (None,) * 4
-        return _combine_grad_raw(y, weights, g, position, offsets, ctx.top_k, *ctx.needs_input_grad[:2]) + (None,) * 4
-
-
-def _combine_grad_raw(y, weights, g, position, offsets, top_k, want_y=True, want_weights=True):
-    dy = torch.empty_like(y) if want_y else None
-    dw = torch.empty_like(weights) if want_weights else None
-    _launch(N.load().gptq_hip_expert_combine_grad, y.get_device(), "expert_combine_grad", y.data_ptr(), g.data_ptr(),
-            _DT[y.dtype], g.shape[0], top_k, y.shape[1], position.data_ptr(), offsets.data_ptr(), offsets.numel() - 1,
-            None if weights is None else weights.data_ptr(), N.F32 if weights is None else _DT[weights.dtype],
-            None if dy is None else dy.data_ptr(), None if dw is None else dw.data_ptr())
-    return dy, dw
-
-
-class _CombineGradFn(torch.autograd.Function):
-    """dy[p] = w[t, j] g[t] and dw[t, j] = <g[t], y[p]> for the pair (t, j) of row p, to be differentiated again: with
-    ey, ew in the places of their gradients, y gets ew g and w gets <g, ey>, which is the same operator, and g the sum
-    of w ey + ew y over the pairs of a token."""
-
-    @staticmethod
-    def forward(ctx, y, weights, g, position, offsets, top_k):
-        ctx.save_for_backward(y, weights, g, position, offsets)
-        ctx.top_k = top_k
-        return _combine_grad_raw(y, weights, g, position, offsets, top_k)
-
-    @staticmethod
-    def backward(ctx, ey, ew):
-        y, weights, g, position, offsets = ctx.saved_tensors
-        top_k, ey, ew = ctx.top_k, ey.contiguous(), ew.contiguous()
-        dg = _combine(ey, weights, position, offsets, top_k, g.dtype) + _combine(y, ew, position, offsets, top_k, g.dtype)
-        if torch.is_grad_enabled():
-            dy, dw = _CombineGradFn.apply(ey, ew, g, position, offsets, top_k)
-        else:
-            dy, dw = _combine_grad_raw(ey, ew, g, position, offsets, top_k)
-        return dy, dw, dg, None, None, None
-
-
-def _combine(y, weights, position, offsets, top_k, out_dtype):
-    if _differentiated(y) or (weights is not None and _differentiated(weights)):
-        return _CombineFn.apply(y, weights, position, offsets, top_k, out_dtype)
-    return _combine_raw(y, weights, position, offsets, top_k, out_dtype)
+    return N.load_torch().gather(x, plan.position, plan.offsets, plan.top_k)
 
 
 def combine_tokens(y, plan, weights=None):
@@ -315,56 +190,8 @@ def combine_tokens(y, plan, weights=None):
         weights = _on_device(_float_tensor(weights), plan.order, "weights")
         if weights.numel() != plan.n_rows or (weights.shape[-1] != plan.top_k if weights.dim() > 1 else plan.top_k > 1):
             raise ValueError(f"weights must be [..., {plan.top_k}] with one row per token")
-    out = _combine(y, weights, plan.position, plan.offsets, plan.top_k, y.dtype)
+    out = N.load_torch().combine(y, weights, plan.position, plan.offsets, plan.top_k)
     return out if len(plan.token_shape) == 1 else out.reshape(plan.token_shape + (y.size(1),))
-
-
-def _expert_matmul_raw(x, packed, zero, scale, order, offsets, top_k, bits, group, sorted_rows, transpose_b, out_dtype):
-    lib = N.load()
-    E, R, C = packed.shape
-    x_rows, x_dtype, n_rows = x.size(0), _DT[x.dtype], order.numel()
-    out = x.new_empty((n_rows, R * (8 // bits) if transpose_b else C), dtype=out_dtype)
-    if transpose_b and x.data_ptr() % 16:
-        x = x.clone()           # (the transposed kernels load 16 bytes at a time)
-    nbytes = lib.gptq_hip_expert_qmatmul_workspace_bytes(x_rows, n_rows, R, C, bits, group, E, x_dtype, _DT[zero.dtype],
-                                                         transpose_b)
-    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    _launch(lib.gptq_hip_expert_qmatmul, x.get_device(), "expert_qmatmul", x.data_ptr(), x_dtype, x_rows,
-            None if sorted_rows else order.data_ptr(), top_k, n_rows, offsets.data_ptr(), E, packed.data_ptr(), R, C,
-            zero.data_ptr(), scale.data_ptr(), _DT[zero.dtype], group, bits, transpose_b, out.data_ptr(), _DT[out_dtype],
-            ws.data_ptr() if nbytes else None, nbytes)
-    return out
-
-
-class _ExpertMatmulFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, packed, zero, scale, order, position, offsets, top_k, bits, group, sorted_rows, transpose_b,
-                out_dtype):
-        ctx.save_for_backward(packed, zero, scale, order, position, offsets)
-        ctx.rest = (top_k, bits, group, sorted_rows, transpose_b, x.dtype)
-        return _expert_matmul_raw(x, packed, zero, scale, order, offsets, top_k, bits, group, sorted_rows, transpose_b,
-                                  out_dtype)
-
-    @staticmethod
-    def backward(ctx, g):
-        packed, zero, scale, order, position, offsets = ctx.saved_tensors
-        top_k, bits, group, sorted_rows, transpose_b, dtype = ctx.rest
-        if not g.is_contiguous():
-            g = g.contiguous()
-        # a token's copies are added up before the one rounding: their gradients travel in fp32
-        dx = _expert_matmul(g, packed, zero, scale, order, position, offsets, top_k, bits, group, True, not transpose_b,
-                            g.dtype if sorted_rows else torch.float32)
-        dx = dx.to(dtype) if sorted_rows else _combine(dx, None, position, offsets, top_k, dtype)
-        return (dx,) + (None,) * 12
-
-
-def _expert_matmul(x, packed, zero, scale, order, position, offsets, top_k, bits, group, sorted_rows, transpose_b,
-                   out_dtype):
-    if _differentiated(x):
-        return _ExpertMatmulFn.apply(x, packed, zero, scale, order, position, offsets, top_k, bits, group, sorted_rows,
-                                     transpose_b, out_dtype)
-    return _expert_matmul_raw(x, packed, zero, scale, order, offsets, top_k, bits, group, sorted_rows, transpose_b,
-                              out_dtype)
 
 
 def quantized_expert_matmul(x, experts, plan, sorted_rows=False, transpose_b=False):
@@ -392,8 +219,8 @@ def quantized_expert_matmul(x, experts, plan, sorted_rows=False, transpose_b=Fal
     scale = _on_device(experts.scale, x, "scale")
     if scale.dtype != zero.dtype:           # the kernels read both in one type: fp32 holds either
         zero, scale = zero.float(), scale.float()
-    return _expert_matmul(x, packed, zero, scale, plan.order, plan.position, plan.offsets, plan.top_k, experts.bits,
-                          experts.group_size, bool(sorted_rows), bool(transpose_b), x.dtype)
+    return N.load_torch().matmul(x, packed, zero, scale, plan.order, plan.position, plan.offsets, plan.top_k, experts.bits,
+                                 experts.group_size, bool(sorted_rows), bool(transpose_b))
 
 
 def gptq_experts(W, xs, expert_ids, bits=4, **options):

@@ -193,3 +193,52 @@ def test_forward_mode_is_refused(X, name):
         with pytest.raises((NotImplementedError, RuntimeError)):
             f(forward.make_dual(x, torch.ones_like(x)), plan)
         assert torch.equal(f(x, plan), want)        # without a tangent: as ever
+
+
+# ------------------------------------------------------------------------------------ the nodes' own duties
+@pytest.mark.parametrize("name", NAMES)
+def test_backward_twice_and_unused_gradients(X, name):
+    f, x, _ = operators(X)[name]
+    plan = X.sort_tokens(ids_of(0, T, TOP_K, E).cuda(), E)
+    x.requires_grad_()
+    out = f(x, plan)
+    want = torch.autograd.grad(out.sum(), x)[0]
+    with pytest.raises(RuntimeError):                       # what it saved is gone, or it saved nothing and agrees
+        again = torch.autograd.grad(out.sum(), x)[0]
+        assert torch.equal(again, want)
+        raise RuntimeError
+    with torch.no_grad():
+        assert not f(x, plan).requires_grad
+    assert not f(x.detach(), plan).requires_grad
+    out = f(x * 1, plan)                                    # an input that is not a leaf
+    out.sum().backward()
+    assert torch.equal(x.grad, want)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_function_transforms_are_right_or_refused(X, name):
+    f, x, _ = operators(X)[name]
+    plan = X.sort_tokens(ids_of(0, T, TOP_K, E).cuda(), E)
+    leaf = x.clone().requires_grad_()
+    want = torch.autograd.grad(f(leaf, plan).sum(), leaf)[0]
+    both = torch.stack([x, 2 * x])
+    for call, right in ((lambda: torch.func.grad(lambda a: f(a, plan).sum())(x), want),
+                        (lambda: torch.func.jvp(lambda a: f(a, plan), (x,), (x,))[1], f(x, plan)),
+                        (lambda: torch.func.vmap(lambda a: f(a, plan))(both), torch.stack([f(x, plan), f(2 * x, plan)]))):
+        try:
+            got = call()
+        except (RuntimeError, NotImplementedError):
+            continue
+        assert torch.equal(got, right)
+
+
+def test_only_the_gradients_that_are_wanted(X):
+    plan = X.sort_tokens(ids_of(0, T, TOP_K, E).cuda(), E)
+    y, w = torch.randn(T * TOP_K, N).cuda(), torch.rand(T, TOP_K).cuda()
+    want = None
+    for need_y, need_w in ((True, True), (True, False), (False, True)):
+        a, b = y.clone().requires_grad_(need_y), w.clone().requires_grad_(need_w)
+        X.combine_tokens(a, plan, b).sum().backward()
+        want = want or (a.grad, b.grad)
+        assert (torch.equal(a.grad, want[0]) if need_y else a.grad is None)
+        assert (torch.equal(b.grad, want[1]) if need_w else b.grad is None)
