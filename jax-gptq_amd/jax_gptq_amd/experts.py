@@ -22,7 +22,7 @@ from __future__ import annotations
 import torch
 
 from . import _native as N
-from .gptq import _DT, QuantizedMatrix, _dev, _float_dev, gptq, pack_matrix
+from .gptq import _DT, QuantizedMatrix, _dev, _float_dev, _ptr, _stream, gptq, pack_matrix
 
 __all__ = ["QuantizedExperts", "TokenPlan", "stack_experts", "gptq_experts", "sort_tokens", "gather_tokens",
            "combine_tokens", "quantized_expert_matmul"]
@@ -223,11 +223,22 @@ def quantized_expert_matmul(x, experts, plan, sorted_rows=False, transpose_b=Fal
                                  experts.group_size, bool(sorted_rows), bool(transpose_b))
 
 
+def _rows_at(x, rows):
+    """Copies of some rows of ``x``."""
+    out = x.new_empty((rows.numel(), x.shape[1]))
+    rows = rows.long()
+    with torch.cuda.device(x.device):
+        N.check(N.load().gptq_hip_gather_rows(_stream(), _ptr(x), _ptr(out), x.element_size(), out.shape[0], x.shape[1],
+                                              _ptr(rows)), "gather_rows")
+    return out
+
+
 def gptq_experts(W, xs, expert_ids, bits=4, **options):
     """The solve for all experts of a layer: ``W`` ``[E, K, N]``, calibration batches ``xs`` ``[..., K]`` and for each
     the router's ids ``[..., top_k]`` -> :class:`QuantizedExperts`.
 
-    Each expert is solved by :func:`gptq` against the rows that reach it (sorted and gathered by the operators above).
+    Each expert is solved by :func:`gptq` against the rows that reach it, copied when its turn comes: one expert's rows are
+    held beside the batches, not ``top_k`` copies of them.
     An expert that no row reaches has no Hessian; it is rounded to its own grid, which is the solve with the identity
     as its Hessian.  ``options`` are those of :func:`gptq` (``block_size``, ``damping``, ``group_size``, ...) but ``H``
     and ``shared``, which are one Hessian for several matrices."""
@@ -242,19 +253,16 @@ def gptq_experts(W, xs, expert_ids, bits=4, **options):
     xs, expert_ids = list(xs), list(expert_ids)
     if len(xs) != len(expert_ids):
         raise ValueError("one tensor of expert ids per calibration batch")
-    rows = [[] for _ in range(E)]
+    routed = []
     for x, ids in zip(xs, expert_ids):
         plan = sort_tokens(ids, E)
-        gathered = gather_tokens(x, plan)
-        if gathered.shape[1] != K:
-            raise ValueError(f"calibration feature dim {gathered.shape[1]} != K={K}")
-        at = plan.offsets.tolist()
-        for e in range(E):
-            if at[e + 1] > at[e]:
-                rows[e].append(gathered[at[e]:at[e + 1]])
+        x = _rows_of(_float_tensor(x), plan.n_tokens, plan, "x")
+        if x.shape[1] != K:
+            raise ValueError(f"calibration feature dim {x.shape[1]} != K={K}")
+        routed.append((x, plan, plan.offsets.tolist()))
     out = []
     for e in range(E):
-        batches = rows[e]
+        batches = [_rows_at(x, plan.order[at[e]:at[e + 1]] // plan.top_k) for x, plan, at in routed if at[e + 1] > at[e]]
         if not batches:
             batches = [torch.eye(K, dtype=torch.float32, device=_dev(W[e]).device)]
         Q, params = gptq(W[e], batches, bits=bits, **options)
