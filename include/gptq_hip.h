@@ -354,7 +354,7 @@ int gptq_hip_expert_combine_grad(void *stream, const void *y, const void *g, int
  * is rounded once to out_dtype (x_dtype or F32).  transpose_b applies the scale to x: 16-bit rows times scale enter as
  * two bf16 parts, which leave out up to 2^-18 of each term.  A row with an infinity or a NaN may be NaN throughout;
  * other rows are untouched by it.  rows < 2^24, K <= 262140, C <= 2^20.  Equal calls give equal bits; the order of a row's sums
- * depends on how many rows every expert has.
+ * depends on `rows` and on how many of them every expert has.
  * ws, 16-byte aligned: gptq_hip_expert_qmatmul_workspace_bytes (contents need no preparation; calls that overlap in
  * time need one each; 0 for sizes that the product refuses).  The first call of a kind on a device raises kernels'
  * limits of LDS: make one before capturing.  Plain kernels, an order of magnitude slower, take groups that are no

@@ -54,8 +54,8 @@ __device__ __forceinline__ float table_value(const char *p, int dtype, int64_t i
 // Codes are exact in either: a 4-bit code sits in the mantissa under the exponent of 64 (fp16: 64 + c) or 128 (bf16:
 // 128 + c), and the offset leaves with the zero point; 8-bit codes, and codes against fp32 parts, where the offset
 // would cost bits of the sum, become c itself.  (The bits of a code are also the subnormal fp16 c 2^-24, one
-// instruction less; but sums of products with subnormals came out with errors of 1e-4 of their size, two thousand
-// times those of the same sums with 64 + c.)
+// instruction less.  Single products of it are exact; sums of 32 to 512 with random rows come out up to 8e-6 of their
+// size off, those with 16 c 2^-24 3e-7 to 9e-7, with c 2e-7 to 9e-7, with 64 + c, its 64 sum x taken off, 2e-6 to 1e-5.)
 template <int XT> struct Op;
 template <> struct Op<GPTQ_HIP_F16> {
   static constexpr int PARTS = 1;

@@ -5,8 +5,8 @@
 // registers) and builds its weight operands in registers from its own 128 channels (lane (l16, g): 8 bytes = 8
 // channels of each packed row that holds its 8 k of the k-step; product tile t8 takes byte t8 of every row).
 //
-// fp16 rows: the weight operand is the RAW codes read as fp16 subnormals, which the MFMA multiplies exactly: a
-// byte permute puts byte t8 into both halves of a register and one mask leaves {lo, hi << 4} = {lo 2^-24,
+// fp16 rows: the weight operand is the RAW codes read as fp16 subnormals, which the MFMA multiplies exactly (sums of
+// such products are up to 8e-6 of their size off, a sixtieth of the rounding to fp16 that follows): a byte permute puts byte t8 into both halves of a register and one mask leaves {lo, hi << 4} = {lo 2^-24,
 // 16 hi 2^-24}: two vector instructions per operand register, no conversion.  The 16 goes to the other operand
 // (the activations of odd k are divided by 16 on their way into LDS, the row sums' operand holds 16 for them);
 // 2^24, the scale and the zero point (- zero sum_k x[m][k], the row sums from a ninth tile) wait for the epilogue.

@@ -206,7 +206,8 @@ def quantized_expert_matmul(x, experts, plan, sorted_rows=False, transpose_b=Fal
     term.  A row of ``x`` with an infinity or a NaN may become NaN throughout, other rows do not see it; so may one whose
     sums of ``x`` times codes over a group, which come before the scale, or, transposed, of ``x`` times scale times codes
     leave fp32's range.  Equal calls give equal bits; which kernel runs, and with it the order of a row's sums, follows
-    from the number of rows of every expert.  Differentiable with respect to ``x``."""
+    from the number of pairs for each expert on average, those that go nowhere included, and from the rows that every
+    expert has.  Differentiable with respect to ``x``."""
     if not isinstance(experts, QuantizedExperts):
         raise TypeError("experts must be QuantizedExperts")
     if len(experts) != plan.n_experts:
