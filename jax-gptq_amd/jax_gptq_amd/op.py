@@ -86,9 +86,16 @@ class _QuantizedMatmulFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, y_bar):
         int_weight, zero, scale = ctx.saved_tensors
-        x_bar = _quantized_matmul_raw(y_bar.contiguous(), int_weight, zero, scale,
-                                      not ctx.transpose_b, ctx.bits, ctx.group_size)
+        # (recorded again where a graph of the gradient is asked for)
+        x_bar = _recorded_matmul(y_bar.contiguous(), int_weight, zero, scale,
+                                 not ctx.transpose_b, ctx.bits, ctx.group_size)
         return x_bar, None, None, None, None, None, None
+
+
+def _recorded_matmul(x, int_weight, zero, scale, transpose_b, bits, group_size):
+    if _differentiated(x):
+        return _QuantizedMatmulFn.apply(x, int_weight, zero, scale, transpose_b, bits, group_size)
+    return _quantized_matmul_raw(x, int_weight, zero, scale, transpose_b, bits, group_size)
 
 
 def _quantized_matmul(x, quantized_matrix, transpose_b):
@@ -102,9 +109,7 @@ def _quantized_matmul(x, quantized_matrix, transpose_b):
     if bits not in (4, 8):
         raise ValueError("quantized_matmul takes 4-bit or 8-bit codes")
     group = int(getattr(quantized_matrix, "group_size", 0) or 0)
-    if _differentiated(x):
-        return _QuantizedMatmulFn.apply(x, iw, zero, scale, bool(transpose_b), bits, group)
-    return _quantized_matmul_raw(x, iw, zero, scale, bool(transpose_b), bits, group)
+    return _recorded_matmul(x, iw, zero, scale, bool(transpose_b), bits, group)
 
 
 def quantized_matmul(x, quantized_matrix, transpose_b=False):

@@ -24,3 +24,29 @@ def test_forward_mode_is_refused(transpose):
         with pytest.raises((NotImplementedError, RuntimeError)):
             quantized_matmul(forward.make_dual(x, torch.ones_like(x)), w, transpose_b=transpose)
         assert torch.equal(quantized_matmul(x, w, transpose_b=transpose), want)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("transpose", [False, True])
+def test_a_graph_of_the_gradient_is_recorded(bits, transpose):
+    """grad(sum(grad(sum(y^2) / 2) . v)) = W W^T v, which was missing without a word beside other terms."""
+    from jax_gptq_amd.gptq import unpack_matrix
+    from jax_gptq_amd.op import quantized_matmul
+    torch.manual_seed(0)
+    w = _matrix(bits)
+    if bits == 8:
+        w.zero.fill_(128)
+        w.scale /= 16
+    dense = unpack_matrix(w).double()
+    dense = dense.t() if transpose else dense
+    x = torch.randn(5, dense.shape[0]).half().cuda().requires_grad_()
+    v = torch.randn_like(x)
+    y = quantized_matmul(x, w, transpose_b=transpose)
+    plain = torch.autograd.grad(y, x, y.detach(), retain_graph=True)[0]
+    dx = torch.autograd.grad((y.float().square() / 2).sum(), x, create_graph=True)[0]
+    assert torch.equal(plain, dx)
+    second = torch.autograd.grad((dx.float() * v.float()).sum() + x.float().sum(), x)[0]
+    want = v.double() @ dense @ dense.t() + 1
+    # two products and a sum, each rounded once to fp16 (a half step of the largest value), and what the kernels' operands
+    # leave out (2^-11 of a term): 2^-8 of the largest value covers them
+    assert (second.double() - want).abs().max() <= 2.0 ** -8 * want.abs().max()
