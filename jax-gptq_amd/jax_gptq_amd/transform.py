@@ -68,7 +68,8 @@ class _UnpackedDot(torch.autograd.Function):
         x0 = torch.zeros(ctx.x_shape, dtype=g.dtype, device=g.device, requires_grad=True)
         with torch.enable_grad():
             y = ctx.dot.evaluate(w, x0)
-        (gx,) = torch.autograd.grad(y, x0, g)      # the product is linear in x
+        # the product is linear in x; recorded where a graph of the gradient is asked for
+        (gx,) = torch.autograd.grad(y, x0, g, create_graph=torch.is_grad_enabled())
         return gx, None, None
 
 

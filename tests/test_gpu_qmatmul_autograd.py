@@ -50,3 +50,23 @@ def test_a_graph_of_the_gradient_is_recorded(bits, transpose):
     # two products and a sum, each rounded once to fp16 (a half step of the largest value), and what the kernels' operands
     # leave out (2^-11 of a term): 2^-8 of the largest value covers them
     assert (second.double() - want).abs().max() <= 2.0 ** -8 * want.abs().max()
+
+
+@pytest.mark.parametrize("remat", [False, True])
+def test_a_graph_of_the_gradient_is_recorded_by_unpacked_products(remat):
+    """The same where a model function's product unpacks the matrix, and drops it until the backward pass."""
+    from jax_gptq_amd import use_quantized
+    from jax_gptq_amd.gptq import unpack_matrix
+    torch.manual_seed(0)
+    w = _matrix()
+    dense = unpack_matrix(w).double()
+    x = torch.randn(5, dense.shape[0]).cuda().requires_grad_()
+    v = torch.randn_like(x)
+    y = use_quantized(lambda p, a: a @ p, use_kernel=False, remat_unpack=remat)(w, x)
+    plain = torch.autograd.grad(y, x, y.detach(), retain_graph=True)[0]
+    dx = torch.autograd.grad((y.square() / 2).sum(), x, create_graph=True)[0]
+    assert torch.equal(plain, dx)
+    second = torch.autograd.grad((dx * v).sum() + x.sum(), x)[0]
+    want = v.double() @ dense @ dense.t() + 1
+    # two fp32 products of 128 and 96 terms: (128 + 96) 2^-24 of the terms' sizes, well under 2^-14 of the largest value
+    assert (second.double() - want).abs().max() <= 2.0 ** -14 * want.abs().max()
