@@ -69,6 +69,28 @@ template <typename N, typename... T> std::shared_ptr<N> node_of(const T &...inpu
   return node;
 }
 SavedVariable saved(const Tensor &t) { return SavedVariable(t, false); }
+// A plan's or a stack's tensor, saved.  One that was made in inference mode cannot be: nothing counts what is written to
+// it.  It is kept as it is, so that a stack that was quantised in inference mode can be trained through.
+class Kept {
+ public:
+  void keep(const Tensor &t) {
+    if (t.is_inference()) plain = t;
+    else counted = saved(t);
+  }
+  Tensor unpack() const {
+    const Tensor t = plain.defined() ? plain : counted.unpack();
+    TORCH_CHECK(t.defined(), "a second backward pass through a graph that the first has released");
+    return t;
+  }
+  void release() {
+    plain.reset();
+    counted.reset_data();
+  }
+
+ private:
+  SavedVariable counted;
+  Tensor plain;
+};
 Tensor dense(const Tensor &t) { return t.is_contiguous() ? t : t.contiguous(); }
 
 std::tuple<Tensor, Tensor, Tensor> sort(const Tensor &ids, int64_t n_experts) {
@@ -156,18 +178,18 @@ Tensor matmul(const Tensor &x, const Product &p, at::ScalarType type);
 
 // A node that reads a plan.  apply() holds the lock: another thread may release what is saved.
 struct PlanNode : torch::autograd::Node {
-  SavedVariable position, offsets;
+  Kept position, offsets;
   int64_t top_k;
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
-    position.reset_data();
-    offsets.reset_data();
+    position.release();
+    offsets.release();
     release();
   }
   virtual void release() {}
   void keep(const Tensor &position_, const Tensor &offsets_, int64_t top_k_) {
-    position = saved(position_);
-    offsets = saved(offsets_);
+    position.keep(position_);
+    offsets.keep(offsets_);
     top_k = top_k_;
   }
 };
@@ -227,16 +249,16 @@ struct CombineGradNode : PlanNode {
 };
 
 struct MatmulNode : PlanNode {
-  SavedVariable packed, zero, scale, order;
+  Kept packed, zero, scale, order;
   int64_t bits, group;
   bool sorted_rows, transpose;
   at::ScalarType type;                 // of x
   std::string name() const override { return "ExpertMatmulBackward"; }
   void release() override {
-    packed.reset_data();
-    zero.reset_data();
-    scale.reset_data();
-    order.reset_data();
+    packed.release();
+    zero.release();
+    scale.release();
+    order.release();
   }
   variable_list apply(variable_list &&grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
@@ -296,10 +318,10 @@ Tensor matmul(const Tensor &x, const Product &p, at::ScalarType type) {
   const Tensor out = matmul_raw(x, p, type);
   if (node) {
     node->keep(p.position, p.offsets, p.top_k);
-    node->packed = saved(p.packed);
-    node->zero = saved(p.zero);
-    node->scale = saved(p.scale);
-    node->order = saved(p.order);
+    node->packed.keep(p.packed);
+    node->zero.keep(p.zero);
+    node->scale.keep(p.scale);
+    node->order.keep(p.order);
     node->bits = p.bits;
     node->group = p.group;
     node->sorted_rows = p.sorted_rows;

@@ -242,3 +242,23 @@ def test_only_the_gradients_that_are_wanted(X):
         want = want or (a.grad, b.grad)
         assert (torch.equal(a.grad, want[0]) if need_y else a.grad is None)
         assert (torch.equal(b.grad, want[1]) if need_w else b.grad is None)
+
+
+def test_a_plan_and_a_stack_made_in_inference_mode(X):
+    """They can be trained through: the gradient is that of a plan and a stack made outside of it."""
+    ids, g = ids_of(0, T, TOP_K, E).cuda(), torch.randn(T * TOP_K, N).cuda()
+    made = []
+    for mode in (False, True):
+        with torch.inference_mode(mode):
+            stack, plan = Layer(X, 1, E, K, N, 4, 64).stack, X.sort_tokens(ids, E)
+        torch.manual_seed(5)
+        x, w = torch.randn(T, K).cuda().requires_grad_(), torch.rand(T, TOP_K).cuda().requires_grad_()
+        rows = X.quantized_expert_matmul(x, stack, plan) + X.gather_tokens(x, plan)[:, :N]
+        out = X.combine_tokens(rows * g, plan, w)
+        made.append(torch.autograd.grad(out.sum(), (x, w), retain_graph=True))
+        for a, b in zip(made[-1], torch.autograd.grad(out.sum(), (x, w))):
+            assert torch.equal(a, b)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(out.sum(), (x, w))
+    for a, b in zip(*made):
+        assert torch.equal(a, b)
