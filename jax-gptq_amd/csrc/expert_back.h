@@ -51,10 +51,10 @@ constexpr int BACK_MOST = 4, BACK_MIN_STAGES = 8;
 
 // Rows of a tile, by the rows of an expert on average.  The instructions that make the operands of codes are shared by
 // its rows, so a tall tile is the faster the fuller it is.  Measured with 32 / 64 / 128 rows, us a call:
-//   8 experts 4096 x 4096, fp16:   8 rows each 47 69 77,  60: 74 76 83,  125: 150 106 131,  200: 160 141 145,
-//                                  375: 318 236 234,  512: 382 301 274
-//   64 experts 2048 x 1424, bf16:  10 rows each 55 81 124,  31: 80 88 125,  64: 126 128 130,  256: 370 342 367
-//   8 experts 4096 x 4096, fp32:   8 rows each 60 70 126,  40: 116 75 125,  162: 223 250 235,  512: 568 518 524
+//   8 experts 4096 x 4096, fp16:   8 rows each 46 68 78,  60: 75 78 87,  125: 146 112 139,  200: 180 149 154,
+//                                  375: 324 246 242,  512: 368 305 280
+//   64 experts 2048 x 1424, bf16:  10 rows each 62 94 140,  31: 89 97 141,  64: 142 146 146,  256: 390 380 412
+//   8 experts 4096 x 4096, fp32:   8 rows each 58 62 111,  40: 109 68 114,  162: 218 216 211,  512: 494 481 476
 enum BackRows { BACK_32, BACK_64, BACK_128 };
 static inline BackRows back_rows(int64_t P, int E) {
   const int64_t rows = P / E;
